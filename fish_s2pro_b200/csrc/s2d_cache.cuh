@@ -1,0 +1,89 @@
+// s2d_cache.cuh -- shared parts of the paged-cache operators (s2d_cache.cu,
+// s2d_cache_attn.cu; the interface is include/s2d_cache.h).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "../../include/s2d_cache.h"
+#include "s2d_common.cuh"
+
+namespace s2d {
+
+constexpr int kCachePage = S2D_CACHE_PAGE;
+constexpr int kCacheMaxRep = 16;
+
+__device__ __forceinline__ void cache_flag(int32_t *status, int bits) {
+    if (status) atomicOr(status, bits);
+}
+
+// Element offset of slot t's row of KV head g, page table row `table`; -1
+// (and the status bit) when the page id is outside the pool.
+__device__ __forceinline__ int64_t cache_row(const S2dCacheView &c, const int32_t *table, int g, int t) {
+    const int page = __ldg(table + t / kCachePage);
+    if ((uint32_t)page >= (uint32_t)c.n_pages) {
+        cache_flag(c.status, S2D_CACHE_BAD_PAGE);
+        return -1;
+    }
+    return (int64_t)page * c.page_stride + (int64_t)g * c.head_stride + (int64_t)(t % kCachePage) * c.head_dim;
+}
+
+// A sequence's length, held inside its page table.
+__device__ __forceinline__ int cache_length(const S2dCacheView &c, int b) {
+    const int n = __ldg(c.lengths + b), cap = c.max_pages * kCachePage;
+    if (n < 0 || n > cap) {
+        cache_flag(c.status, S2D_CACHE_BAD_LENGTH);
+        return n < 0 ? 0 : cap;
+    }
+    return n;
+}
+
+// Rows [first, first + count) of a packed batch that belong to sequence b,
+// held inside [0, tokens].
+__device__ __forceinline__ int cache_tokens(const int32_t *q_start, int tokens, int b, int &first, int32_t *status) {
+    if (!q_start) {
+        first = b;
+        return b < tokens ? 1 : 0;
+    }
+    const int t0 = __ldg(q_start + b), t1 = __ldg(q_start + b + 1);
+    if (t0 < 0 || t1 < t0 || t1 > tokens) {
+        cache_flag(status, S2D_CACHE_BAD_LENGTH);
+        first = 0;
+        return 0;
+    }
+    first = t0;
+    return t1 - t0;
+}
+
+// Runs the enclosed host code with `device` current.
+struct DeviceGuard {
+    int before = -1;
+    cudaError_t error;
+    explicit DeviceGuard(int device) {
+        error = cudaGetDevice(&before);
+        if (!error && before != device) error = cudaSetDevice(device);
+        else if (!error) before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+inline int32_t cache_fail(char *err, size_t cap, int32_t code, const char *msg) {
+    if (err && cap) snprintf(err, cap, "%s", msg);
+    return code;
+}
+inline int32_t cache_cuda(char *err, size_t cap, const char *what, cudaError_t e) {
+    if (!e) return S2D_OK;
+    if (err && cap) snprintf(err, cap, "%s: %s", what, cudaGetErrorString(e));
+    return S2D_ECUDA;
+}
+
+// nullptr if the view can be used, else what is wrong with it.
+const char *cache_view_fault(const S2dCacheView *c);
+inline bool cache_aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+
+}  // namespace s2d

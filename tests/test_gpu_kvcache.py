@@ -1,0 +1,406 @@
+"""The paged-cache operators (kvcache.py, include/s2d_cache.h) against plain 64-bit forms.
+
+Unused pages, the rows of a page past a sequence's length, and the mass and positions of free slots are NaN or nonsense in
+every case: nothing may read them into a result.
+"""
+import math
+
+import numpy as np
+import pytest
+
+import kvcache_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+PAGE = 64
+# Half a step of each type relative to a value; f32 results are held to the attention tests' 2e-5 of the largest value.
+HALF_STEP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+F32_TOL = 2e-5
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+def act_dtype(torch, ty):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[ty]
+
+
+def rounded(torch, x, dtype):
+    """float64 numpy of x rounded to dtype, and the tensor."""
+    t = torch.from_numpy(np.asarray(x, np.float32)).to(dtype)
+    return t.double().numpy(), t.cuda()
+
+
+class Case:
+    """A cache of random pages: k64 / v64 the values in float64 (NaN outside the sequences), c the PagedKvCache."""
+
+    def __init__(self, torch, ty, H, G, D, lengths, tokens=None, prefix_len=0, extra_pages=3, layered=False, spare=0, seed=0, pad=0,
+                 k_scale=1.0):
+        from fish_s2pro_b200 import PagedKvCache
+        rng = np.random.default_rng(seed + 17 * D + H)
+        self.torch, self.ty, self.H, self.G, self.D = torch, ty, H, G, D
+        self.kv = torch.bfloat16 if ty == "bf16" else torch.float16
+        B = len(lengths)
+        per = max(1, -(-max(max(lengths), 1) // PAGE)) + spare
+        n_prefix = -(-prefix_len // PAGE)
+        n_pages = B * per + n_prefix + extra_pages
+        ids = rng.permutation(n_pages)
+        self.table, self.prefix = ids[: B * per].reshape(B, per), ids[B * per: B * per + n_prefix]
+        pool = np.full((2, n_pages, G, PAGE, D), np.nan, np.float32)
+        for i in range(2):
+            for b in range(B):
+                for j in range(0, lengths[b], PAGE):
+                    m = min(PAGE, lengths[b] - j)
+                    pool[i, self.table[b, j // PAGE], :, :m] = rng.standard_normal((G, m, D)) * (k_scale if i == 0 else 1.0)
+            for j in range(0, prefix_len, PAGE):
+                m = min(PAGE, prefix_len - j)
+                pool[i, self.prefix[j // PAGE], :, :m] = rng.standard_normal((G, m, D)) * (k_scale if i == 0 else 1.0)
+        (self.k64, k), (self.v64, v) = rounded(torch, pool[0], self.kv), rounded(torch, pool[1], self.kv)
+        if layered:  # layer 1 of a pool laid out [page][layer][K | V][head][64][D]
+            big = torch.full((n_pages, 3, 2, G, PAGE, D), float("nan"), dtype=self.kv, device="cuda")
+            big[:, 1, 0], big[:, 1, 1] = k, v
+            k, v = big[:, 1, 0], big[:, 1, 1]
+        self.lengths = np.asarray(lengths, np.int32)
+        self.scale = 1 / math.sqrt(D)
+        slots = per * PAGE
+        self.mass0 = np.full((B, G, slots), np.nan, np.float32)
+        for b in range(B):
+            self.mass0[b, :, : lengths[b]] = rng.random((G, lengths[b]))
+        self.pos0 = np.broadcast_to(np.arange(slots, dtype=np.int32), (B, G, slots)).copy()
+        self.mass, self.positions = (torch.from_numpy(x.copy()).cuda() for x in (self.mass0, self.pos0))
+        self.ints = lambda x: torch.from_numpy(np.asarray(x, np.int32)).cuda()
+        self.c = PagedKvCache(k, v, self.ints(self.table), self.ints(lengths), positions=self.positions, mass=self.mass)
+        self.tokens = tokens
+        counts = [1] * B if tokens is None else tokens
+        self.starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        T = int(self.starts[-1]) + pad
+        self.q64, self.q = rounded(torch, rng.standard_normal((T, H, D)) * 2.0, act_dtype(torch, ty))
+        self.q_start = None if tokens is None else self.ints(self.starts)
+        self.prefix_len = prefix_len
+        self.prefix_pages = self.ints(self.prefix) if prefix_len else None
+
+    def attend(self, **kw):
+        return self.c.attention(self.q, q_start=self.q_start, prefix_pages=self.prefix_pages, prefix_len=self.prefix_len,
+                                return_lse=True, **kw)
+
+    def expected(self):
+        return ref.attention(self.q64, self.k64, self.v64, self.table, self.lengths, self.starts, self.scale, self.prefix, self.prefix_len)
+
+    def compare(self, out, lse, weigh=False):
+        want, want_lse, weights, spread = self.expected()
+        T = int(self.starts[-1])
+        got = out[:T].double().cpu().numpy()
+        u = HALF_STEP[self.ty]
+        # the result's rounding, the weights' rounding to the cache's type (of 16-bit queries), and the f32 sums
+        bound = u * np.abs(want[:T]) + (u * spread[:T] if self.ty != "f32" else 0) + F32_TOL * max(np.abs(self.v64[np.isfinite(self.v64)]).max(initial=0), 1e-30)
+        assert np.all(np.abs(got - want[:T]) <= bound), np.max(np.abs(got - want[:T]) / bound)
+        gl = lse[:T].double().cpu().numpy()
+        seen = np.isfinite(want_lse[:T])
+        assert np.array_equal(seen, np.isfinite(gl)) and np.all(gl[~seen] == -np.inf)
+        assert np.all(np.abs(gl[seen] - want_lse[:T][seen]) <= F32_TOL * np.maximum(1, np.abs(want_lse[:T][seen])))
+        mass = self.mass.cpu().numpy()
+        if weigh:
+            for b in range(len(self.lengths)):
+                n = self.lengths[b]
+                w = self.mass0[b, :, :n].astype(np.float64) + weights[b, :, :n]
+                assert np.all(np.abs(mass[b, :, :n] - w) <= F32_TOL * np.maximum(w, 1))
+                assert np.array_equal(mass[b, :, n:], self.mass0[b, :, n:], equal_nan=True)
+        else:
+            assert np.array_equal(mass, self.mass0, equal_nan=True)
+        self.c.check()
+
+
+ATTENTION = [  # type, H, G, D, own lengths, tokens per sequence (None: one each), prefix, padding rows
+    ("f32", 8, 2, 64, [1], None, 0, 0),
+    ("f32", 8, 2, 64, [65], None, 0, 0),
+    ("f32", 32, 8, 128, [1, 63, 64, 65, 700, 2], None, 0, 0),
+    ("f32", 32, 8, 128, [0, 5, 0, 130], None, 0, 0),       # rows that see nothing
+    ("f32", 32, 8, 128, [0, 5, 0, 130], None, 1, 0),       # the prefix alone
+    ("f16", 32, 8, 128, [33, 1, 200], None, 63, 0),
+    ("bf16", 32, 8, 128, [33, 1, 200], None, 64, 0),
+    ("bf16", 16, 2, 64, [17] * 9, None, 65, 0),
+    ("f16", 8, 8, 64, [300, 7], None, 1000, 0),            # one head per group
+    ("f32", 16, 1, 128, [90, 40, 3], None, 129, 0),        # sixteen heads per group
+    ("bf16", 6, 2, 128, [90, 40, 3], None, 129, 0),        # three heads per group
+    ("f16", 10, 2, 64, [500, 1], None, 20, 0),             # five
+    ("f16", 32, 4, 128, [1500, 4100], None, 300, 0),
+    ("bf16", 32, 8, 128, [20] * 70, None, 500, 0),         # more pooled rows than one tile
+    ("f32", 32, 8, 128, [10 + i for i in range(40)], None, 2100, 0),
+    ("f32", 32, 8, 128, [33, 2, 1, 64], [33, 2, 1, 64], 0, 0),       # fresh prompts
+    ("f32", 32, 8, 128, [70, 9, 0, 300], [30, 9, 0, 17], 100, 5),    # later chunks, a sequence without tokens, padding
+    ("f16", 32, 8, 128, [70, 9, 4, 300], [30, 9, 0, 17], 100, 3),
+    ("bf16", 16, 8, 128, [400, 260], [400, 130], 77, 0),
+    ("bf16", 8, 2, 64, [150, 2, 70], [150, 2, 1], 200, 1),
+    ("f16", 8, 1, 64, [129, 65, 1], [64, 65, 1], 0, 0),
+    ("f32", 8, 2, 64, [5, 200], [9, 200], 0, 0),           # more tokens than slots: the first four see nothing
+    ("f16", 6, 2, 128, [140, 33], [140, 33], 64, 0),       # three heads per group: tiles that cut tokens
+    ("f32", 10, 2, 128, [140, 33], [40, 33], 10, 2),
+    ("bf16", 32, 8, 128, [1000], [1000], 300, 0),
+]
+
+
+@pytest.mark.parametrize("weigh", [False, True])
+@pytest.mark.parametrize("case", range(len(ATTENTION)))
+def test_attention(torch, case, weigh):
+    ty, H, G, D, lengths, tokens, prefix, pad = ATTENTION[case]
+    s = Case(torch, ty, H, G, D, lengths, tokens, prefix, layered=case % 2 == 1, spare=case % 3, pad=pad, seed=case)
+    before = torch.full_like(s.q, 7.0)
+    out, lse = s.attend(weigh=weigh, out=before)
+    assert out is before
+    s.compare(out, lse, weigh)
+    if pad:
+        assert torch.all(out[-pad:] == 7.0)
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("tokens", [None, [3, 70]])
+def test_attention_large_scores(torch, ty, tokens):
+    """Scores of some hundreds: one position holds nearly all the weight and the running maximum climbs."""
+    s = Case(torch, ty, 8, 2, 128, [300, 200], tokens, 500, k_scale=12.0, seed=5)
+    # 2^-24 of a score of ~1,000 (base 2) is off by 6e-5 in the exponent: weights and lse to that
+    want, want_lse, _, spread = s.expected()
+    out, lse = s.attend()
+    u = HALF_STEP[ty]
+    big = np.abs(want_lse).max() / math.log(2) * 2.0 ** -21
+    bound = u * np.abs(want) + (u if ty != "f32" else 0) * spread + (big + F32_TOL) * 4.0
+    assert np.all(np.abs(out.double().cpu().numpy() - want) <= bound)
+    assert np.all(np.abs(lse.double().cpu().numpy() - want_lse) <= F32_TOL * np.abs(want_lse))
+
+
+def test_attention_tiny_and_huge_queries(torch):
+    """f32 rows whose elements are subnormal (all scores 0: the mean of v) or near the type's top."""
+    s = Case(torch, "f32", 8, 2, 64, [40, 40], None, 0, seed=9)
+    s.q[0] = 1e-42
+    s.q[1] = s.q[1] * 1e30
+    s.scale = 1e-30
+    s.q64 = s.q.double().cpu().numpy()
+    out, lse = s.attend(scale=s.scale)
+    s.compare(out, lse)
+
+
+def test_attention_nan_stays_in_its_row(torch):
+    s = Case(torch, "f32", 8, 2, 128, [70, 30], None, 40, seed=3)
+    s.q[1, 2] = float("nan")
+    out, lse = s.attend()
+    bad = torch.zeros(2, 8, dtype=torch.bool, device="cuda")
+    bad[1, 2] = True
+    assert torch.equal(torch.isnan(out).all(-1), bad) and torch.equal(torch.isnan(out).any(-1), bad)
+    assert torch.equal(torch.isnan(lse), bad)
+
+
+def test_attention_without_tokens(torch):
+    s = Case(torch, "f16", 8, 2, 64, [3, 4], [0, 0], 0)
+    out, lse = s.attend(weigh=True)
+    assert out.shape == (0, 8, 64) and np.array_equal(s.mass.cpu().numpy(), s.mass0, equal_nan=True)
+
+
+def test_attention_packed_queries_and_output(torch):
+    """q as a slice of packed QKV rows, out as a slice of wider rows."""
+    s = Case(torch, "bf16", 8, 2, 64, [50, 60], None, 70, seed=4)
+    wide = torch.zeros(2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    wide[:, 4:12] = s.q
+    to = torch.full((2, 9, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+    s.q = wide[:, 4:12]
+    out, lse = s.attend(out=to[:, 1:])
+    s.compare(out, lse)
+    assert torch.all(to[:, 0] == 3.0)
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,G,D", [(8, 2, 64), (32, 8, 128), (6, 2, 128), (16, 1, 64)])
+@pytest.mark.parametrize("tokens", [None, [1, 0, 70, 5]])
+@pytest.mark.parametrize("norm", [True, False])
+def test_append(torch, ty, H, G, D, tokens, norm):
+    from fish_s2pro_b200 import PagedKvCache
+    rng = np.random.default_rng(H + D)
+    B, per = 4, 3
+    kv = torch.bfloat16 if ty == "bf16" else torch.float16
+    past = np.array([0, 63, 100, 64], np.int32)
+    counts = [1] * B if tokens is None else tokens
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    T, pad = int(starts[-1]), 0 if tokens is None else 3
+    table = rng.permutation(B * per).reshape(B, per).astype(np.int32)
+    pos = rng.integers(0, 32768, T + pad).astype(np.int32)
+    pos[:3] = [0, 2 ** 31 - 1, -5]
+    dt = act_dtype(torch, ty)
+    (q64, q), (k64, k), (v64, v) = (rounded(torch, rng.standard_normal((T + pad, n, D)) * 1.7, dt) for n in (H, G, G))
+    gains = [(1 + 0.2 * rng.standard_normal(D)).astype(np.float32) if norm else None for _ in range(2)]
+    dev = lambda x: None if x is None else torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    kp, vp = (torch.full((B * per, G, PAGE, D), 9.0, dtype=kv, device="cuda") for _ in range(2))
+    lengths = torch.full((B,), -1, dtype=torch.int32, device="cuda")
+    positions = torch.full((B, G, per * PAGE), -7, dtype=torch.int32, device="cuda")
+    mass = torch.full((B, G, per * PAGE), 5.0, device="cuda")
+    c = PagedKvCache(kp, vp, dev(table), lengths, positions=positions, mass=mass)
+    before = torch.full_like(q, 7.0)
+    got = c.append(q, k, v, dev(pos), dev(past), q_start=None if tokens is None else dev(starts.astype(np.int32)), q_norm=dev(gains[0]),
+                   k_norm=dev(gains[1]), eps=1e-6, rope_base=1e6, out=before)
+    c.check()
+    # norm: sum of squares, rsqrt (2 ulp), two products; rotation: angle pi 2^-25 off, sines 2 ulp, two products and a sum: under
+    # 2^-20 of the pair's size in all
+    def close(got, want, u):
+        pair = np.repeat(np.sqrt(want[..., 0::2] ** 2 + want[..., 1::2] ** 2), 2, -1)
+        assert np.all(np.abs(got - want) <= 2.0 ** -20 * pair + u * np.abs(want) + 1e-30)
+    want_q, want_k = ref.rotate(q64[:T], gains[0], pos[:T], 1e-6, 1e6), ref.rotate(k64[:T], gains[1], pos[:T], 1e-6, 1e6)
+    close(got[:T].double().cpu().numpy(), want_q, HALF_STEP[ty])
+    assert torch.all(got[T:] == 7.0)
+    k_all, v_all = kp.double().cpu().numpy(), vp.double().cpu().numpy()
+    touched = np.zeros((B * per, PAGE), bool)
+    for b in range(B):
+        for i in range(counts[b]):
+            t, slot = int(starts[b]) + i, int(past[b]) + i
+            page, r = table[b, slot // PAGE], slot % PAGE
+            touched[page, r] = True
+            close(k_all[page, :, r], want_k[t], HALF_STEP["bf16" if ty == "bf16" else "f16"] + 2.0 ** -24)
+            assert np.array_equal(v_all[page, :, r], torch.from_numpy(v64[t]).to(kv).double().numpy())
+            assert torch.all(positions[b, :, slot] == int(pos[t])) and torch.all(mass[b, :, slot] == 0)
+        free = np.ones(per * PAGE, bool)
+        free[past[b]: past[b] + counts[b]] = False
+        assert torch.all(positions[b][:, dev(free)] == -7) and torch.all(mass[b][:, dev(free)] == 5.0)
+    assert np.all(k_all.transpose(0, 2, 1, 3)[~touched] == 9.0) and np.all(v_all.transpose(0, 2, 1, 3)[~touched] == 9.0)
+    assert lengths.tolist() == [int(p) + n for p, n in zip(past, counts)]
+
+
+def test_append_in_place_from_packed_rows(torch):
+    """q, k and v as slices of packed QKV rows, the queries rotated in place; no positions or mass."""
+    from fish_s2pro_b200 import PagedKvCache
+    rng = np.random.default_rng(1)
+    packed64, packed = rounded(torch, rng.standard_normal((2, 12, 64)), torch.float32)
+    kp, vp = (torch.zeros(2, 2, PAGE, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    c = PagedKvCache(kp, vp, ints(1, 0).view(2, 1), ints(0, 0))
+    q = packed[:, :8]
+    got = c.append(q, packed[:, 8:10], packed[:, 10:], ints(70, 900), ints(4, 9), out=q)
+    assert got.data_ptr() == packed.data_ptr()
+    want = ref.rotate(packed64[:, :10], None, np.array([70, 900]), 1e-6, 1e6)
+    assert np.max(np.abs(packed[:, :8].double().cpu().numpy() - want[:, :8])) < 2.0 ** -20 * 4
+    assert np.max(np.abs(kp[1, :, 4].double().cpu().numpy() - want[0, 8:])) < 2.0 ** -9
+    assert torch.equal(vp[0, :, 9], packed[1, 10:].half())
+    assert torch.equal(packed[:, 8:].double().cpu(), torch.from_numpy(packed64[:, 8:]))
+    assert c.lengths.tolist() == [5, 10]
+
+
+def evict_case(torch, lengths, budget, recent, G=3, D=64, kv="f16", seed=0, edit=None, layered=False, spare=0):
+    from fish_s2pro_b200 import PagedKvCache
+    rng = np.random.default_rng(seed)
+    dt = torch.float16 if kv == "f16" else torch.bfloat16
+    B, per = len(lengths), max(1, -(-max(lengths) // PAGE)) + spare
+    table = rng.permutation(B * per + 2)[: B * per].reshape(B, per).astype(np.int32)
+    pool = torch.randn(B * per + 2, 2, G, PAGE, D, generator=torch.Generator().manual_seed(seed)).to(dt)
+    slots = per * PAGE
+    mass = (rng.random((B, G, slots)) ** 4).astype(np.float32)
+    mass[rng.random(mass.shape) < 0.3] = 0.0  # ties
+    pos = np.stack([[rng.permutation(slots) for _ in range(G)] for _ in range(B)]).astype(np.int32)
+    if edit:
+        edit(mass, pos, rng)
+    dev = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    dpool = pool.cuda()
+    k, v = (dpool[:, 0], dpool[:, 1]) if layered else (dpool[:, 0].contiguous(), dpool[:, 1].contiguous())
+    dmass, dpos, past = dev(mass), dev(pos), torch.full((B,), -1, dtype=torch.int32, device="cuda")
+    c = PagedKvCache(k, v, dev(table), dev(np.asarray(lengths, np.int32)), positions=dpos, mass=dmass)
+    c.evict(budget, recent, past)
+    c.check()
+    want = pool.view(torch.int16).numpy().copy()
+    wm, wp = mass.copy(), pos.copy()
+    for b in range(B):
+        for g in range(G):
+            to, fro = ref.evict(pos[b, g], mass[b, g], lengths[b], budget, recent)
+            for i, j in zip(to, fro):
+                want[table[b, i // PAGE], :, g, i % PAGE] = want[table[b, j // PAGE], :, g, j % PAGE]
+                wm[b, g, i], wp[b, g, i] = wm[b, g, j], wp[b, g, j]
+    assert past.tolist() == [min(n, budget) for n in lengths]
+    assert c.lengths.tolist() == list(lengths)
+    assert np.array_equal(dpos.cpu().numpy(), wp)
+    assert np.array_equal(dmass.cpu().numpy().view(np.int32), wm.view(np.int32))
+    assert np.array_equal(k.contiguous().cpu().view(torch.int16).numpy(), want[:, 0])
+    assert np.array_equal(v.contiguous().cpu().view(torch.int16).numpy(), want[:, 1])
+
+
+def _odd_mass(mass, pos, rng):
+    flat = mass.reshape(-1)
+    for x in (np.nan, np.inf, -np.inf, -0.0, 1e-42, -1.0):
+        flat[rng.integers(0, flat.size, 40)] = x
+
+
+def _equal_mass(mass, pos, rng):
+    mass[:] = 0.25
+
+
+def _same_positions(mass, pos, rng):
+    pos[:] = 11
+
+
+EVICT = [  # lengths, budget, recent, keywords
+    ([1, 2, 0], 1, 0, {}),
+    ([1, 2, 5], 1, 1, {}),
+    ([64, 65, 63, 200], 64, 10, {}),
+    ([65], 64, 64, {}),
+    ([700, 1300, 130], 128, 32, dict(kv="bf16", D=128)),
+    ([1500, 2049], 1000, 500, dict(layered=True)),
+    ([2049] * 3, 2048, 512, dict(spare=1)),
+    ([5000], 17, 3, {}),
+    ([5000], 4990, 0, {}),
+    ([400, 900], 300, 50, dict(edit=_odd_mass)),
+    ([400, 900], 300, 0, dict(edit=_equal_mass)),
+    ([400, 900], 300, 7, dict(edit=_same_positions)),   # every slot is recent: the lowest stay
+    ([130, 700], 5000, 100, {}),                        # within the budget: untouched
+    ([9000], 4096, 1024, dict(G=2)),
+    ([33000, 20], 16384, 100, dict(G=1)),
+]
+
+
+@pytest.mark.parametrize("case", range(len(EVICT)))
+def test_evict(torch, case):
+    lengths, budget, recent, kw = EVICT[case]
+    evict_case(torch, lengths, budget, recent, seed=case, **kw)
+
+
+def test_decode_loop_keeps_its_budget(torch):
+    """append -> attention with weights -> evict over one shared prefix, step by step against the plain forms: sequences of
+    different lengths grow to the budget and stay there.  The choice of what to evict is checked on the device's own mass (the
+    reference's differs in the last bits), everything else on the reference's values."""
+    s = Case(torch, "f32", 8, 2, 64, [5, 37, 40], None, 70, spare=1, seed=21)
+    B, G, D, budget, recent = 3, 2, 64, 40, 8
+    rng = np.random.default_rng(2)
+    past = s.ints(s.lengths)
+    seen = s.lengths.astype(np.int64).copy()
+    k64, v64, pos_ref = s.k64.copy(), s.v64.copy(), s.pos0.copy()
+    for step in range(12):
+        pos = 70 + seen
+        (q64, q), (kn64, kn), (vn64, vn) = (rounded(torch, rng.standard_normal((B, n, D)), torch.float32) for n in (8, G, G))
+        have = past.cpu().numpy()
+        qr = s.c.append(q, kn, vn, s.ints(pos), past)
+        lengths = have + 1
+        assert s.c.lengths.tolist() == lengths.tolist()
+        kr = ref.rotate(kn64, None, pos, 0.0, 1e6)
+        for b in range(B):
+            page, r = s.table[b, have[b] // PAGE], have[b] % PAGE
+            k64[page, :, r], v64[page, :, r] = torch.from_numpy(kr[b]).half().double().numpy(), torch.from_numpy(vn64[b]).half().double().numpy()
+            pos_ref[b, :, have[b]] = pos[b]
+        mass = s.mass.cpu().numpy()
+        out, lse = s.c.attention(qr, prefix_pages=s.prefix_pages, prefix_len=70, weigh=True, return_lse=True)
+        want, want_lse, weights, _ = ref.attention(ref.rotate(q64, None, pos, 0.0, 1e6), k64, v64, s.table, lengths, np.arange(B + 1),
+                                                   s.scale, s.prefix, 70)
+        # keys may differ from the reference's by an f16 step where the rotation rounds the other way: 2^-10 of a key in one score
+        assert np.max(np.abs(out.double().cpu().numpy() - want)) < 2e-3
+        after = s.mass.cpu().numpy()
+        for b in range(B):
+            n = lengths[b]
+            assert np.max(np.abs(after[b, :, :n] - mass[b, :, :n] - weights[b, :, :n])) < 2e-3
+        s.c.evict(budget, recent, past)
+        for b in range(B):
+            for g in range(G):
+                to, fro = ref.evict(pos_ref[b, g], after[b, g], lengths[b], budget, recent)
+                for i, j in zip(to, fro):
+                    for x in (k64, v64):
+                        x[s.table[b, i // PAGE], g, i % PAGE] = x[s.table[b, j // PAGE], g, j % PAGE]
+                    pos_ref[b, g, i] = pos_ref[b, g, j]
+        assert past.tolist() == [min(n, budget) for n in lengths]
+        got_pos = s.positions.cpu().numpy()
+        for b in range(B):
+            n = min(lengths[b], budget)
+            assert np.array_equal(got_pos[b, :, :n], pos_ref[b, :, :n])
+        seen += 1
+    s.c.check()
