@@ -7,9 +7,10 @@
 // join by rescaling with 2^(m_i - m).  The prefix is the same for every
 // sequence, so the query rows of all sequences that share a KV head
 // (tokens * heads / kv_heads of them) are its rows together.
-#include "s2d_cache.cuh"
+#include "s2d_cache_attn.cuh"
 
 #include <math.h>
+#include <string.h>
 
 #include <algorithm>
 
@@ -56,97 +57,37 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename E>
-__device__ __forceinline__ uint32_t pack2(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <typename E>
-__device__ __forceinline__ float2 unpack2(uint32_t v);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
-}
-// (x, y) = hi + lo, both of the cache's type
-template <typename E>
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    hi = pack2<E>(x, y);
-    const float2 h = unpack2<E>(hi);
-    lo = pack2<E>(x - h.x, y - h.y);
-}
-
 __device__ __forceinline__ void store_out(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_out(__half *p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void store_out(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-// What a part (pm, pl) counts in a softmax whose maximum is m: nothing if it
-// saw no position (or only scores of -inf), all of it if its scores are NaN
-// (which fmaxf leaves out of pm), so that a NaN reaches its row.
-__device__ __forceinline__ float part_factor(float pm, float pl, float m) {
-    return pm == -INFINITY ? (pl == 0.f ? 0.f : 1.f) : exp2f(pm - m);
-}
-
-// How the call is cut up (from sizes that the host knows).
-struct AttnPlan {
-    int rep;                        // query heads per KV head
-    int prefix_tiles, prefix_splits;  // row tiles over the pooled rows; position splits
-    int own_tiles, own_splits;      // at most this many row tiles over all sequences
-    int parts;                      // prefix_splits (0 without a prefix) + own_splits
-    float *part;                    // [tokens][heads][parts][2 + head_dim]
-    float *lse2;                    // [tokens][heads], base 2 (weigh)
-};
-constexpr int kTileRows = 8;
-
-// Rows that belong to some sequence: tokens [0, this).
-__device__ __forceinline__ int real_tokens(const S2dCacheAttention &a, int n_seq) {
-    const int n = a.q_start ? __ldg(a.q_start + n_seq) : n_seq;
-    return max(0, min(n, a.tokens));
-}
-
-// The sequence and its row tile behind own tile `tile` (tiles of `rows` rows,
-// the sequences' tiles one after the other); b = -1 when there is none.
-// Called by a whole warp.
-__device__ __forceinline__ void find_tile(const S2dCacheView &c, const S2dCacheAttention &a, int rep, int rows, int &tile,
-                                          int &b) {
-    if (!a.q_start) {
-        const int per = (rep + rows - 1) / rows;
-        b = tile / per, tile %= per;
-        if (b >= min(c.n_seq, a.tokens)) b = -1;
+// All threads of the cluster's CTAs (of the CTA where it is alone).
+__device__ __forceinline__ void cluster_sync(int size) {
+    if (size == 1) {
+        __syncthreads();
         return;
     }
-    const int lane = threadIdx.x & 31;
-    for (int b0 = 0; b0 < c.n_seq; b0 += 32) {
-        int first, n = 0;
-        if (b0 + lane < c.n_seq) n = (int)(((int64_t)cache_tokens(a.q_start, a.tokens, b0 + lane, first, c.status) * rep + rows - 1) / rows);
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += x;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, sum > tile);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            tile -= __shfl_sync(0xffffffffu, sum - n, l);
-            b = b0 + l;
-            return;
-        }
-        tile -= __shfl_sync(0xffffffffu, sum, 31);
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// *p in the shared memory of CTA `rank` of the cluster
+template <typename T>
+__device__ __forceinline__ T cluster_get(const T *p, int rank, int size) {
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two words");
+    if (size == 1) return *p;
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    T v;
+    if constexpr (sizeof(T) == 4) {
+        uint32_t x;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+        memcpy(&v, &x, 4);
+    } else {
+        uint2 x;
+        asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(at) : "memory");
+        memcpy(&v, &x, 8);
     }
-    b = -1;
+    return v;
 }
 
 // The query row of a lane's MMA row (g = lane / 4), as A fragments: rows g
@@ -192,70 +133,66 @@ __device__ __forceinline__ void load_q(const Q *row, float scale, int t, uint32_
     }
 }
 
-// One block: 8 query rows (MMA rows 0-7 their values, 8-15 the remainders of
-// what the cache's type rounds: f32 queries, and the weights of every type)
-// against one split of the positions, four warps taking its 16-position
-// chunks in turn.
+// Single tokens: the rep <= 8 query heads of one (sequence, KV head) against
+// the sequence's own slots, shared by the CTAs of a cluster (chunks of 16
+// slots, contiguous ranges) and in each by four warps in turn, every warp with
+// its own two-stage copy ring.  MMA rows 0-7 hold the heads' values, rows 8-15
+// the remainders of what the cache's type rounds (f32 queries, and the weights
+// of every type), so the sums have f32's precision at no extra MMA.
+//
+// The CTAs' parts meet through distributed shared memory, together with the
+// prefix's parts from the workspace: the call needs no kernel to join them.
+// When weighing, the scores stay in shared memory until the row's sum over
+// prefix and own slots is known, and each CTA adds its slots' weights to the
+// mass: the keys are read once and no score leaves the SM.
 template <typename Q, typename E, int HD>
-__global__ void __launch_bounds__(128) part_kernel(const S2dCacheView c, const S2dCacheAttention a, const AttnPlan p) {
-    constexpr int KC = 16, NO = HD / 8, UNITS = HD / 8, PITCH = HD * 2 + 16, STAGE = 2 * KC * PITCH, NW = 4;
+__global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const S2dCacheAttention a, const AttnPlan p, int score_pitch) {
+    constexpr int KC = 16, NO = HD / 8, UNITS = HD / 8, PITCH = HD * 2 + 16, STAGE = 2 * KC * PITCH, NW = 4, R = 8;
     extern __shared__ __align__(16) uint8_t sm[];
+    __shared__ float2 s_ml[R];        // this CTA's (m, l) of each row
+    __shared__ float s_lse[R];        // lse2 of each row
+    __shared__ float s_rank[R][16];   // what each CTA's part counts, over the row's sum
+    float *s_o = reinterpret_cast<float *>(sm + NW * 2 * STAGE);  // [R][HD]: this CTA's O
+    float *s_pre = s_o + R * HD;                                  // [R][parts]: what each prefix part counts
+    float *s_score = s_pre + R * p.parts;                         // [rep][score_pitch]
     const int G = c.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
-    const int prefix_items = p.prefix_tiles * p.prefix_splits * G;
-    int item = (int)blockIdx.x;
-    const bool own = item >= prefix_items;
-    if (own) item -= prefix_items;
-    const int g = item % G;
-    item /= G;
-    const int splits = own ? p.own_splits : p.prefix_splits, split = item % splits;
-    int tile = item / splits, b = 0, first = 0, n_rows, span, limit;
-    const int32_t *table = a.prefix_pages;
-    if (own) {
-        find_tile(c, a, p.rep, kTileRows, tile, b);
-        if (b < 0) return;
-        const int nt = cache_tokens(a.q_start, a.tokens, b, first, c.status), n = cache_length(c, b);
-        table = c.page_table + (int64_t)b * c.table_stride;
-        n_rows = nt * p.rep - tile * kTileRows;
-        const int tok = tile * kTileRows + min(gl, n_rows - 1), last = tile * kTileRows + min(kTileRows, n_rows) - 1;
-        limit = max(0, n - nt + tok / p.rep + 1);
-        span = max(0, n - nt + last / p.rep + 1);
-    } else {
-        n_rows = real_tokens(a, c.n_seq) * p.rep - tile * kTileRows;
-        if (n_rows <= 0) return;
-        limit = span = a.prefix_len;
-    }
-    n_rows = min(n_rows, kTileRows);
-    const int r = tile * kTileRows + gl, tok = first + r / p.rep, head = g * p.rep + r % p.rep;
-    const bool real = gl < n_rows;
-    const int nch = (span + KC - 1) / KC, per = (nch + splits - 1) / splits;
-    const int ch0 = min(nch, split * per), ch1 = min(nch, ch0 + per);
+    const int S = p.own_splits, rank = (int)blockIdx.x % S;
+    int item = (int)blockIdx.x / S;
+    const int groups = (p.rep + R - 1) / R, grp = item % groups;  // more than 8 heads: groups of 8
+    item /= groups;
+    const int g = item % G, b = item / G;
+    const int head0 = g * p.rep + grp * R, n_rows = min(R, p.rep - grp * R);
+    const int n = cache_length(c, b), nch = (n + KC - 1) / KC, per = (nch + S - 1) / S;
+    const int ch0 = min(nch, rank * per), ch1 = min(nch, ch0 + per);
+    const int32_t *table = c.page_table + (int64_t)b * c.table_stride;
+    const bool keep = score_pitch > 0;
 
     uint8_t *ring = sm + (size_t)warp * 2 * STAGE;
     auto issue = [&](int ch, int stage) {
         uint8_t *kt = ring + (size_t)stage * STAGE, *vt = kt + KC * PITCH;
         const int64_t at = cache_row(c, table, g, ch * KC);  // a chunk never spans two pages
-        const int n = at < 0 ? 0 : min(KC, span - ch * KC);
+        const int have = at < 0 ? 0 : min(KC, n - ch * KC);
         const char *ks = static_cast<const char *>(c.k) + 2 * max(at, (int64_t)0), *vs = static_cast<const char *>(c.v) + 2 * max(at, (int64_t)0);
 #pragma unroll
         for (int i = 0; i < KC * UNITS / 32; ++i) {
             const int u = lane + 32 * i, row = u / UNITS, cc = u % UNITS;
-            const int64_t src = (int64_t)(row < n ? row : 0) * (HD * 2) + cc * 16;
-            cp_async16(kt + row * PITCH + cc * 16, ks + src, row < n);
-            cp_async16(vt + row * PITCH + cc * 16, vs + src, row < n);
+            const int64_t src = (int64_t)(row < have ? row : 0) * (HD * 2) + cc * 16;
+            cp_async16(kt + row * PITCH + cc * 16, ks + src, row < have);
+            cp_async16(vt + row * PITCH + cc * 16, vs + src, row < have);
         }
         cp_commit();
-        return n;
+        return have;
     };
+    int ch = ch0 + warp, have = 0, next = 0;
+    if (ch < ch1) have = issue(ch, 0);
     uint32_t qa[HD / 16][4];
     float qmul;
-    load_q<Q, E, HD>(real ? static_cast<const Q *>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * HD : nullptr, a.scale, t, qa, qmul);
+    load_q<Q, E, HD>(gl < n_rows ? static_cast<const Q *>(a.q) + (int64_t)b * a.q_stride + (int64_t)(head0 + gl) * HD : nullptr, a.scale, t, qa, qmul);
 
     float o[NO][4];
 #pragma unroll
     for (int j = 0; j < NO; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float mrun = -INFINITY, lrun = 0.f;
-    int ch = ch0 + warp, have = 0, next = 0;
-    if (ch < ch1) have = issue(ch, 0);
     for (int stage = 0; ch < ch1; ch += NW, stage ^= 1, have = next) {
         if (ch + NW < ch1) next = issue(ch + NW, stage ^ 1);
         else cp_commit();
@@ -273,14 +210,16 @@ __global__ void __launch_bounds__(128) part_kernel(const S2dCacheView c, const S
                 mma<E>(s[q], qa[2 * kk + 1], kf[2], kf[3]);
             }
         float x[2][2], mx = -INFINITY;
-        const int vis = min(have, limit - ch * KC);
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+        for (int q = 0; q < 2; ++q) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                x[q][e] = q * 8 + 2 * t + e < vis ? (s[q][e] + s[q][2 + e]) * qmul : -INFINITY;
+                x[q][e] = q * 8 + 2 * t + e < have ? (s[q][e] + s[q][2 + e]) * qmul : -INFINITY;
                 mx = fmaxf(mx, x[q][e]);
             }
+            if (keep && gl < n_rows)
+                *reinterpret_cast<float2 *>(s_score + gl * score_pitch + (ch - ch0) * KC + q * 8 + 2 * t) = make_float2(x[q][0], x[q][1]);
+        }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float mnew = fmaxf(mrun, mx), base = mnew == -INFINITY ? 0.f : mnew;  // nothing seen yet: all weights 0
@@ -311,11 +250,11 @@ __global__ void __launch_bounds__(128) part_kernel(const S2dCacheView c, const S
     cp_wait<0>();
     __syncthreads();
 
-    // join the warps: [warp][row][2 + HD] over the drained rings
+    // join the warps, over the drained rings: [warp][row][HD + 2]
     float *ms = reinterpret_cast<float *>(sm);
     lrun += __shfl_xor_sync(0xffffffffu, lrun, 1);
     lrun += __shfl_xor_sync(0xffffffffu, lrun, 2);
-    float *w = ms + (warp * kTileRows + gl) * (HD + 2);
+    float *w = ms + (warp * R + gl) * (HD + 2);
     if (t == 0) w[0] = mrun, w[1] = lrun;
 #pragma unroll
     for (int j = 0; j < NO; ++j) {
@@ -323,22 +262,71 @@ __global__ void __launch_bounds__(128) part_kernel(const S2dCacheView c, const S
         w[2 + j * 8 + 2 * t + 1] = o[j][1] + o[j][3];
     }
     __syncthreads();
-    const int part = own ? (p.parts - p.own_splits) + split : split;
     for (int i = threadIdx.x; i < n_rows * HD; i += 128) {
-        const int row = i / HD, d = i % HD, rr = tile * kTileRows + row;
+        const int row = i / HD, d = i % HD;
         float m = -INFINITY, l = 0.f, sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < NW; ++k) m = fmaxf(m, ms[(k * kTileRows + row) * (HD + 2)]);
+        for (int k = 0; k < NW; ++k) m = fmaxf(m, ms[(k * R + row) * (HD + 2)]);
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
-            const float *ws = ms + (k * kTileRows + row) * (HD + 2);
+            const float *ws = ms + (k * R + row) * (HD + 2);
             const float f = part_factor(ws[0], ws[1], m);
             l = fmaf(ws[1], f, l), sum = fmaf(ws[2 + d], f, sum);
         }
-        float *to = p.part + (((int64_t)(first + rr / p.rep) * a.heads + g * p.rep + rr % p.rep) * p.parts + part) * (HD + 2);
-        if (d == 0) to[0] = m, to[1] = l;
-        to[2 + d] = sum;
+        if (d == 0) s_ml[row] = make_float2(m, l);
+        s_o[row * HD + d] = sum;
     }
+    if (p.parts) grid_dep_wait();  // the prefix's parts are in the workspace
+    cluster_sync(S);
+
+    // what every part counts in the row's softmax: ranks, then prefix parts
+    for (int row = warp; row < n_rows; row += NW) {
+        const int64_t id = (int64_t)b * a.heads + head0 + row;
+        float2 mine = make_float2(-INFINITY, 0.f);
+        if (lane < S) mine = cluster_get(&s_ml[row], lane, S);
+        float m = mine.x;
+        for (int k = lane; k < p.parts; k += 32) m = fmaxf(m, __ldcg(&p.ml[id * p.parts + k]).x);
+        m = warp_max(m);
+        const float f = lane < S ? part_factor(mine.x, mine.y, m) : 0.f;
+        float l = lane < S ? f * mine.y : 0.f;
+        for (int k = lane; k < p.parts; k += 32) {
+            const float2 e = __ldcg(&p.ml[id * p.parts + k]);
+            const float fk = part_factor(e.x, e.y, m);
+            s_pre[row * p.parts + k] = fk;
+            l = fmaf(e.y, fk, l);
+        }
+        l = warp_sum(l);
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
+        if (lane < S) s_rank[row][lane] = f * inv;
+        for (int k = lane; k < p.parts; k += 32) s_pre[row * p.parts + k] *= inv;
+        if (lane == 0) {
+            const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+            s_lse[row] = l == 0.f ? 0.f : lse2;
+            if (rank == 0) {
+                if (a.lse) a.lse[id] = lse2 * kLn2;
+                if (p.lse2) p.lse2[id] = lse2;
+            }
+        }
+    }
+    __syncthreads();
+    // the outputs, shared by the ranks
+    for (int i = rank * 128 + (int)threadIdx.x; i < n_rows * HD; i += S * 128) {
+        const int row = i / HD, d = i % HD;
+        const int64_t id = (int64_t)b * a.heads + head0 + row;
+        float sum = 0.f;
+        for (int k = 0; k < S; ++k) sum = fmaf(cluster_get(&s_o[row * HD + d], k, S), s_rank[row][k], sum);
+        for (int k = 0; k < p.parts; ++k) sum = fmaf(__ldcg(p.part + (id * p.parts + k) * HD + d), s_pre[row * p.parts + k], sum);
+        store_out(static_cast<Q *>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + row) * HD + d, sum);
+    }
+    if (keep) {
+        float *mass = c.mass + ((int64_t)b * G + g) * c.max_pages * kCachePage;
+        for (int j = ch0 * KC + (int)threadIdx.x; j < min(n, ch1 * KC); j += 128) {
+            float sum = 0.f;
+            for (int row = 0; row < n_rows; ++row) sum += exp2f(s_score[row * score_pitch + j - ch0 * KC] - s_lse[row]);
+            mass[j] += sum;
+        }
+    }
+    cluster_sync(S);  // no CTA leaves while another may read its part
 }
 
 // One warp per (token, head): joins its parts in their order.
@@ -349,15 +337,15 @@ __global__ void __launch_bounds__(128) join_kernel(const S2dCacheView c, const S
     if (id >= (int64_t)real_tokens(a, c.n_seq) * a.heads) return;
     const int64_t tok = id / a.heads;
     const int head = (int)(id % a.heads);
-    const float *part = p.part + id * p.parts * (HD + 2);
+    const float2 *ml = p.ml + id * p.parts;
+    const float *part = p.part + id * p.parts * HD;
     float m = -INFINITY, l = 0.f, o[HD / 32] = {};
-    for (int k = 0; k < p.parts; ++k) m = fmaxf(m, part[k * (HD + 2)]);
+    for (int k = 0; k < p.parts; ++k) m = fmaxf(m, ml[k].x);
     for (int k = 0; k < p.parts; ++k) {
-        const float *w = part + k * (HD + 2);
-        const float f = part_factor(w[0], w[1], m);
-        l = fmaf(w[1], f, l);
+        const float f = part_factor(ml[k].x, ml[k].y, m);
+        l = fmaf(ml[k].y, f, l);
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(w[2 + lane + 32 * i], f, o[i]);
+        for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(part[k * HD + lane + 32 * i], f, o[i]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
     Q *out = static_cast<Q *>(a.out) + tok * a.out_stride + (int64_t)head * HD;
@@ -365,7 +353,7 @@ __global__ void __launch_bounds__(128) join_kernel(const S2dCacheView c, const S
     for (int i = 0; i < HD / 32; ++i) store_out(out + lane + 32 * i, o[i] * inv);
     if (lane == 0) {
         const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
-        if (a.lse) a.lse[id] = lse2 * 0.6931471805599453f;
+        if (a.lse) a.lse[id] = lse2 * kLn2;
         if (p.lse2) p.lse2[id] = lse2;
     }
 }
@@ -453,40 +441,105 @@ const char *attention_fault(const S2dCacheView *c, const S2dCacheAttention *a) {
     return nullptr;
 }
 
+constexpr int kTcTile = 256;      // query rows of a tcgen05 item
+constexpr int kMaxCluster = 8;    // CTAs that share one (sequence, KV head) of single tokens
+constexpr int kSms = 148;
+constexpr int kTokenSmemMost = 224 * 1024;
+
+// Shared memory of the token kernel: rings (16 slots x 2 stages x 4 warps of
+// K and V), the CTA's part, the factors of the prefix parts, the scores.
+size_t token_smem(const S2dCacheView &c, const AttnPlan &p, int pitch) {
+    return (size_t)4 * 2 * 2 * 16 * (c.head_dim * 2 + 16) + sizeof(float) * 8 * ((size_t)c.head_dim + p.parts) +
+           sizeof(float) * (size_t)std::min(p.rep, 8) * pitch;
+}
+// Floats between the rows of kept scores, 0 if none are kept; + 8 spreads the
+// rows over the banks.
+int score_pitch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p) {
+    if (!a.weigh || p.rep > 8) return 0;
+    const int chunks = c.max_pages * (kCachePage / 16), pitch = (chunks + p.own_splits - 1) / p.own_splits * 16 + 8;
+    return token_smem(c, p, pitch) <= (size_t)kTokenSmemMost ? pitch : 0;
+}
+
 void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, size_t &bytes) {
     p = {};
     p.rep = a.heads / c.kv_heads;
+    p.tile_rows = kTcTile;
     const int64_t rows = (int64_t)a.tokens * p.rep;
-    const int target = 2 * 148;
-    auto cut = [&](int64_t blocks, int64_t positions) {  // splits that fill the GPU, of at least 64 positions
-        const int64_t want = (target + blocks - 1) / std::max<int64_t>(blocks, 1);
-        return (int)std::max<int64_t>(1, std::min<int64_t>({want, (positions + 63) / 64, 64}));
+    // splits that give every SM an item, of at least `least` positions
+    auto cut = [&](int64_t items, int64_t positions, int64_t least) {
+        const int64_t want = kSms / std::max<int64_t>(items, 1);
+        return (int)std::max<int64_t>(1, std::min<int64_t>({want, (positions + least - 1) / least, 64}));
     };
-    if (a.prefix_len) {
-        p.prefix_tiles = (int)((rows + kTileRows - 1) / kTileRows);
-        p.prefix_splits = cut((int64_t)p.prefix_tiles * c.kv_heads, a.prefix_len);
+    const int64_t pooled = (rows + kTcTile - 1) / kTcTile;
+    if (!a.q_start) {
+        if (a.prefix_len) {
+            p.prefix_tiles = (int)pooled;
+            p.prefix_splits = cut(pooled * c.kv_heads, a.prefix_len, 128);
+        }
+        const int64_t items = (int64_t)a.tokens * c.kv_heads;
+        p.own_splits = 1;
+        while (p.own_splits < kMaxCluster && items * p.own_splits < 4 * kSms) p.own_splits *= 2;
+        p.parts = p.prefix_splits;
+    } else {
+        const int64_t own = rows / kTcTile + std::min<int64_t>(c.n_seq, rows);  // sum of ceil(rows of b / 256) is no more
+        const bool fill = own * c.kv_heads >= kSms;
+        p.own_tiles = (int)own;
+        p.own_splits = fill ? 1 : cut(own * c.kv_heads, (int64_t)c.max_pages * kCachePage, 128);
+        p.fused = a.prefix_len && fill && rows >= (int64_t)c.n_seq * kTcTile / 2;
+        if (a.prefix_len && !p.fused) {
+            p.prefix_tiles = (int)pooled;
+            p.prefix_splits = cut(pooled * c.kv_heads, a.prefix_len, 128);
+        }
+        p.parts = p.prefix_splits + p.own_splits;
+        if (p.parts == 1) p.parts = 0;  // an item sees all that its rows see
     }
-    p.own_tiles = (int)(a.q_start ? rows / kTileRows + c.n_seq : (int64_t)a.tokens * ((p.rep + kTileRows - 1) / kTileRows));
-    p.own_splits = cut((int64_t)p.own_tiles * c.kv_heads, (int64_t)c.max_pages * kCachePage);
-    p.parts = p.prefix_splits + p.own_splits;
-    const size_t part = align256(sizeof(float) * (size_t)a.tokens * a.heads * p.parts * (c.head_dim + 2));
-    bytes = part + (a.weigh ? align256(sizeof(float) * (size_t)a.tokens * a.heads) : 0);
+    size_t at = 0;
     char *w = static_cast<char *>(a.workspace);
-    p.part = reinterpret_cast<float *>(w);
-    p.lse2 = a.weigh && w ? reinterpret_cast<float *>(w + part) : nullptr;
+    auto take = [&](size_t n) {
+        char *to = w && n ? w + at : nullptr;
+        at += align256(n);
+        return to;
+    };
+    const size_t ids = (size_t)a.tokens * a.heads;
+    p.part = reinterpret_cast<float *>(take(sizeof(float) * ids * p.parts * c.head_dim));
+    p.ml = reinterpret_cast<float2 *>(take(sizeof(float2) * ids * p.parts));
+    const bool again = a.weigh && (a.q_start || !score_pitch(c, a, p));  // weights by computing the scores again
+    p.lse2 = reinterpret_cast<float *>(take(again ? sizeof(float) * ids : 0));
+    bytes = at;
+}
+
+template <typename Q, typename E, int HD>
+cudaError_t token_launch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
+    const int pitch = score_pitch(c, a, p);
+    const size_t smem = token_smem(c, p, pitch);
+    // the limit, not this call's size: calls of other threads may launch in between
+    cudaError_t e = cudaFuncSetAttribute(token_kernel<Q, E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTokenSmemMost);
+    if (e) return e;
+    const int64_t blocks = (int64_t)a.tokens * c.kv_heads * ((p.rep + 7) / 8) * p.own_splits;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(128), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.own_splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    // behind the prefix's items: may start while they end, and waits for them before it reads their parts
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = p.parts ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, token_kernel<Q, E, HD>, c, a, p, pitch);
 }
 
 template <typename Q, typename E, int HD>
 cudaError_t attention_launch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
-    const size_t smem = (size_t)4 * 2 * 2 * 16 * (HD * 2 + 16);  // also holds the join: 4 warps x 8 rows x (HD + 2) floats
-    cudaError_t e = cudaFuncSetAttribute(part_kernel<Q, E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e) return e;
-    const int64_t items = ((int64_t)p.prefix_tiles * p.prefix_splits + (int64_t)p.own_tiles * p.own_splits) * c.kv_heads;
-    if (items > 0x7fffffff) return cudaErrorInvalidValue;
-    part_kernel<Q, E, HD><<<(unsigned)items, 128, smem, s>>>(c, a, p);
-    if ((e = cudaGetLastError())) return e;
-    join_kernel<Q, HD><<<(unsigned)(((int64_t)a.tokens * a.heads + 3) / 4), 128, 0, s>>>(c, a, p);
-    if ((e = cudaGetLastError()) || !a.weigh) return e;
+    cudaError_t e = cudaSuccess;
+    if (p.prefix_tiles || p.own_tiles) e = launch_rows_tc(c, a, p, s);
+    if (!e && !a.q_start) {
+        e = token_launch<Q, E, HD>(c, a, p, s);
+    } else if (!e && p.parts) {
+        join_kernel<Q, HD><<<(unsigned)(((int64_t)a.tokens * a.heads + 3) / 4), 128, 0, s>>>(c, a, p);
+        e = cudaGetLastError();
+    }
+    if (e || !p.lse2) return e;
     weigh_kernel<Q, E, HD><<<dim3((unsigned)c.max_pages, (unsigned)c.n_seq, (unsigned)c.kv_heads), 128, 0, s>>>(c, a, p);
     return cudaGetLastError();
 }

@@ -1,0 +1,100 @@
+// s2d_cache_attn.cuh -- what the paged attention kernels share
+// (s2d_cache_attn.cu: single tokens, joining, weighing; s2d_cache_tc.cu: many
+// rows on tcgen05).
+#pragma once
+
+#include "s2d_cache.cuh"
+
+namespace s2d {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <typename E>
+__device__ __forceinline__ uint32_t pack2(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <typename E>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
+}
+// (x, y) = hi + lo, both of the cache's type
+template <typename E>
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    hi = pack2<E>(x, y);
+    const float2 h = unpack2<E>(hi);
+    lo = pack2<E>(x - h.x, y - h.y);
+}
+
+// What a part (pm, pl) counts in a softmax whose reference is m: nothing if it
+// saw no position (or only scores of -inf), all of it if its scores are NaN
+// (which fmaxf leaves out of pm), so that a NaN reaches its row.
+__device__ __forceinline__ float part_factor(float pm, float pl, float m) {
+    return pm == -INFINITY ? (pl == 0.f ? 0.f : 1.f) : exp2f(pm - m);
+}
+
+// How a call is cut up, from sizes that the host knows.  A query row is a
+// (token, query head); a row's results over a set of positions are its part:
+// (m, l) and O with l = sum 2^(s - m), O = sum 2^(s - m) v in base 2.
+struct AttnPlan {
+    int rep;                          // query heads per KV head
+    int tile_rows;                    // query rows of one item
+    int prefix_tiles, prefix_splits;  // items over the pooled rows and the prefix
+    int own_tiles, own_splits;        // at most this many row tiles over all sequences, and position splits
+    int fused;                        // own items walk the prefix too
+    int parts;                        // parts per row in the workspace; 0: items write the results
+    float *part;                      // [tokens][heads][parts][head_dim]
+    float2 *ml;                       // [tokens][heads][parts]
+    float *lse2;                      // [tokens][heads] in base 2, for the weigh kernel, or NULL
+};
+
+// Tokens that belong to some sequence: [0, this).
+__device__ __forceinline__ int real_tokens(const S2dCacheAttention &a, int n_seq) {
+    const int n = a.q_start ? __ldg(a.q_start + n_seq) : n_seq;
+    return max(0, min(n, a.tokens));
+}
+
+// The sequence and its row tile behind own tile `tile` (tiles of `rows` rows,
+// the sequences' tiles one after the other); b = -1 when there is none.
+// Called by a whole warp.
+__device__ __forceinline__ void find_tile(const S2dCacheView &c, const S2dCacheAttention &a, int rep, int rows, int &tile, int &b) {
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < c.n_seq; b0 += 32) {
+        int first, n = 0;
+        if (b0 + lane < c.n_seq) n = (int)(((int64_t)cache_tokens(a.q_start, a.tokens, b0 + lane, first, c.status) * rep + rows - 1) / rows);
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, sum > tile);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            tile -= __shfl_sync(0xffffffffu, sum - n, l);
+            b = b0 + l;
+            return;
+        }
+        tile -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    b = -1;
+}
+
+// s2d_cache_tc.cu: the items of `p` on tcgen05.
+cudaError_t launch_rows_tc(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s);
+
+}  // namespace s2d

@@ -1,0 +1,545 @@
+// s2d_cache_tc.cu -- attention of many query rows over paged keys and values
+// on tcgen05 (sm_100a): the pooled rows of a batch against the shared prefix,
+// and the rows of prompts against prefix and own pages.
+//
+// A CTA takes 256 query rows of one KV head as two tiles of 128 (the M of
+// every MMA) and walks the positions of its item in tiles of BN:
+//   S = Q K^T        both operands in shared memory, S in TMEM
+//   P = 2^(s - m)    one thread per row, S read from and P written to TMEM,
+//                    P over the columns that S leaves
+//   O += P V         P from TMEM, V from shared memory (MN-major), O in TMEM
+// The two row tiles alternate: while one is in its softmax, the tensor core
+// runs P V and the next S of the other.
+//
+// f32 queries: Q and P enter as f16 pairs hi + lo (two MMAs into one
+// accumulator, about 22 bits), BN = 64.  16-bit queries: Q as it is, P rounded
+// once to the cache's type (its relative error, half a step of that type, is
+// that of the output's own rounding), BN = 128.  Sums and maxima are f32.
+//
+// m is not the running maximum itself but a reference that follows it: it is
+// set 6 below the first tile's maximum and moves (and O is rescaled in TMEM)
+// only when a tile's maximum is more than 14 above it.  P stays below 2^14,
+// an f16, and its small entries keep their bits.
+//
+// Warps: 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (warp w owns
+// TMEM lanes 32 (w % 4) ..), 8 loads K and V pages by TMA (one page of 64
+// positions x 64 columns a box, 128-byte swizzle) into a ring of tiles,
+// 9 issues the MMAs.  Every wait is bounded; one that gives up sets the
+// status word's S2D_CACHE_ABORTED, and the CTA leaves with its TMEM freed.
+#include <cuda.h>
+
+#include "s2d_cache_attn.cuh"
+#include "s2d_tc_common.cuh"
+
+#include <type_traits>
+
+namespace s2d {
+
+namespace {
+
+constexpr int kTcThreads = 320;
+constexpr int kTcRows = 128;
+constexpr int kTcColumns = 512;
+
+// Byte offset of 16-byte chunk c of row r in a 128-byte-swizzled region.
+__device__ __forceinline__ uint32_t swizzle(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ void tma_page(void *dst, const CUtensorMap *map, int x, int g, int page, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            su32(dst)),
+        "l"(map), "r"(x), "r"(0), "r"(g), "r"(page), "r"(su32(bar))
+        : "memory");
+}
+// D += A B with A in TMEM (lane = row, two 16-bit elements per column)
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    const uint32_t z = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(z), "r"(z), "r"(z), "r"(z));
+}
+#define S2D_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define S2D_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 columns of this thread's lane; the values are there after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : S2D_R8(r, 0), S2D_R8(r, 8), S2D_R8(r, 16), S2D_R8(r, 24)
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::S2D_I8(r, 0),
+        S2D_I8(r, 8), S2D_I8(r, 16), S2D_I8(r, 24), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15};" ::S2D_I8(r, 0),
+        S2D_I8(r, 8), "r"(addr)
+        : "memory");
+}
+// 2^x on the special-function unit; results below 2^-126 are 0.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename Q, int HD>
+struct TcShape {
+    static constexpr bool kF32 = sizeof(Q) == 4;
+    static constexpr int BN = kF32 ? 64 : 128;             // positions per tile
+    static constexpr int kPages = BN / kCachePage;         // pages per tile
+    static constexpr int kHalves = HD / 64;                // 128-byte column blocks of a row
+    static constexpr int kSplit = kF32 ? 2 : 1;            // hi and lo
+    static constexpr int kQHalf = kTcRows * 128;           // one column block of one row tile
+    static constexpr int kQTile = kHalves * kSplit * kQHalf;
+    static constexpr int kKvHalf = BN * 128;               // one column block of a K or V tile
+    static constexpr int kSlot = kHalves * kKvHalf;        // a K or a V tile
+    static constexpr int kFit = (224 * 1024 - 2 * kQTile) / kSlot;
+    static constexpr int kSlots = kFit < 8 ? kFit : 8;     // K and V tiles in flight
+    static constexpr int kSmem = 2 * kQTile + kSlots * kSlot + 1024;
+    static constexpr uint32_t kO = 2 * BN;                 // TMEM: S0, S1 (BN columns each), O0, O1 (HD each)
+    static_assert(kO + 2 * HD <= kTcColumns, "TMEM columns");
+    static_assert(kSlots >= 4, "K and V of two tiles");
+};
+
+struct TcShared {
+    uint64_t full[8], empty[8], s_full[2], p_full[2], fin[2], q_full;
+    uint32_t tmem;
+    int abort;
+};
+
+template <typename Q, typename E, int HD>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    rows_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const S2dCacheView c,
+                   const S2dCacheAttention a, const AttnPlan p) {
+    using Sh = TcShape<Q, HD>;
+    constexpr int BN = Sh::BN;
+    extern __shared__ uint8_t raw[];
+    __shared__ TcShared sh;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t sbase = su32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // ---- the item: rows, positions, where the result goes (every warp alike) ----
+    const int G = c.kv_heads;
+    int item = (int)blockIdx.x;
+    const int prefix_items = p.prefix_tiles * p.prefix_splits * G;
+    const bool pooled = item < prefix_items;
+    // own tiles from the back: a sequence's later tiles see more positions
+    if (!pooled) item = p.own_tiles * p.own_splits * G - 1 - (item - prefix_items);
+    const int g = item % G;
+    item /= G;
+    const int splits = pooled ? p.prefix_splits : p.own_splits, split = item % splits;
+    int tile = item / splits, b = 0, first = 0, rows, back = 0;  // back: own slots before the first token
+    int pre0 = 0, pre1 = 0, own_span = 0;                        // prefix positions, own slots that the last row sees
+    if (pooled) {
+        rows = real_tokens(a, c.n_seq) * p.rep - tile * p.tile_rows;
+        const int tiles = (a.prefix_len + BN - 1) / BN, per = (tiles + splits - 1) / splits;
+        pre0 = min(a.prefix_len, split * per * BN), pre1 = min(a.prefix_len, pre0 + per * BN);
+    } else {
+        find_tile(c, a, p.rep, p.tile_rows, tile, b);
+        if (b < 0) return;
+        const int nt = cache_tokens(a.q_start, a.tokens, b, first, c.status);
+        back = cache_length(c, b) - nt;
+        rows = nt * p.rep - tile * p.tile_rows;
+        if (p.fused) pre1 = a.prefix_len;
+    }
+    if (rows <= 0) return;
+    rows = min(rows, p.tile_rows);
+    const int r0 = tile * p.tile_rows, nq = rows > kTcRows ? 2 : 1;
+    // own slots that rows [0, n) of the tile see together
+    auto own_seen = [&](int n) { return pooled ? 0 : max(0, back + (r0 + n - 1) / p.rep + 1); };
+    own_span = own_seen(rows);
+    int own0 = 0;
+    if (!pooled) {
+        const int tiles = (own_span + BN - 1) / BN, per = (tiles + splits - 1) / splits;
+        own0 = min(own_span, split * per * BN);
+        own_span = min(own_span, own0 + per * BN);
+    }
+    const int jp = (pre1 - pre0 + BN - 1) / BN;                    // prefix tiles, then own tiles
+    auto tiles_of = [&](int n) { return jp + max(0, (min(own_seen(n), own_span) - own0 + BN - 1) / BN); };
+    const int J1 = tiles_of(rows), J0 = nq == 2 ? tiles_of(kTcRows) : J1;
+    // positions of tile j that exist
+    auto valid_of = [&](int j) { return j < jp ? pre1 - pre0 - j * BN : own_span - own0 - (j - jp) * BN; };
+    volatile int *abort_v = &sh.abort;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < Sh::kSlots; ++i) mb_init(&sh.full[i], 1), mb_init(&sh.empty[i], 1);
+        for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_full[i], 4), mb_init(&sh.fin[i], 1);
+        mb_init(&sh.q_full, 4 * nq);
+        sh.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sh.tmem)),
+                     "r"(kTcColumns));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp == 8) {
+        // ---- loader: K then V of every tile ----
+        const int32_t *own_table = pooled ? nullptr : c.page_table + (int64_t)b * c.table_stride;
+        int ids = 0, have = -1;  // page ids 32 * have + lane of the current segment
+        int issued = 0;
+        bool ok = true, was_own = false;
+        for (int j = 0; j < J1 && ok; ++j) {
+            const bool own = j >= jp;
+            const int32_t *table = own ? own_table : a.prefix_pages;
+            if (own != was_own) have = -1, was_own = own;
+            const int page0 = own ? own0 / kCachePage + (j - jp) * Sh::kPages : pre0 / kCachePage + j * Sh::kPages;
+            const int n_pages = min(Sh::kPages, (valid_of(j) + kCachePage - 1) / kCachePage);
+            const int last = ((own ? own_span : pre1) - 1) / kCachePage;  // last page of the segment
+            int page[Sh::kPages];
+#pragma unroll
+            for (int i = 0; i < Sh::kPages; ++i) {
+                const int at = min(page0 + i, last);
+                if (at / 32 != have) {
+                    have = at / 32;
+                    ids = __ldg(table + min(have * 32 + lane, last));
+                    if ((uint32_t)ids >= (uint32_t)c.n_pages) {
+                        cache_flag(c.status, S2D_CACHE_BAD_PAGE);
+                        ids = 0;
+                    }
+                }
+                page[i] = __shfl_sync(0xffffffffu, ids, at & 31);
+            }
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv, ++issued) {
+                const int s = issued % Sh::kSlots, use = issued / Sh::kSlots;
+                if (use > 0 && !mb_wait(&sh.empty[s], (use & 1) ^ 1, abort_v)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
+                    uint8_t *slot = smem + 2 * Sh::kQTile + s * Sh::kSlot;
+                    mb_expect_tx(&sh.full[s], (uint32_t)(n_pages * Sh::kHalves * kCachePage * 128));
+#pragma unroll
+                    for (int i = 0; i < Sh::kPages; ++i)
+                        if (i < n_pages)
+#pragma unroll
+                            for (int h = 0; h < Sh::kHalves; ++h)
+                                tma_page(slot + h * Sh::kKvHalf + i * kCachePage * 128, kv ? &mv : &mk, 64 * h, g, page[i], &sh.full[s]);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) *abort_v = 1;
+        // no copy may still be landing when the CTA leaves
+        for (int i = max(0, issued - Sh::kSlots); i < issued; ++i) (void)mb_wait(&sh.full[i % Sh::kSlots], (i / Sh::kSlots) & 1, abort_v, false);
+    } else if (warp == 9) {
+        // ---- MMA issuer ----
+        constexpr uint32_t type = std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+        constexpr uint32_t id_s = idesc_f16_f32(kTcRows, BN) | type, id_o = idesc_f16_f32_bmn(kTcRows, HD) | type;
+        auto wait = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, mb_wait(bar, par, abort_v)) != 0; };
+        auto slot_wait = [&](int i) { return wait(&sh.full[i % Sh::kSlots], (uint32_t)(i / Sh::kSlots) & 1); };
+        auto slot_base = [&](int i) { return sbase + 2 * Sh::kQTile + (uint32_t)(i % Sh::kSlots) * Sh::kSlot; };
+        auto issue_s = [&](int q, int j) {
+            if (lane == 0) {
+                const uint32_t k = slot_base(2 * j), qt = sbase + (uint32_t)q * Sh::kQTile, d = tmem + (uint32_t)(q * BN);
+#pragma unroll
+                for (int part = 0; part < Sh::kSplit; ++part)
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint32_t half = (uint32_t)(kk >> 2), off = (uint32_t)((kk & 3) * 32);
+                        umma_f16(d, desc_k_sw128(qt + (uint32_t)(part * Sh::kHalves * Sh::kQHalf) + half * Sh::kQHalf + off),
+                                 desc_k_sw128(k + half * Sh::kKvHalf + off), id_s, (uint32_t)(part | kk));
+                    }
+                umma_commit(&sh.s_full[q]);
+                if (q == nq - 1) umma_commit(&sh.empty[(2 * j) % Sh::kSlots]);
+            }
+            __syncwarp();
+        };
+        bool ok = J1 > 0 && wait(&sh.q_full, 0);
+        tc_fence_after();
+        if (ok && (ok = slot_wait(0))) {
+            if (J0 > 0) issue_s(0, 0);
+            if (nq == 2) issue_s(1, 0);
+        }
+        for (int j = 0; j < J1 && ok; ++j) {
+            if (!(ok = slot_wait(2 * j + 1))) break;
+            if (valid_of(j) < BN) {
+                // rows of V past the last position hold anything: their weights are 0, and 0 times a NaN is not
+                const uint32_t v = slot_base(2 * j + 1);
+                const int n0 = valid_of(j);
+                for (int i = lane; i < (BN - n0) * 8 * Sh::kHalves; i += 32) {
+                    const int h = i / ((BN - n0) * 8), at = i % ((BN - n0) * 8);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (uint32_t)(h * Sh::kKvHalf + n0 * 128 + at * 16)), "r"(0) : "memory");
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            for (int q = 0; q < nq && ok; ++q) {
+                const int Jq = q ? J1 : J0;
+                if (j >= Jq) continue;
+                if (!(ok = wait(&sh.p_full[q], (uint32_t)j & 1))) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t v = slot_base(2 * j + 1), d = tmem + Sh::kO + (uint32_t)(q * HD), pt = tmem + (uint32_t)(q * BN);
+#pragma unroll
+                    for (int part = 0; part < Sh::kSplit; ++part)
+#pragma unroll
+                        for (int kk = 0; kk < BN / 16; ++kk)
+                            umma_ts(d, pt + (uint32_t)(part * (BN / 2) + kk * 8), desc_mn_sw128(v + (uint32_t)kk * 2048u, Sh::kKvHalf), id_o,
+                                    (uint32_t)(j | part | kk));
+                    if (j + 1 == Jq) umma_commit(&sh.fin[q]);
+                    if (q == nq - 1) umma_commit(&sh.empty[(2 * j + 1) % Sh::kSlots]);
+                }
+                __syncwarp();
+                if (j + 1 < Jq) {
+                    if (!(ok = slot_wait(2 * j + 2))) break;
+                    issue_s(q, j + 1);
+                }
+            }
+        }
+        if (!ok && J1 > 0) *abort_v = 1;
+    } else if ((warp >> 2) < nq) {
+        // ---- softmax and epilogue of row tile q: one thread per row ----
+        const int q = warp >> 2, r = 32 * (warp & 3) + lane, row = q * kTcRows + r;
+        const bool real = row < rows;
+        const int rr = r0 + (real ? row : 0), tok = first + rr / p.rep, head = g * p.rep + rr % p.rep;
+        const int Jq = q ? J1 : J0;
+        const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        // Q row: its sign takes the scale's, so that the scores' maximum is that of q . k
+        const Q *src = static_cast<const Q *>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * HD;
+        const uint32_t qdst = sbase + (uint32_t)q * Sh::kQTile;
+        float qmul = fabsf(a.scale) * kLog2e;
+        if constexpr (Sh::kF32) {
+            float amax = 0.f;
+            for (int i = 0; i < HD / 4; ++i) {
+                const float4 v = real ? reinterpret_cast<const float4 *>(src)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            }
+            int ex = 0;
+            frexpf(amax, &ex);
+            ex = max(ex, -100);
+            const float up = copysignf(ldexpf(1.f, 14 - ex), a.scale);
+            qmul *= ldexpf(1.f, ex - 14);
+            for (int i = 0; i < HD / 8; ++i) {
+                const float4 x = real ? reinterpret_cast<const float4 *>(src)[2 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 y = real ? reinterpret_cast<const float4 *>(src)[2 * i + 1] : make_float4(0.f, 0.f, 0.f, 0.f);
+                uint32_t hi[4], lo[4];
+                split2<E>(x.x * up, x.y * up, hi[0], lo[0]);
+                split2<E>(x.z * up, x.w * up, hi[1], lo[1]);
+                split2<E>(y.x * up, y.y * up, hi[2], lo[2]);
+                split2<E>(y.z * up, y.w * up, hi[3], lo[3]);
+                const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]),
+                             "r"(lo[2]), "r"(lo[3])
+                             : "memory");
+            }
+        } else {
+            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            for (int i = 0; i < HD / 8; ++i) {
+                uint4 v = real ? reinterpret_cast<const uint4 *>(src)[i] : make_uint4(0, 0, 0, 0);
+                const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
+                             : "memory");
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mb_arrive(&sh.q_full);
+
+        const int own_limit = min(pooled ? 0 : max(0, back + rr / p.rep + 1), own_span) - own0;  // own slots of the item that this row sees
+        float mref = -INFINITY, l = 0.f;
+        bool ok = true;
+        const uint32_t st = lane_t + (uint32_t)(q * BN), ot = lane_t + Sh::kO + (uint32_t)(q * HD);
+        for (int j = 0; j < Jq; ++j) {
+            ok = __all_sync(0xffffffffu, mb_wait(&sh.s_full[q], (uint32_t)j & 1, abort_v)) != 0;
+            if (!ok) break;
+            tc_fence_after();
+            const int vis = real ? (j < jp ? pre1 - pre0 - j * BN : own_limit - (j - jp) * BN) : BN;
+            const bool whole = __all_sync(0xffffffffu, vis >= BN);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < BN / 64; ++h) {
+                uint32_t s0[32], s1[32];
+                tmem_ld(st + 64 * h, s0);
+                tmem_ld(st + 64 * h + 32, s1);
+                tmem_wait_ld();
+                if (whole) {
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        m4[0] = fmaxf(m4[0], __uint_as_float(s0[i])), m4[1] = fmaxf(m4[1], __uint_as_float(s0[i + 1]));
+                        m4[2] = fmaxf(m4[2], __uint_as_float(s1[i])), m4[3] = fmaxf(m4[3], __uint_as_float(s1[i + 1]));
+                    }
+                    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (64 * h + i < vis) mx = fmaxf(mx, __uint_as_float(s0[i]));
+                        if (64 * h + 32 + i < vis) mx = fmaxf(mx, __uint_as_float(s1[i]));
+                    }
+                }
+            }
+            mx *= qmul;
+            const bool up = mx > mref + 14.f;
+            const float mnew = up ? mx - 6.f : mref;
+            const float corr = up && mref > -INFINITY ? ex2(mref - mnew) : 1.f;
+            if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                // S of this tile was issued after P V of the last one: O holds every tile before this
+#pragma unroll 1
+                for (int i = 0; i < HD; i += 32) {
+                    uint32_t o[32];
+                    tmem_ld(ot + i, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                    tmem_st32(ot + i, o);
+                }
+            }
+            l *= corr;
+            mref = mnew;
+            const float base = mref == -INFINITY ? 0.f : mref;  // nothing seen yet: weights are 0 by the mask
+            auto weight = [&](uint32_t s, int col) {
+                const float x = ex2(fmaf(__uint_as_float(s), qmul, -base));
+                return whole || col < vis ? x : 0.f;
+            };
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (Sh::kF32) {
+                uint32_t s0[32], s1[32], hi[32], lo[32];
+                tmem_ld(st, s0);
+                tmem_ld(st + 32, s1);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x0 = weight(s0[2 * i], 2 * i), x1 = weight(s0[2 * i + 1], 2 * i + 1);
+                    const float y0 = weight(s1[2 * i], 32 + 2 * i), y1 = weight(s1[2 * i + 1], 33 + 2 * i);
+                    sum[0] += x0, sum[1] += x1, sum[2] += y0, sum[3] += y1;
+                    split2<E>(x0, x1, hi[i], lo[i]);
+                    split2<E>(y0, y1, hi[16 + i], lo[16 + i]);
+                }
+                tmem_st32(st, hi);
+                tmem_st32(st + 32, lo);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {  // P of columns 32 h .. into TMEM columns 16 h .., which S has left
+                    uint32_t s0[32], w[16];
+                    tmem_ld(st + 32 * h, s0);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x0 = weight(s0[2 * i], 32 * h + 2 * i), x1 = weight(s0[2 * i + 1], 32 * h + 2 * i + 1);
+                        sum[i & 1] += x0, sum[2 + (i & 1)] += x1;
+                        w[i] = pack2<E>(x0, x1);
+                    }
+                    tmem_st16(st + 16 * h, w);
+                }
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mb_arrive(&sh.p_full[q]);
+        }
+        if (!ok) *abort_v = 1;
+        if (Jq > 0) ok = __all_sync(0xffffffffu, ok && mb_wait(&sh.fin[q], 0, abort_v)) != 0;
+        tc_fence_after();
+        if (ok) {
+            const int64_t id = (int64_t)tok * a.heads + head;
+            const bool parts = p.parts > 0;
+            const int part = pooled ? split : p.prefix_splits + split;
+            const float inv = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
+            if (real) {
+                if (parts) {
+                    p.ml[id * p.parts + part] = make_float2(mref, l);
+                } else {
+                    const float lse2 = l == 0.f ? -INFINITY : mref + log2f(l);
+                    if (a.lse) a.lse[id] = lse2 * kLn2;
+                    if (p.lse2) p.lse2[id] = lse2;
+                }
+            }
+#pragma unroll 1
+            for (int i = 0; i < HD; i += 32) {
+                uint32_t o[32];
+                if (Jq > 0) {
+                    tmem_ld(ot + i, o);  // warp-collective
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                }
+                if (!real) {
+                } else if (parts || Sh::kF32) {
+                    float *to = parts ? p.part + (id * p.parts + part) * HD + i
+                                      : reinterpret_cast<float *>(static_cast<Q *>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * HD + i);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        reinterpret_cast<float4 *>(to)[e / 4] = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                                                            __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                } else {
+                    uint4 *to = reinterpret_cast<uint4 *>(static_cast<Q *>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * HD + i);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            w[x] = pack2<E>(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv);
+                        to[e / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    __syncwarp();
+    if (threadIdx.x == 0 && *abort_v) cache_flag(c.status, S2D_CACHE_ABORTED);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcColumns));
+    }
+}
+
+// The pool as [page][head][position][element], boxes of one page's 64
+// positions x 64 elements with 128-byte swizzle.
+bool page_map(CUtensorMap *m, const S2dCacheView &c, void *base) {
+    EncodeTiled enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, kCachePage, (cuuint64_t)c.kv_heads, (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.head_dim * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[4] = {64, kCachePage, 1, 1}, one[4] = {1, 1, 1, 1};
+    return enc(m, c.type == S2D_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, one,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Q, typename E, int HD>
+cudaError_t launch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
+    CUtensorMap mk, mv;
+    if (!page_map(&mk, c, c.k) || !page_map(&mv, c, c.v)) return cudaErrorInvalidValue;
+    constexpr int smem = TcShape<Q, HD>::kSmem;
+    cudaError_t e = cudaFuncSetAttribute(rows_tc_kernel<Q, E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e) return e;
+    const int64_t items = ((int64_t)p.prefix_tiles * p.prefix_splits + (int64_t)p.own_tiles * p.own_splits) * c.kv_heads;
+    if (items > 0x7fffffff) return cudaErrorInvalidValue;
+    rows_tc_kernel<Q, E, HD><<<(unsigned)items, kTcThreads, smem, s>>>(mk, mv, c, a, p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_rows_tc(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
+    const bool wide = c.head_dim == 128;
+    if (a.type == S2D_TYPE_F32) return wide ? launch<float, __half, 128>(c, a, p, s) : launch<float, __half, 64>(c, a, p, s);
+    if (a.type == S2D_TYPE_F16) return wide ? launch<__half, __half, 128>(c, a, p, s) : launch<__half, __half, 64>(c, a, p, s);
+    return wide ? launch<__nv_bfloat16, __nv_bfloat16, 128>(c, a, p, s) : launch<__nv_bfloat16, __nv_bfloat16, 64>(c, a, p, s);
+}
+
+}  // namespace s2d

@@ -32,7 +32,7 @@ _c = ctypes
 _P = ctypes.POINTER
 PAGE = 64  # S2D_CACHE_PAGE
 S2D_EDEVICE = -6
-BAD_PAGE, BAD_LENGTH, FULL = 1, 2, 4  # bits of the status word
+BAD_PAGE, BAD_LENGTH, FULL, ABORTED = 1, 2, 4, 8  # bits of the status word
 
 
 class _View(_c.Structure):
@@ -301,5 +301,5 @@ class PagedKvCache:
         self._call(self._lib.s2d_cache_status(self._view_ref, _c.byref(bits), self._stream(), self._err, 256))
         if bits.value:
             what = [t for b, t in ((BAD_PAGE, "a page id outside the pool"), (BAD_LENGTH, "a length, past or q_start out of range"),
-                                   (FULL, "a token past the last slot of its sequence")) if bits.value & b]
+                                   (FULL, "a token past the last slot of its sequence"), (ABORTED, "a kernel gave up waiting")) if bits.value & b]
             raise S2dError(S2D_EDEVICE, "paged cache: " + ", ".join(what))

@@ -32,8 +32,9 @@
  * Errors in the arguments return S2D_EINVAL before any device work, with the
  * message in err.  What only the device can see (a page id outside the pool,
  * a length outside the page table, a sequence that is full) sets bits in the
- * view's status word; the kernels leave out the rows concerned and touch no
- * memory outside the buffers.  s2d_cache_status reads the word.
+ * view's status word; what the sequences concerned get is then unspecified,
+ * but nothing outside the buffers is touched.  s2d_cache_status reads the
+ * word.
  */
 #ifndef S2D_CACHE_H
 #define S2D_CACHE_H
@@ -55,6 +56,7 @@ extern "C" {
 #define S2D_CACHE_BAD_PAGE 1   /* a page id outside [0, n_pages)             */
 #define S2D_CACHE_BAD_LENGTH 2 /* a length, past or q_start entry out of range */
 #define S2D_CACHE_FULL 4       /* a token past the last slot of its sequence   */
+#define S2D_CACHE_ABORTED 8    /* a kernel gave up waiting: results incomplete  */
 
 typedef struct S2dCacheView {
     /* The row of (page p, KV head g, place r) starts at element
