@@ -463,7 +463,6 @@ int score_pitch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPla
 void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, size_t &bytes) {
     p = {};
     p.rep = a.heads / c.kv_heads;
-    p.tile_rows = kTcTile;
     const int64_t rows = (int64_t)a.tokens * p.rep;
     // splits that give every SM an item, of at least `least` positions
     auto cut = [&](int64_t items, int64_t positions, int64_t least) {

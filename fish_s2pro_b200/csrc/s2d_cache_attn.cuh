@@ -52,7 +52,6 @@ __device__ __forceinline__ float part_factor(float pm, float pl, float m) {
 // (m, l) and O with l = sum 2^(s - m), O = sum 2^(s - m) v in base 2.
 struct AttnPlan {
     int rep;                          // query heads per KV head
-    int tile_rows;                    // query rows of one item
     int prefix_tiles, prefix_splits;  // items over the pooled rows and the prefix
     int own_tiles, own_splits;        // at most this many row tiles over all sequences, and position splits
     int fused;                        // own items walk the prefix too

@@ -2,43 +2,50 @@
 // on tcgen05 (sm_100a): the pooled rows of a batch against the shared prefix,
 // and the rows of prompts against prefix and own pages.
 //
-// A CTA takes 256 query rows of one KV head as two tiles of 128 (the M of
-// every MMA) and walks the positions of its item in tiles of BN:
+// A CTA takes items of 256 query rows of one KV head as two tiles of 128 (the
+// M of every MMA) and walks the positions of an item in tiles of BN:
 //   S = Q K^T        both operands in shared memory, S in TMEM
-//   P = 2^(s - m)    one thread per row, S read from and P written to TMEM,
-//                    P over the columns that S leaves
+//   P = 2^(s - m)    one thread per row, S read from and P written to TMEM
 //   O += P V         P from TMEM, V from shared memory (MN-major), O in TMEM
 // The two row tiles alternate: while one is in its softmax, the tensor core
-// runs P V and the next S of the other.
+// runs the products of the other.  One CTA per SM takes items in turn, so that
+// one item's first loads run under the last one's epilogue.
+//
+// 16-bit queries: Q as it is, P rounded once to the cache's type (its relative
+// error, half a step of that type, is that of the output's own rounding),
+// BN = 128, P over the TMEM columns that S leaves.
 //
 // f32 queries: Q and P enter as f16 pairs hi + lo (two MMAs into one
-// accumulator, about 22 bits), BN = 64.  16-bit queries: Q as it is, P rounded
-// once to the cache's type (its relative error, half a step of that type, is
-// that of the output's own rounding), BN = 128.  Sums and maxima are f32.
+// accumulator, about 22 bits), BN = 64, P in columns of its own.  Every MMA
+// step of 16 positions truncates its sum to f32 (measured: 1.6e-8 of the
+// result a step, all toward zero: 3.4e-5 after 16,000 positions), so O is
+// moved every kFlush tiles into registers, where it is added with rounding.
 //
 // m is not the running maximum itself but a reference that follows it: it is
-// set 6 below the first tile's maximum and moves (and O is rescaled in TMEM)
-// only when a tile's maximum is more than 14 above it.  P stays below 2^14,
-// an f16, and its small entries keep their bits.
+// set 6 below the first tile's maximum and moves (and what is summed so far is
+// rescaled) only when a tile's maximum is more than 14 above it.  P stays
+// below 2^14, an f16, and its small entries keep their bits.
 //
 // Warps: 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (warp w owns
 // TMEM lanes 32 (w % 4) ..), 8 loads K and V pages by TMA (one page of 64
 // positions x 64 columns a box, 128-byte swizzle) into a ring of tiles,
-// 9 issues the MMAs.  Every wait is bounded; one that gives up sets the
+// 9 issues the MMAs (10 and 11 only give up registers).  Every wait is bounded; one that gives up sets the
 // status word's S2D_CACHE_ABORTED, and the CTA leaves with its TMEM freed.
 #include <cuda.h>
 
 #include "s2d_cache_attn.cuh"
 #include "s2d_tc_common.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace s2d {
 
 namespace {
 
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 384;
 constexpr int kTcRows = 128;
+constexpr int kTcItemRows = 2 * kTcRows;
 constexpr int kTcColumns = 512;
 
 // Byte offset of 16-byte chunk c of row r in a 128-byte-swizzled region.
@@ -69,6 +76,13 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[32]) {
         : S2D_R8(r, 0), S2D_R8(r, 8), S2D_R8(r, 16), S2D_R8(r, 24)
         : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : S2D_R8(r, 0), S2D_R8(r, 8)
+        : "r"(addr));
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
@@ -78,18 +92,57 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
         S2D_I8(r, 8), S2D_I8(r, 16), S2D_I8(r, 24), "r"(addr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-        "%14, %15};" ::S2D_I8(r, 0),
-        S2D_I8(r, 8), "r"(addr)
-        : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::S2D_I8(r, 0), "r"(addr) : "memory");
 }
 // 2^x on the special-function unit; results below 2^-126 are 0.
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two f32 sums or products in one instruction.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ float2 untwo(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// The maximum of N scores (NaN left out) in four chains.
+template <int N>
+__device__ __forceinline__ float max_of(const uint32_t (&s)[N]) {
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m[k] = max3(m[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+// Scores of columns [0, N) that the row does not see: -inf.
+template <int N>
+__device__ __forceinline__ void mask(uint32_t (&s)[N], int vis) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = i < vis ? s[i] : 0xff800000u;
 }
 
 template <typename Q, int HD>
@@ -106,21 +159,74 @@ struct TcShape {
     static constexpr int kFit = (224 * 1024 - 2 * kQTile) / kSlot;
     static constexpr int kSlots = kFit < 8 ? kFit : 8;     // K and V tiles in flight
     static constexpr int kSmem = 2 * kQTile + kSlots * kSlot + 1024;
+    static constexpr int kFlush = 4;                       // f32: tiles that O takes before it moves to registers
     static constexpr uint32_t kO = 2 * BN;                 // TMEM: S0, S1 (BN columns each), O0, O1 (HD each)
-    static_assert(kO + 2 * HD <= kTcColumns, "TMEM columns");
+    static constexpr uint32_t kP = kF32 ? kO + 2 * HD : 0;  // f32: P0, P1 (hi and lo, BN / 2 columns each); else P over S
+    static_assert(kP + 2 * BN <= kTcColumns && kO + 2 * HD <= kTcColumns, "TMEM columns");
     static_assert(kSlots >= 4, "K and V of two tiles");
 };
 
 struct TcShared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], fin[2], q_full;
+    uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2];
     uint32_t tmem;
     int abort;
+};
+
+// What an item is: its rows, its positions, where its results go.
+template <int BN>
+struct TcItem {
+    int g, split, b, first, rows, r0, back;  // back: own slots before the sequence's first token
+    int pre0, pre1, own0, own1;              // prefix positions and own slots of the item
+    int jp, J[2], nq;                        // prefix tiles; tiles of the row tiles; row tiles
+    bool pooled;
+
+    // own slots that rows [0, n) of the item see together
+    __device__ __forceinline__ int seen(int n, int rep) const { return pooled ? 0 : max(0, back + (r0 + n - 1) / rep + 1); }
+    // positions of tile j that exist
+    __device__ __forceinline__ int valid(int j) const { return j < jp ? pre1 - pre0 - j * BN : own1 - own0 - (j - jp) * BN; }
+
+    // false: nothing to do.  Called by whole warps.
+    __device__ bool get(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, int item) {
+        const int G = c.kv_heads, prefix_items = p.prefix_tiles * p.prefix_splits * G;
+        pooled = item < prefix_items;
+        // own tiles from the back: a sequence's later tiles see more positions
+        if (!pooled) item = p.own_tiles * p.own_splits * G - 1 - (item - prefix_items);
+        g = item % G;
+        item /= G;
+        const int splits = pooled ? p.prefix_splits : p.own_splits;
+        split = item % splits;
+        int tile = item / splits;
+        b = first = back = pre0 = pre1 = own0 = own1 = 0;
+        if (pooled) {
+            rows = real_tokens(a, c.n_seq) * p.rep - tile * kTcItemRows;
+            const int tiles = (a.prefix_len + BN - 1) / BN, per = (tiles + splits - 1) / splits;
+            pre0 = min(a.prefix_len, split * per * BN), pre1 = min(a.prefix_len, pre0 + per * BN);
+        } else {
+            find_tile(c, a, p.rep, kTcItemRows, tile, b);
+            if (b < 0) return false;
+            const int nt = cache_tokens(a.q_start, a.tokens, b, first, c.status);
+            back = cache_length(c, b) - nt;
+            rows = nt * p.rep - tile * kTcItemRows;
+            if (p.fused) pre1 = a.prefix_len;
+        }
+        if (rows <= 0) return false;
+        rows = min(rows, kTcItemRows);
+        r0 = tile * kTcItemRows, nq = rows > kTcRows ? 2 : 1;
+        if (!pooled) {
+            const int span = seen(rows, p.rep), tiles = (span + BN - 1) / BN, per = (tiles + splits - 1) / splits;
+            own0 = min(span, split * per * BN), own1 = min(span, own0 + per * BN);
+        }
+        jp = (pre1 - pre0 + BN - 1) / BN;
+        J[nq - 1] = jp + (own1 - own0 + BN - 1) / BN;
+        if (nq == 2) J[0] = jp + max(0, (min(seen(kTcRows, p.rep), own1) - own0 + BN - 1) / BN);
+        return true;
+    }
 };
 
 template <typename Q, typename E, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
     rows_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const S2dCacheView c,
-                   const S2dCacheAttention a, const AttnPlan p) {
+                   const S2dCacheAttention a, const AttnPlan p, const int items) {
     using Sh = TcShape<Q, HD>;
     constexpr int BN = Sh::BN;
     extern __shared__ uint8_t raw[];
@@ -128,54 +234,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = su32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-    // ---- the item: rows, positions, where the result goes (every warp alike) ----
-    const int G = c.kv_heads;
-    int item = (int)blockIdx.x;
-    const int prefix_items = p.prefix_tiles * p.prefix_splits * G;
-    const bool pooled = item < prefix_items;
-    // own tiles from the back: a sequence's later tiles see more positions
-    if (!pooled) item = p.own_tiles * p.own_splits * G - 1 - (item - prefix_items);
-    const int g = item % G;
-    item /= G;
-    const int splits = pooled ? p.prefix_splits : p.own_splits, split = item % splits;
-    int tile = item / splits, b = 0, first = 0, rows, back = 0;  // back: own slots before the first token
-    int pre0 = 0, pre1 = 0, own_span = 0;                        // prefix positions, own slots that the last row sees
-    if (pooled) {
-        rows = real_tokens(a, c.n_seq) * p.rep - tile * p.tile_rows;
-        const int tiles = (a.prefix_len + BN - 1) / BN, per = (tiles + splits - 1) / splits;
-        pre0 = min(a.prefix_len, split * per * BN), pre1 = min(a.prefix_len, pre0 + per * BN);
-    } else {
-        find_tile(c, a, p.rep, p.tile_rows, tile, b);
-        if (b < 0) return;
-        const int nt = cache_tokens(a.q_start, a.tokens, b, first, c.status);
-        back = cache_length(c, b) - nt;
-        rows = nt * p.rep - tile * p.tile_rows;
-        if (p.fused) pre1 = a.prefix_len;
-    }
-    if (rows <= 0) return;
-    rows = min(rows, p.tile_rows);
-    const int r0 = tile * p.tile_rows, nq = rows > kTcRows ? 2 : 1;
-    // own slots that rows [0, n) of the tile see together
-    auto own_seen = [&](int n) { return pooled ? 0 : max(0, back + (r0 + n - 1) / p.rep + 1); };
-    own_span = own_seen(rows);
-    int own0 = 0;
-    if (!pooled) {
-        const int tiles = (own_span + BN - 1) / BN, per = (tiles + splits - 1) / splits;
-        own0 = min(own_span, split * per * BN);
-        own_span = min(own_span, own0 + per * BN);
-    }
-    const int jp = (pre1 - pre0 + BN - 1) / BN;                    // prefix tiles, then own tiles
-    auto tiles_of = [&](int n) { return jp + max(0, (min(own_seen(n), own_span) - own0 + BN - 1) / BN); };
-    const int J1 = tiles_of(rows), J0 = nq == 2 ? tiles_of(kTcRows) : J1;
-    // positions of tile j that exist
-    auto valid_of = [&](int j) { return j < jp ? pre1 - pre0 - j * BN : own_span - own0 - (j - jp) * BN; };
     volatile int *abort_v = &sh.abort;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < Sh::kSlots; ++i) mb_init(&sh.full[i], 1), mb_init(&sh.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_full[i], 4), mb_init(&sh.fin[i], 1);
-        mb_init(&sh.q_full, 4 * nq);
+        for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_full[i], 4), mb_init(&sh.pv_done[i], 1), mb_init(&sh.q_full[i], 4);
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -188,272 +251,340 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    TcItem<BN> it;
 
-    if (warp == 8) {
-        // ---- loader: K then V of every tile ----
-        const int32_t *own_table = pooled ? nullptr : c.page_table + (int64_t)b * c.table_stride;
-        int ids = 0, have = -1;  // page ids 32 * have + lane of the current segment
-        int issued = 0;
-        bool ok = true, was_own = false;
-        for (int j = 0; j < J1 && ok; ++j) {
-            const bool own = j >= jp;
-            const int32_t *table = own ? own_table : a.prefix_pages;
-            if (own != was_own) have = -1, was_own = own;
-            const int page0 = own ? own0 / kCachePage + (j - jp) * Sh::kPages : pre0 / kCachePage + j * Sh::kPages;
-            const int n_pages = min(Sh::kPages, (valid_of(j) + kCachePage - 1) / kCachePage);
-            const int last = ((own ? own_span : pre1) - 1) / kCachePage;  // last page of the segment
-            int page[Sh::kPages];
-#pragma unroll
-            for (int i = 0; i < Sh::kPages; ++i) {
-                const int at = min(page0 + i, last);
-                if (at / 32 != have) {
-                    have = at / 32;
-                    ids = __ldg(table + min(have * 32 + lane, last));
-                    if ((uint32_t)ids >= (uint32_t)c.n_pages) {
-                        cache_flag(c.status, S2D_CACHE_BAD_PAGE);
-                        ids = 0;
+    // Registers: 168 a thread at launch (three warps on a scheduler); warps
+    // 8-11 give theirs to the softmax warps: 2 x 216 + 72 = 3 x 168.
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8) {
+            // ---- loader: K then V of every tile of every item ----
+            int issued = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+                if (!it.get(c, a, p, item)) continue;
+                const int32_t *own_table = c.page_table + (int64_t)it.b * c.table_stride;
+                int ids = 0, have = -1;  // page ids 32 * have + lane of the current segment
+                const int J = it.J[it.nq - 1];
+                for (int j = 0; j < J && ok; ++j) {
+                    const bool own = j >= it.jp;
+                    if (j == it.jp) have = -1;
+                    const int32_t *table = own ? own_table : a.prefix_pages;
+                    const int page0 = own ? it.own0 / kCachePage + (j - it.jp) * Sh::kPages : it.pre0 / kCachePage + j * Sh::kPages;
+                    const int n_pages = min(Sh::kPages, (it.valid(j) + kCachePage - 1) / kCachePage);
+                    const int last = ((own ? it.own1 : it.pre1) - 1) / kCachePage;  // last page of the segment
+                    int page[Sh::kPages];
+    #pragma unroll
+                    for (int i = 0; i < Sh::kPages; ++i) {
+                        const int at = min(page0 + i, last);
+                        if (at / 32 != have) {
+                            have = at / 32;
+                            ids = __ldg(table + min(have * 32 + lane, last));
+                            if ((uint32_t)ids >= (uint32_t)c.n_pages) {
+                                cache_flag(c.status, S2D_CACHE_BAD_PAGE);
+                                ids = 0;
+                            }
+                        }
+                        page[i] = __shfl_sync(0xffffffffu, ids, at & 31);
+                    }
+    #pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const int s = issued % Sh::kSlots, use = issued / Sh::kSlots;
+                        if (use > 0 && !__all_sync(0xffffffffu, mb_wait(&sh.empty[s], (use & 1) ^ 1, abort_v))) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) {
+                            uint8_t *slot = smem + 2 * Sh::kQTile + s * Sh::kSlot;
+                            mb_expect_tx(&sh.full[s], (uint32_t)(n_pages * Sh::kHalves * kCachePage * 128));
+    #pragma unroll
+                            for (int i = 0; i < Sh::kPages; ++i)
+                                if (i < n_pages)
+    #pragma unroll
+                                    for (int h = 0; h < Sh::kHalves; ++h)
+                                        tma_page(slot + h * Sh::kKvHalf + i * kCachePage * 128, kv ? &mv : &mk, 64 * h, it.g, page[i], &sh.full[s]);
+                        }
+                        __syncwarp();
+                        ++issued;
                     }
                 }
-                page[i] = __shfl_sync(0xffffffffu, ids, at & 31);
             }
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv, ++issued) {
-                const int s = issued % Sh::kSlots, use = issued / Sh::kSlots;
-                if (use > 0 && !mb_wait(&sh.empty[s], (use & 1) ^ 1, abort_v)) {
-                    ok = false;
-                    break;
-                }
+            if (!ok) *abort_v = 1;
+            // no copy may still be landing when the CTA leaves
+            for (int i = max(0, issued - Sh::kSlots); i < issued; ++i) (void)mb_wait(&sh.full[i % Sh::kSlots], (i / Sh::kSlots) & 1, abort_v, false);
+        } else if (warp == 9) {
+            // ---- MMA issuer ----
+            constexpr uint32_t type = std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t id_s = idesc_f16_f32(kTcRows, BN) | type, id_o = idesc_f16_f32_bmn(kTcRows, HD) | type;
+            auto wait = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, mb_wait(bar, par, abort_v)) != 0; };
+            auto slot_wait = [&](int i) { return wait(&sh.full[i % Sh::kSlots], (uint32_t)(i / Sh::kSlots) & 1); };
+            auto slot_base = [&](int i) { return sbase + 2 * Sh::kQTile + (uint32_t)(i % Sh::kSlots) * Sh::kSlot; };
+            int kv = 0;                // tiles of earlier items: tile j's K is load 2 (kv + j), its V the next
+            uint32_t np[2] = {0, 0};   // P tiles taken so far
+            uint32_t nitem[2] = {0, 0};
+            bool ok = true;
+            auto issue_s = [&](int q, int j) {
                 if (lane == 0) {
-                    uint8_t *slot = smem + 2 * Sh::kQTile + s * Sh::kSlot;
-                    mb_expect_tx(&sh.full[s], (uint32_t)(n_pages * Sh::kHalves * kCachePage * 128));
-#pragma unroll
-                    for (int i = 0; i < Sh::kPages; ++i)
-                        if (i < n_pages)
-#pragma unroll
-                            for (int h = 0; h < Sh::kHalves; ++h)
-                                tma_page(slot + h * Sh::kKvHalf + i * kCachePage * 128, kv ? &mv : &mk, 64 * h, g, page[i], &sh.full[s]);
+                    const int load = 2 * (kv + j);
+                    const uint32_t k = slot_base(load), qt = sbase + (uint32_t)q * Sh::kQTile, d = tmem + (uint32_t)(q * BN);
+    #pragma unroll
+                    for (int part = Sh::kSplit - 1; part >= 0; --part)  // the remainders first: their sums are small
+    #pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            const uint32_t half = (uint32_t)(kk >> 2), off = (uint32_t)((kk & 3) * 32);
+                            umma_f16(d, desc_k_sw128(qt + (uint32_t)(part * Sh::kHalves * Sh::kQHalf) + half * Sh::kQHalf + off),
+                                     desc_k_sw128(k + half * Sh::kKvHalf + off), id_s, (uint32_t)(part != Sh::kSplit - 1 || kk > 0));
+                        }
+                    umma_commit(&sh.s_full[q]);
+                    if (q == it.nq - 1) umma_commit(&sh.empty[load % Sh::kSlots]);
                 }
                 __syncwarp();
-            }
-        }
-        if (!ok) *abort_v = 1;
-        // no copy may still be landing when the CTA leaves
-        for (int i = max(0, issued - Sh::kSlots); i < issued; ++i) (void)mb_wait(&sh.full[i % Sh::kSlots], (i / Sh::kSlots) & 1, abort_v, false);
-    } else if (warp == 9) {
-        // ---- MMA issuer ----
-        constexpr uint32_t type = std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
-        constexpr uint32_t id_s = idesc_f16_f32(kTcRows, BN) | type, id_o = idesc_f16_f32_bmn(kTcRows, HD) | type;
-        auto wait = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, mb_wait(bar, par, abort_v)) != 0; };
-        auto slot_wait = [&](int i) { return wait(&sh.full[i % Sh::kSlots], (uint32_t)(i / Sh::kSlots) & 1); };
-        auto slot_base = [&](int i) { return sbase + 2 * Sh::kQTile + (uint32_t)(i % Sh::kSlots) * Sh::kSlot; };
-        auto issue_s = [&](int q, int j) {
-            if (lane == 0) {
-                const uint32_t k = slot_base(2 * j), qt = sbase + (uint32_t)q * Sh::kQTile, d = tmem + (uint32_t)(q * BN);
-#pragma unroll
-                for (int part = 0; part < Sh::kSplit; ++part)
-#pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {
-                        const uint32_t half = (uint32_t)(kk >> 2), off = (uint32_t)((kk & 3) * 32);
-                        umma_f16(d, desc_k_sw128(qt + (uint32_t)(part * Sh::kHalves * Sh::kQHalf) + half * Sh::kQHalf + off),
-                                 desc_k_sw128(k + half * Sh::kKvHalf + off), id_s, (uint32_t)(part | kk));
-                    }
-                umma_commit(&sh.s_full[q]);
-                if (q == nq - 1) umma_commit(&sh.empty[(2 * j) % Sh::kSlots]);
-            }
-            __syncwarp();
-        };
-        bool ok = J1 > 0 && wait(&sh.q_full, 0);
-        tc_fence_after();
-        if (ok && (ok = slot_wait(0))) {
-            if (J0 > 0) issue_s(0, 0);
-            if (nq == 2) issue_s(1, 0);
-        }
-        for (int j = 0; j < J1 && ok; ++j) {
-            if (!(ok = slot_wait(2 * j + 1))) break;
-            if (valid_of(j) < BN) {
-                // rows of V past the last position hold anything: their weights are 0, and 0 times a NaN is not
-                const uint32_t v = slot_base(2 * j + 1);
-                const int n0 = valid_of(j);
-                for (int i = lane; i < (BN - n0) * 8 * Sh::kHalves; i += 32) {
-                    const int h = i / ((BN - n0) * 8), at = i % ((BN - n0) * 8);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (uint32_t)(h * Sh::kKvHalf + n0 * 128 + at * 16)), "r"(0) : "memory");
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-            }
-            for (int q = 0; q < nq && ok; ++q) {
-                const int Jq = q ? J1 : J0;
-                if (j >= Jq) continue;
-                if (!(ok = wait(&sh.p_full[q], (uint32_t)j & 1))) break;
-                tc_fence_after();
+            };
+            auto issue_pv = [&](int q, int j) {
                 if (lane == 0) {
-                    const uint32_t v = slot_base(2 * j + 1), d = tmem + Sh::kO + (uint32_t)(q * HD), pt = tmem + (uint32_t)(q * BN);
-#pragma unroll
+                    const int load = 2 * (kv + j) + 1;
+                    const uint32_t v = slot_base(load), d = tmem + Sh::kO + (uint32_t)(q * HD), pt = tmem + Sh::kP + (uint32_t)(q * BN);
+                    const bool fresh = Sh::kF32 ? j % Sh::kFlush == 0 : j == 0;
+    #pragma unroll
                     for (int part = 0; part < Sh::kSplit; ++part)
-#pragma unroll
+    #pragma unroll
                         for (int kk = 0; kk < BN / 16; ++kk)
                             umma_ts(d, pt + (uint32_t)(part * (BN / 2) + kk * 8), desc_mn_sw128(v + (uint32_t)kk * 2048u, Sh::kKvHalf), id_o,
-                                    (uint32_t)(j | part | kk));
-                    if (j + 1 == Jq) umma_commit(&sh.fin[q]);
-                    if (q == nq - 1) umma_commit(&sh.empty[(2 * j + 1) % Sh::kSlots]);
+                                    (uint32_t)(!fresh || part || kk));
+                    umma_commit(&sh.pv_done[q]);
+                    if (q == it.nq - 1) umma_commit(&sh.empty[load % Sh::kSlots]);
                 }
                 __syncwarp();
-                if (j + 1 < Jq) {
-                    if (!(ok = slot_wait(2 * j + 2))) break;
-                    issue_s(q, j + 1);
+            };
+            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+                if (!it.get(c, a, p, item)) continue;
+                const int nq = it.nq, J = it.J[nq - 1];
+                for (int q = 0; q < nq && ok; ++q) {
+                    ok = wait(&sh.q_full[q], nitem[q]++ & 1);
+                    tc_fence_after();
+                    if (ok && it.J[q] > 0 && (ok = slot_wait(2 * kv))) issue_s(q, 0);
+                }
+                for (int j = 0; j < J && ok; ++j) {
+                    const int load = 2 * (kv + j) + 1;
+                    bool v_ready = false;
+                    for (int q = 0; q < nq && ok; ++q) {
+                        if (j >= it.J[q]) continue;
+                        if (!(ok = wait(&sh.p_full[q], np[q]++ & 1))) break;
+                        tc_fence_after();
+                        const bool more = j + 1 < it.J[q];
+                        // P in columns of its own: S is free, and the next S goes out before P V
+                        if (Sh::kF32 && more) {
+                            if (!(ok = slot_wait(load + 1))) break;
+                            issue_s(q, j + 1);
+                        }
+                        if (!v_ready) {
+                            if (!(ok = slot_wait(load))) break;
+                            v_ready = true;
+                            const int n0 = it.valid(j);
+                            if (n0 < BN) {
+                                // rows of V past the last position hold anything: their weights are 0, and 0 times a NaN is not
+                                const uint32_t v = slot_base(load);
+                                for (int i = lane; i < (BN - n0) * 8 * Sh::kHalves; i += 32) {
+                                    const int h = i / ((BN - n0) * 8), at = i % ((BN - n0) * 8);
+                                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (uint32_t)(h * Sh::kKvHalf + n0 * 128 + at * 16)), "r"(0) : "memory");
+                                }
+                                fence_proxy_async_smem();
+                                __syncwarp();
+                            }
+                        }
+                        issue_pv(q, j);
+                        if (!Sh::kF32 && more) {
+                            if (!(ok = slot_wait(load + 1))) break;
+                            issue_s(q, j + 1);
+                        }
+                    }
+                }
+                kv += J;
+            }
+            if (!ok) *abort_v = 1;
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // ---- softmax and epilogue of row tile q: one thread per row ----
+        const int q = warp >> 2, r = 32 * (warp & 3) + lane;
+        const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t st = lane_t + (uint32_t)(q * BN), ot = lane_t + Sh::kO + (uint32_t)(q * HD), pt = lane_t + Sh::kP + (uint32_t)(q * BN);
+        const uint32_t qdst = sbase + (uint32_t)q * Sh::kQTile;
+        uint32_t ns = 0;  // S tiles taken so far; P V tiles done are as many
+        bool ok = true;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            if (!it.get(c, a, p, item) || q >= it.nq) continue;
+            const int row = q * kTcRows + r, J = it.J[q];
+            const bool real = row < it.rows;
+            const int rr = it.r0 + (real ? row : 0), tok = it.first + rr / p.rep, head = it.g * p.rep + rr % p.rep;
+            // Q row: its sign takes the scale's, so that the scores' maximum is that of q . k
+            const Q *src = static_cast<const Q *>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * HD;
+            float qmul = fabsf(a.scale) * kLog2e;
+            if constexpr (Sh::kF32) {
+                float amax = 0.f;
+                for (int i = 0; i < HD / 4; ++i) {
+                    const float4 v = real ? reinterpret_cast<const float4 *>(src)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                }
+                int ex = 0;
+                frexpf(amax, &ex);
+                ex = max(ex, -100);
+                const float up = copysignf(ldexpf(1.f, 14 - ex), a.scale);
+                qmul *= ldexpf(1.f, ex - 14);
+                for (int i = 0; i < HD / 8; ++i) {
+                    const float4 x = real ? reinterpret_cast<const float4 *>(src)[2 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    const float4 y = real ? reinterpret_cast<const float4 *>(src)[2 * i + 1] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    uint32_t hi[4], lo[4];
+                    split2<E>(x.x * up, x.y * up, hi[0], lo[0]);
+                    split2<E>(x.z * up, x.w * up, hi[1], lo[1]);
+                    split2<E>(y.x * up, y.y * up, hi[2], lo[2]);
+                    split2<E>(y.z * up, y.w * up, hi[3], lo[3]);
+                    const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]),
+                                 "r"(lo[2]), "r"(lo[3])
+                                 : "memory");
+                }
+            } else {
+                const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 4
+                for (int i = 0; i < HD / 8; ++i) {
+                    const uint4 v = real ? reinterpret_cast<const uint4 *>(src)[i] : make_uint4(0, 0, 0, 0);
+                    const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
+                                 : "memory");
                 }
             }
-        }
-        if (!ok && J1 > 0) *abort_v = 1;
-    } else if ((warp >> 2) < nq) {
-        // ---- softmax and epilogue of row tile q: one thread per row ----
-        const int q = warp >> 2, r = 32 * (warp & 3) + lane, row = q * kTcRows + r;
-        const bool real = row < rows;
-        const int rr = r0 + (real ? row : 0), tok = first + rr / p.rep, head = g * p.rep + rr % p.rep;
-        const int Jq = q ? J1 : J0;
-        const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        // Q row: its sign takes the scale's, so that the scores' maximum is that of q . k
-        const Q *src = static_cast<const Q *>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * HD;
-        const uint32_t qdst = sbase + (uint32_t)q * Sh::kQTile;
-        float qmul = fabsf(a.scale) * kLog2e;
-        if constexpr (Sh::kF32) {
-            float amax = 0.f;
-            for (int i = 0; i < HD / 4; ++i) {
-                const float4 v = real ? reinterpret_cast<const float4 *>(src)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-            }
-            int ex = 0;
-            frexpf(amax, &ex);
-            ex = max(ex, -100);
-            const float up = copysignf(ldexpf(1.f, 14 - ex), a.scale);
-            qmul *= ldexpf(1.f, ex - 14);
-            for (int i = 0; i < HD / 8; ++i) {
-                const float4 x = real ? reinterpret_cast<const float4 *>(src)[2 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
-                const float4 y = real ? reinterpret_cast<const float4 *>(src)[2 * i + 1] : make_float4(0.f, 0.f, 0.f, 0.f);
-                uint32_t hi[4], lo[4];
-                split2<E>(x.x * up, x.y * up, hi[0], lo[0]);
-                split2<E>(x.z * up, x.w * up, hi[1], lo[1]);
-                split2<E>(y.x * up, y.y * up, hi[2], lo[2]);
-                split2<E>(y.z * up, y.w * up, hi[3], lo[3]);
-                const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]),
-                             "r"(lo[2]), "r"(lo[3])
-                             : "memory");
-            }
-        } else {
-            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-            for (int i = 0; i < HD / 8; ++i) {
-                uint4 v = real ? reinterpret_cast<const uint4 *>(src)[i] : make_uint4(0, 0, 0, 0);
-                const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
-                             : "memory");
-            }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mb_arrive(&sh.q_full);
+            qmul = fmaxf(qmul, 1e-38f);  // a masked score stays -inf when the scale is 0
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mb_arrive(&sh.q_full[q]);
 
-        const int own_limit = min(pooled ? 0 : max(0, back + rr / p.rep + 1), own_span) - own0;  // own slots of the item that this row sees
-        float mref = -INFINITY, l = 0.f;
-        bool ok = true;
-        const uint32_t st = lane_t + (uint32_t)(q * BN), ot = lane_t + Sh::kO + (uint32_t)(q * HD);
-        for (int j = 0; j < Jq; ++j) {
-            ok = __all_sync(0xffffffffu, mb_wait(&sh.s_full[q], (uint32_t)j & 1, abort_v)) != 0;
-            if (!ok) break;
-            tc_fence_after();
-            const int vis = real ? (j < jp ? pre1 - pre0 - j * BN : own_limit - (j - jp) * BN) : BN;
-            const bool whole = __all_sync(0xffffffffu, vis >= BN);
-            float mx = -INFINITY;
+            const int own_limit = min(it.pooled ? 0 : max(0, it.back + rr / p.rep + 1), it.own1) - it.own0;  // own slots of the item that this row sees
+            float mref = -INFINITY, l = 0.f;
+            float acc[Sh::kF32 ? HD : 1];
 #pragma unroll
-            for (int h = 0; h < BN / 64; ++h) {
-                uint32_t s0[32], s1[32];
-                tmem_ld(st + 64 * h, s0);
-                tmem_ld(st + 64 * h + 32, s1);
-                tmem_wait_ld();
-                if (whole) {
-                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int i = 0; i < (Sh::kF32 ? HD : 1); ++i) acc[i] = 0.f;
+            // acc += O (f32), once P V of the last tile is done
+            auto flush = [&](bool clear) {
+                if constexpr (Sh::kF32) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        m4[0] = fmaxf(m4[0], __uint_as_float(s0[i])), m4[1] = fmaxf(m4[1], __uint_as_float(s0[i + 1]));
-                        m4[2] = fmaxf(m4[2], __uint_as_float(s1[i])), m4[3] = fmaxf(m4[3], __uint_as_float(s1[i + 1]));
+                    for (int i = 0; i < HD; i += 32) {
+                        uint32_t o[32];
+                        tmem_ld(ot + i, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) acc[i + e] += __uint_as_float(o[e]);
+                        if (clear) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = 0;
+                            tmem_st32(ot + i, o);
+                        }
                     }
-                    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                }
+            };
+            for (int j = 0; j < J; ++j, ++ns) {
+                ok = __all_sync(0xffffffffu, mb_wait(&sh.s_full[q], ns & 1, abort_v)) != 0;
+                if (!ok) break;
+                tc_fence_after();
+                const int vis = !real ? BN : j < it.jp ? it.pre1 - it.pre0 - j * BN : own_limit - (j - it.jp) * BN;
+                const bool whole = __all_sync(0xffffffffu, vis >= BN);
+                uint32_t s[Sh::kF32 ? 32 : BN];
+                float mx;
+                if constexpr (Sh::kF32) {
+                    tmem_ld(st, s);
+                    tmem_wait_ld();
+                    if (!whole) mask(s, vis);
+                    mx = max_of(s);
+                    tmem_ld(st + 32, s);
+                    tmem_wait_ld();
+                    if (!whole) mask(s, vis - 32);
+                    mx = fmaxf(mx, max_of(s));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (64 * h + i < vis) mx = fmaxf(mx, __uint_as_float(s0[i]));
-                        if (64 * h + 32 + i < vis) mx = fmaxf(mx, __uint_as_float(s1[i]));
-                    }
+                    for (int h = 0; h < BN / 32; ++h) tmem_ld(st + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * h]));
+                    tmem_wait_ld();
+                    if (!whole) mask(s, vis);
+                    mx = max_of(s);
                 }
-            }
-            mx *= qmul;
-            const bool up = mx > mref + 14.f;
-            const float mnew = up ? mx - 6.f : mref;
-            const float corr = up && mref > -INFINITY ? ex2(mref - mnew) : 1.f;
-            if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-                // S of this tile was issued after P V of the last one: O holds every tile before this
+                mx *= qmul;
+                const bool up = mx > mref + 14.f;
+                const float mnew = up ? mx - 6.f : mref;
+                const float corr = up && mref > -INFINITY ? ex2(mref - mnew) : 1.f;
+                const bool rescale = j > 0 && __any_sync(0xffffffffu, corr != 1.f);
+                if (j > 0) {
+                    // P and O are free once P V of the last tile is done
+                    ok = __all_sync(0xffffffffu, mb_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v)) != 0;
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                if constexpr (Sh::kF32) {
+                    if (j > 0 && (rescale || j % Sh::kFlush == 0)) flush(j % Sh::kFlush != 0);
+                    if (rescale) {
+#pragma unroll
+                        for (int i = 0; i < HD; ++i) acc[i] *= corr;
+                    }
+                } else if (rescale) {
 #pragma unroll 1
-                for (int i = 0; i < HD; i += 32) {
-                    uint32_t o[32];
-                    tmem_ld(ot + i, o);
-                    tmem_wait_ld();
+                    for (int i = 0; i < HD; i += 32) {
+                        uint32_t o[32];
+                        tmem_ld(ot + i, o);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                    tmem_st32(ot + i, o);
-                }
-            }
-            l *= corr;
-            mref = mnew;
-            const float base = mref == -INFINITY ? 0.f : mref;  // nothing seen yet: weights are 0 by the mask
-            auto weight = [&](uint32_t s, int col) {
-                const float x = ex2(fmaf(__uint_as_float(s), qmul, -base));
-                return whole || col < vis ? x : 0.f;
-            };
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (Sh::kF32) {
-                uint32_t s0[32], s1[32], hi[32], lo[32];
-                tmem_ld(st, s0);
-                tmem_ld(st + 32, s1);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float x0 = weight(s0[2 * i], 2 * i), x1 = weight(s0[2 * i + 1], 2 * i + 1);
-                    const float y0 = weight(s1[2 * i], 32 + 2 * i), y1 = weight(s1[2 * i + 1], 33 + 2 * i);
-                    sum[0] += x0, sum[1] += x1, sum[2] += y0, sum[3] += y1;
-                    split2<E>(x0, x1, hi[i], lo[i]);
-                    split2<E>(y0, y1, hi[16 + i], lo[16 + i]);
-                }
-                tmem_st32(st, hi);
-                tmem_st32(st + 32, lo);
-            } else {
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {  // P of columns 32 h .. into TMEM columns 16 h .., which S has left
-                    uint32_t s0[32], w[16];
-                    tmem_ld(st + 32 * h, s0);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float x0 = weight(s0[2 * i], 32 * h + 2 * i), x1 = weight(s0[2 * i + 1], 32 * h + 2 * i + 1);
-                        sum[i & 1] += x0, sum[2 + (i & 1)] += x1;
-                        w[i] = pack2<E>(x0, x1);
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                        tmem_st32(ot + i, o);
                     }
-                    tmem_st16(st + 16 * h, w);
                 }
+                l *= corr;
+                mref = mnew;
+                const float base = mref == -INFINITY ? 0.f : mref;  // nothing seen yet: every score is -inf
+                const uint64_t qm2 = two(qmul, qmul), nb2 = two(-base, -base);
+                uint64_t sum[2] = {0, 0};
+                if constexpr (Sh::kF32) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t x[16], hi[8], lo[8];
+                        tmem_ld16(st + 16 * h, x);
+                        tmem_wait_ld();
+                        if (!whole) mask(x, vis - 16 * h);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float2 y = untwo(fma2(two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), qm2, nb2));
+                            const float w0 = ex2(y.x), w1 = ex2(y.y);
+                            sum[i & 1] = add2(sum[i & 1], two(w0, w1));
+                            split2<E>(w0, w1, hi[i], lo[i]);
+                        }
+                        tmem_st8(pt + 8 * h, hi);
+                        tmem_st8(pt + BN / 2 + 8 * h, lo);
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < BN / 64; ++h) {  // P of columns 64 h .. into TMEM columns 32 h ..: all of S has been read
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float2 y = untwo(fma2(two(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1])), qm2, nb2));
+                            const float w0 = ex2(y.x), w1 = ex2(y.y);
+                            sum[i & 1] = add2(sum[i & 1], two(w0, w1));
+                            w[i] = pack2<E>(w0, w1);
+                        }
+                        tmem_st32(pt + 32 * h, w);
+                    }
+                }
+                const float2 total = untwo(add2(sum[0], sum[1]));
+                l += total.x + total.y;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&sh.p_full[q]);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mb_arrive(&sh.p_full[q]);
-        }
-        if (!ok) *abort_v = 1;
-        if (Jq > 0) ok = __all_sync(0xffffffffu, ok && mb_wait(&sh.fin[q], 0, abort_v)) != 0;
-        tc_fence_after();
-        if (ok) {
+            if (ok && J > 0) ok = __all_sync(0xffffffffu, mb_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v)) != 0;
+            if (!ok) break;
+            tc_fence_after();
+            if (J > 0) flush(false);
             const int64_t id = (int64_t)tok * a.heads + head;
             const bool parts = p.parts > 0;
-            const int part = pooled ? split : p.prefix_splits + split;
+            const int part = it.pooled ? it.split : p.prefix_splits + it.split;
             const float inv = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
             if (real) {
                 if (parts) {
@@ -464,43 +595,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (p.lse2) p.lse2[id] = lse2;
                 }
             }
-#pragma unroll 1
+            float *to_part = p.part + (id * p.parts + part) * HD;
+            Q *to_out = static_cast<Q *>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * HD;
+#pragma unroll
             for (int i = 0; i < HD; i += 32) {
-                uint32_t o[32];
-                if (Jq > 0) {
-                    tmem_ld(ot + i, o);  // warp-collective
-                    tmem_wait_ld();
-                } else {
+                float o[32];
+                if constexpr (Sh::kF32) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                    for (int e = 0; e < 32; ++e) o[e] = acc[i + e] * inv;
+                } else {
+                    uint32_t raw_o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) raw_o[e] = 0;
+                    if (J > 0) {
+                        tmem_ld(ot + i, raw_o);  // warp-collective
+                        tmem_wait_ld();
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(raw_o[e]) * inv;
                 }
-                if (!real) {
-                } else if (parts || Sh::kF32) {
-                    float *to = parts ? p.part + (id * p.parts + part) * HD + i
-                                      : reinterpret_cast<float *>(static_cast<Q *>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * HD + i);
+                if (real) {
+                    if (parts || Sh::kF32) {
+                        float4 *to = reinterpret_cast<float4 *>(parts ? to_part + i : reinterpret_cast<float *>(to_out + i));
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        reinterpret_cast<float4 *>(to)[e / 4] = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                                                                            __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-                } else {
-                    uint4 *to = reinterpret_cast<uint4 *>(static_cast<Q *>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * HD + i);
+                        for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    } else {
+                        uint4 *to = reinterpret_cast<uint4 *>(to_out + i);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            w[x] = pack2<E>(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv);
-                        to[e / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int e = 0; e < 4; ++e)
+                            to[e] = make_uint4(pack2<E>(o[8 * e], o[8 * e + 1]), pack2<E>(o[8 * e + 2], o[8 * e + 3]), pack2<E>(o[8 * e + 4], o[8 * e + 5]),
+                                               pack2<E>(o[8 * e + 6], o[8 * e + 7]));
                     }
                 }
                 __syncwarp();
             }
         }
+        if (!ok) *abort_v = 1;
     }
     __syncwarp();
-    if (threadIdx.x == 0 && *abort_v) cache_flag(c.status, S2D_CACHE_ABORTED);
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *abort_v) cache_flag(c.status, S2D_CACHE_ABORTED);
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcColumns));
@@ -528,8 +663,10 @@ cudaError_t launch(const S2dCacheView &c, const S2dCacheAttention &a, const Attn
     cudaError_t e = cudaFuncSetAttribute(rows_tc_kernel<Q, E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e) return e;
     const int64_t items = ((int64_t)p.prefix_tiles * p.prefix_splits + (int64_t)p.own_tiles * p.own_splits) * c.kv_heads;
-    if (items > 0x7fffffff) return cudaErrorInvalidValue;
-    rows_tc_kernel<Q, E, HD><<<(unsigned)items, kTcThreads, smem, s>>>(mk, mv, c, a, p);
+    if (items > 0x7fffffff - 1024) return cudaErrorInvalidValue;
+    int sms = 0;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device))) return e;
+    rows_tc_kernel<Q, E, HD><<<(unsigned)std::min<int64_t>(items, sms), kTcThreads, smem, s>>>(mk, mv, c, a, p, (int)items);
     return cudaGetLastError();
 }
 
