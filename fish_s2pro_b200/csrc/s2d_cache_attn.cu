@@ -502,6 +502,7 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
     const size_t ids = (size_t)a.tokens * a.heads;
     p.part = reinterpret_cast<float *>(take(sizeof(float) * ids * p.parts * c.head_dim));
     p.ml = reinterpret_cast<float2 *>(take(sizeof(float2) * ids * p.parts));
+    p.next_item = reinterpret_cast<int *>(take(p.prefix_tiles || p.own_tiles ? sizeof(int) : 0));
     const bool again = a.weigh && (a.q_start || !score_pitch(c, a, p));  // weights by computing the scores again
     p.lse2 = reinterpret_cast<float *>(take(again ? sizeof(float) * ids : 0));
     bytes = at;

@@ -58,6 +58,7 @@ struct AttnPlan {
     int parts;                        // parts per row in the workspace; 0: items write the results
     float *part;                      // [tokens][heads][parts][head_dim]
     float2 *ml;                       // [tokens][heads][parts]
+    int *next_item;                   // what the tcgen05 CTAs draw further items from
     float *lse2;                      // [tokens][heads] in base 2, for the weigh kernel, or NULL
 };
 

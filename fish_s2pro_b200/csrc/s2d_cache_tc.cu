@@ -3,21 +3,19 @@
 // and the rows of prompts against prefix and own pages.
 //
 // A CTA takes items of 256 query rows of one KV head as two tiles of 128 (the
-// M of every MMA) and walks the positions of an item in tiles of BN:
+// M of every MMA) and walks the positions of an item in tiles of 128:
 //   S = Q K^T        both operands in shared memory, S in TMEM
-//   P = 2^(s - m)    one thread per row, S read from and P written to TMEM
+//   P = 2^(s - m)    one thread per row, S read from TMEM, P written over it
 //   O += P V         P from TMEM, V from shared memory (MN-major), O in TMEM
 // The two row tiles alternate: while one is in its softmax, the tensor core
-// runs the products of the other.  One CTA per SM takes items in turn, so that
-// one item's first loads run under the last one's epilogue.
+// runs the products of the other.  One CTA per SM draws items from a counter,
+// the longest first; one item's first loads run under the last one's epilogue.
 //
 // 16-bit queries: Q as it is, P rounded once to the cache's type (its relative
-// error, half a step of that type, is that of the output's own rounding),
-// BN = 128, P over the TMEM columns that S leaves.
+// error, half a step of that type, is that of the output's own rounding).
 //
 // f32 queries: Q and P enter as f16 pairs hi + lo (two MMAs into one
-// accumulator, about 22 bits), BN = 64, P in columns of its own.  Every MMA
-// step of 16 positions truncates its sum to f32 (measured: 1.6e-8 of the
+// accumulator, about 22 bits).  Every MMA step of 16 positions truncates its sum to f32 (measured: 1.6e-8 of the
 // result a step, all toward zero: 3.4e-5 after 16,000 positions), so O is
 // moved every kFlush tiles into registers, where it is added with rounding.
 //
@@ -58,16 +56,44 @@ __device__ __forceinline__ void tma_page(void *dst, const CUtensorMap *map, int 
         "l"(map), "r"(x), "r"(0), "r"(g), "r"(page), "r"(su32(bar))
         : "memory");
 }
-// D += A B with A in TMEM (lane = row, two 16-bit elements per column)
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    const uint32_t z = 0;
+// D (+)= A B, A and B in shared memory, by the thread whose `one` is set.  The
+// whole warp runs the instruction under a predicate, not under a branch: its
+// operands live in uniform registers, which a branch on the elected thread
+// makes the compiler rebuild for every MMA (80 cycles each to issue).
+__device__ __forceinline__ void umma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(z), "r"(z), "r"(z), "r"(z));
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one));
+}
+// the same with A in TMEM (lane = row, two 16-bit elements per column)
+__device__ __forceinline__ void umma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one));
+}
+__device__ __forceinline__ void commit_one(uint32_t one, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(su32(bar)),
+        "r"(one)
+        : "memory");
 }
 #define S2D_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define S2D_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// One thread of the warp, the same one each time.
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t yes;
+    asm volatile("{ .reg .pred q; elect.sync _|q, 0xffffffff; selp.u32 %0, 1, 0, q; }" : "=r"(yes));
+    return yes;
+}
+// A bounded wait of a whole warp; gives up early once *abort is set.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t par, const volatile int *abort) {
+    for (uint32_t i = 0; !__all_sync(0xffffffffu, mb_try(bar, par)); ++i)
+        if (i >= kTcSpin || ((i & 255u) == 255u && *abort)) return false;
+    return true;
+}
 // 32 columns of this thread's lane; the values are there after tmem_wait_ld.
 __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile(
@@ -148,7 +174,7 @@ __device__ __forceinline__ void mask(uint32_t (&s)[N], int vis) {
 template <typename Q, int HD>
 struct TcShape {
     static constexpr bool kF32 = sizeof(Q) == 4;
-    static constexpr int BN = kF32 ? 64 : 128;             // positions per tile
+    static constexpr int BN = 128;                         // positions per tile
     static constexpr int kPages = BN / kCachePage;         // pages per tile
     static constexpr int kHalves = HD / 64;                // 128-byte column blocks of a row
     static constexpr int kSplit = kF32 ? 2 : 1;            // hi and lo
@@ -159,15 +185,15 @@ struct TcShape {
     static constexpr int kFit = (224 * 1024 - 2 * kQTile) / kSlot;
     static constexpr int kSlots = kFit < 8 ? kFit : 8;     // K and V tiles in flight
     static constexpr int kSmem = 2 * kQTile + kSlots * kSlot + 1024;
-    static constexpr int kFlush = 4;                       // f32: tiles that O takes before it moves to registers
+    static constexpr int kFlush = 2;                       // f32: tiles that O takes before it moves to registers
     static constexpr uint32_t kO = 2 * BN;                 // TMEM: S0, S1 (BN columns each), O0, O1 (HD each)
-    static constexpr uint32_t kP = kF32 ? kO + 2 * HD : 0;  // f32: P0, P1 (hi and lo, BN / 2 columns each); else P over S
-    static_assert(kP + 2 * BN <= kTcColumns && kO + 2 * HD <= kTcColumns, "TMEM columns");
-    static_assert(kSlots >= 4, "K and V of two tiles");
+    static_assert(kO + 2 * HD <= kTcColumns, "TMEM columns");
+    static_assert(kSlots >= 3, "K and V of a tile and the next K");
 };
 
 struct TcShared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2];
+    uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2], item_full[2], item_empty[2];
+    int item[2];
     uint32_t tmem;
     int abort;
 };
@@ -184,6 +210,12 @@ struct TcItem {
     __device__ __forceinline__ int seen(int n, int rep) const { return pooled ? 0 : max(0, back + (r0 + n - 1) / rep + 1); }
     // positions of tile j that exist
     __device__ __forceinline__ int valid(int j) const { return j < jp ? pre1 - pre0 - j * BN : own1 - own0 - (j - jp) * BN; }
+
+    // The fields of the MMA warp's loops, known to be alike in all lanes.
+    __device__ __forceinline__ void uniform() {
+        auto u = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+        pre0 = u(pre0), pre1 = u(pre1), own0 = u(own0), own1 = u(own1), jp = u(jp), nq = u(nq), J[0] = u(J[0]), J[1] = u(J[1]);
+    }
 
     // false: nothing to do.  Called by whole warps.
     __device__ bool get(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, int item) {
@@ -211,6 +243,7 @@ struct TcItem {
         }
         if (rows <= 0) return false;
         rows = min(rows, kTcItemRows);
+        J[0] = J[1] = 0;
         r0 = tile * kTcItemRows, nq = rows > kTcRows ? 2 : 1;
         if (!pooled) {
             const int span = seen(rows, p.rep), tiles = (span + BN - 1) / BN, per = (tiles + splits - 1) / splits;
@@ -233,12 +266,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __shared__ TcShared sh;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = su32(smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // through a shuffle, so that the compiler knows it alike in all lanes: what
+    // the MMA warp computes from such values stays in uniform registers, where
+    // the MMAs take their operands (80 cycles an MMA to issue otherwise)
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int *abort_v = &sh.abort;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < Sh::kSlots; ++i) mb_init(&sh.full[i], 1), mb_init(&sh.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_full[i], 4), mb_init(&sh.pv_done[i], 1), mb_init(&sh.q_full[i], 4);
+        for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_full[i], 4), mb_init(&sh.pv_done[i], 1), mb_init(&sh.q_full[i], 4),
+            mb_init(&sh.item_full[i], 1), mb_init(&sh.item_empty[i], 9);
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -250,9 +287,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    // all 512 columns are this CTA's: its TMEM starts at 0, which the MMAs'
+    // addresses then need not be told at run time
+    constexpr uint32_t tmem = 0;
+    if (sh.tmem != 0) {
+        if (threadIdx.x == 0) cache_flag(c.status, S2D_CACHE_ABORTED);
+        return;
+    }
     TcItem<BN> it;
 
+    // The CTA's n-th item: its own block's, then what the loader drew from the
+    // counter, through a ring of two.  For the MMA and softmax warps.
+    auto take = [&](int n, int &item) {
+        if (n == 0) {
+            item = (int)blockIdx.x;
+            return true;
+        }
+        const int s = n & 1;
+        if (!warp_wait(&sh.item_full[s], ((n - 1) >> 1) & 1, abort_v)) return false;
+        item = *const_cast<volatile int *>(&sh.item[s]);
+        __syncwarp();
+        if (lane == 0) mb_arrive(&sh.item_empty[s]);
+        return true;
+    };
     // Registers: 168 a thread at launch (three warps on a scheduler); warps
     // 8-11 give theirs to the softmax warps: 2 x 216 + 72 = 3 x 168.
     if (warp >= 8) {
@@ -261,8 +318,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ---- loader: K then V of every tile of every item ----
             int issued = 0;
             bool ok = true;
-            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-                if (!it.get(c, a, p, item)) continue;
+            for (int n = 0, item = blockIdx.x; item < items && ok;) {
+                // draw the next item while this one's tiles are loaded
+                int next = items;
+                if (p.next_item) {
+                    if (lane == 0) next = (int)gridDim.x + atomicAdd(p.next_item, 1);
+                    next = __shfl_sync(0xffffffffu, next, 0);
+                }
+                const int s = ++n & 1, use = (n - 1) >> 1;
+                if (use > 0 && !(ok = warp_wait(&sh.item_empty[s], (use - 1) & 1, abort_v))) break;
+                if (lane == 0) {
+                    *const_cast<volatile int *>(&sh.item[s]) = next;
+                    mb_arrive(&sh.item_full[s]);
+                }
+                const bool real = it.get(c, a, p, item);
+                item = next;
+                if (!real) continue;
                 const int32_t *own_table = c.page_table + (int64_t)it.b * c.table_stride;
                 int ids = 0, have = -1;  // page ids 32 * have + lane of the current segment
                 const int J = it.J[it.nq - 1];
@@ -290,7 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         const int s = issued % Sh::kSlots, use = issued / Sh::kSlots;
-                        if (use > 0 && !__all_sync(0xffffffffu, mb_wait(&sh.empty[s], (use & 1) ^ 1, abort_v))) {
+                        if (use > 0 && !warp_wait(&sh.empty[s], (use & 1) ^ 1, abort_v)) {
                             ok = false;
                             break;
                         }
@@ -316,50 +387,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ---- MMA issuer ----
             constexpr uint32_t type = std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t id_s = idesc_f16_f32(kTcRows, BN) | type, id_o = idesc_f16_f32_bmn(kTcRows, HD) | type;
-            auto wait = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, mb_wait(bar, par, abort_v)) != 0; };
+            auto wait = [&](uint64_t *bar, uint32_t par) { return warp_wait(bar, par, abort_v); };
             auto slot_wait = [&](int i) { return wait(&sh.full[i % Sh::kSlots], (uint32_t)(i / Sh::kSlots) & 1); };
             auto slot_base = [&](int i) { return sbase + 2 * Sh::kQTile + (uint32_t)(i % Sh::kSlots) * Sh::kSlot; };
             int kv = 0;                // tiles of earlier items: tile j's K is load 2 (kv + j), its V the next
             uint32_t np[2] = {0, 0};   // P tiles taken so far
             uint32_t nitem[2] = {0, 0};
             bool ok = true;
+            const uint32_t one = elect();
             auto issue_s = [&](int q, int j) {
-                if (lane == 0) {
-                    const int load = 2 * (kv + j);
-                    const uint32_t k = slot_base(load), qt = sbase + (uint32_t)q * Sh::kQTile, d = tmem + (uint32_t)(q * BN);
-    #pragma unroll
-                    for (int part = Sh::kSplit - 1; part >= 0; --part)  // the remainders first: their sums are small
-    #pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk) {
-                            const uint32_t half = (uint32_t)(kk >> 2), off = (uint32_t)((kk & 3) * 32);
-                            umma_f16(d, desc_k_sw128(qt + (uint32_t)(part * Sh::kHalves * Sh::kQHalf) + half * Sh::kQHalf + off),
-                                     desc_k_sw128(k + half * Sh::kKvHalf + off), id_s, (uint32_t)(part != Sh::kSplit - 1 || kk > 0));
-                        }
-                    umma_commit(&sh.s_full[q]);
-                    if (q == it.nq - 1) umma_commit(&sh.empty[load % Sh::kSlots]);
-                }
-                __syncwarp();
+                const int load = 2 * (kv + j);
+                const uint32_t k = slot_base(load), qt = sbase + (uint32_t)q * Sh::kQTile, d = tmem + (uint32_t)(q * BN);
+#pragma unroll
+                for (int part = Sh::kSplit - 1; part >= 0; --part)  // the remainders first: their sums are small
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint32_t half = (uint32_t)(kk >> 2), off = (uint32_t)((kk & 3) * 32);
+                        umma_ss(one, d, desc_k_sw128(qt + (uint32_t)(part * Sh::kHalves * Sh::kQHalf) + half * Sh::kQHalf + off),
+                                 desc_k_sw128(k + half * Sh::kKvHalf + off), id_s, (uint32_t)(part != Sh::kSplit - 1 || kk > 0));
+                    }
+                commit_one(one, &sh.s_full[q]);
+                if (q == it.nq - 1) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
             auto issue_pv = [&](int q, int j) {
-                if (lane == 0) {
-                    const int load = 2 * (kv + j) + 1;
-                    const uint32_t v = slot_base(load), d = tmem + Sh::kO + (uint32_t)(q * HD), pt = tmem + Sh::kP + (uint32_t)(q * BN);
-                    const bool fresh = Sh::kF32 ? j % Sh::kFlush == 0 : j == 0;
-    #pragma unroll
-                    for (int part = 0; part < Sh::kSplit; ++part)
-    #pragma unroll
-                        for (int kk = 0; kk < BN / 16; ++kk)
-                            umma_ts(d, pt + (uint32_t)(part * (BN / 2) + kk * 8), desc_mn_sw128(v + (uint32_t)kk * 2048u, Sh::kKvHalf), id_o,
-                                    (uint32_t)(!fresh || part || kk));
-                    umma_commit(&sh.pv_done[q]);
-                    if (q == it.nq - 1) umma_commit(&sh.empty[load % Sh::kSlots]);
-                }
-                __syncwarp();
+                const int load = 2 * (kv + j) + 1;
+                const uint32_t v = slot_base(load), d = tmem + Sh::kO + (uint32_t)(q * HD), pt = tmem + (uint32_t)(q * BN);
+                const bool fresh = Sh::kF32 ? j % Sh::kFlush == 0 : j == 0;
+#pragma unroll
+                for (int part = 0; part < Sh::kSplit; ++part)
+#pragma unroll
+                    for (int kk = 0; kk < BN / 16; ++kk)
+                        // 16-bit: 8 columns a step; f32: 8 of hi and 8 of lo over the 16 that S leaves
+                        umma_ts(one, d, pt + (uint32_t)(Sh::kF32 ? kk * 16 + part * 8 : kk * 8), desc_mn_sw128(v + (uint32_t)kk * 2048u, Sh::kKvHalf), id_o,
+                                (uint32_t)(!fresh || part || kk));
+                commit_one(one, &sh.pv_done[q]);
+                if (q == it.nq - 1) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
-            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            for (int n = 0, item; ok && (ok = take(n, item)) && item < items; ++n) {
                 if (!it.get(c, a, p, item)) continue;
+                it.uniform();
                 const int nq = it.nq, J = it.J[nq - 1];
-                for (int q = 0; q < nq && ok; ++q) {
+                            for (int q = 0; q < nq && ok; ++q) {
                     ok = wait(&sh.q_full[q], nitem[q]++ & 1);
                     tc_fence_after();
                     if (ok && it.J[q] > 0 && (ok = slot_wait(2 * kv))) issue_s(q, 0);
@@ -372,11 +440,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         if (!(ok = wait(&sh.p_full[q], np[q]++ & 1))) break;
                         tc_fence_after();
                         const bool more = j + 1 < it.J[q];
-                        // P in columns of its own: S is free, and the next S goes out before P V
-                        if (Sh::kF32 && more) {
-                            if (!(ok = slot_wait(load + 1))) break;
-                            issue_s(q, j + 1);
-                        }
                         if (!v_ready) {
                             if (!(ok = slot_wait(load))) break;
                             v_ready = true;
@@ -393,7 +456,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             }
                         }
                         issue_pv(q, j);
-                        if (!Sh::kF32 && more) {
+                        if (more) {
                             if (!(ok = slot_wait(load + 1))) break;
                             issue_s(q, j + 1);
                         }
@@ -408,11 +471,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // ---- softmax and epilogue of row tile q: one thread per row ----
         const int q = warp >> 2, r = 32 * (warp & 3) + lane;
         const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const uint32_t st = lane_t + (uint32_t)(q * BN), ot = lane_t + Sh::kO + (uint32_t)(q * HD), pt = lane_t + Sh::kP + (uint32_t)(q * BN);
+        const uint32_t st = lane_t + (uint32_t)(q * BN), ot = lane_t + Sh::kO + (uint32_t)(q * HD);
         const uint32_t qdst = sbase + (uint32_t)q * Sh::kQTile;
         uint32_t ns = 0;  // S tiles taken so far; P V tiles done are as many
         bool ok = true;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        for (int n = 0, item; ok && (ok = take(n, item)) && item < items; ++n) {
             if (!it.get(c, a, p, item) || q >= it.nq) continue;
             const int row = q * kTcRows + r, J = it.J[q];
             const bool real = row < it.rows;
@@ -484,7 +547,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             };
             for (int j = 0; j < J; ++j, ++ns) {
-                ok = __all_sync(0xffffffffu, mb_wait(&sh.s_full[q], ns & 1, abort_v)) != 0;
+                ok = warp_wait(&sh.s_full[q], ns & 1, abort_v);
                 if (!ok) break;
                 tc_fence_after();
                 const int vis = !real ? BN : j < it.jp ? it.pre1 - it.pre0 - j * BN : own_limit - (j - it.jp) * BN;
@@ -492,14 +555,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint32_t s[Sh::kF32 ? 32 : BN];
                 float mx;
                 if constexpr (Sh::kF32) {
-                    tmem_ld(st, s);
-                    tmem_wait_ld();
-                    if (!whole) mask(s, vis);
-                    mx = max_of(s);
-                    tmem_ld(st + 32, s);
-                    tmem_wait_ld();
-                    if (!whole) mask(s, vis - 32);
-                    mx = fmaxf(mx, max_of(s));
+                    mx = -INFINITY;
+#pragma unroll
+                    for (int h = 0; h < BN / 32; ++h) {
+                        tmem_ld(st + 32 * h, s);
+                        tmem_wait_ld();
+                        if (!whole) mask(s, vis - 32 * h);
+                        mx = fmaxf(mx, max_of(s));
+                    }
                 } else {
 #pragma unroll
                     for (int h = 0; h < BN / 32; ++h) tmem_ld(st + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * h]));
@@ -514,7 +577,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const bool rescale = j > 0 && __any_sync(0xffffffffu, corr != 1.f);
                 if (j > 0) {
                     // P and O are free once P V of the last tile is done
-                    ok = __all_sync(0xffffffffu, mb_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v)) != 0;
+                    ok = warp_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v);
                     if (!ok) break;
                     tc_fence_after();
                 }
@@ -542,7 +605,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint64_t sum[2] = {0, 0};
                 if constexpr (Sh::kF32) {
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
+                    for (int h = 0; h < BN / 16; ++h) {
                         uint32_t x[16], hi[8], lo[8];
                         tmem_ld16(st + 16 * h, x);
                         tmem_wait_ld();
@@ -554,8 +617,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             sum[i & 1] = add2(sum[i & 1], two(w0, w1));
                             split2<E>(w0, w1, hi[i], lo[i]);
                         }
-                        tmem_st8(pt + 8 * h, hi);
-                        tmem_st8(pt + BN / 2 + 8 * h, lo);
+                        tmem_st8(st + 16 * h, hi);
+                        tmem_st8(st + 16 * h + 8, lo);
                     }
                 } else {
 #pragma unroll
@@ -568,7 +631,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             sum[i & 1] = add2(sum[i & 1], two(w0, w1));
                             w[i] = pack2<E>(w0, w1);
                         }
-                        tmem_st32(pt + 32 * h, w);
+                        tmem_st32(st + 32 * h, w);
                     }
                 }
                 const float2 total = untwo(add2(sum[0], sum[1]));
@@ -578,7 +641,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 if (lane == 0) mb_arrive(&sh.p_full[q]);
             }
-            if (ok && J > 0) ok = __all_sync(0xffffffffu, mb_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v)) != 0;
+            if (ok && J > 0) ok = warp_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v);
             if (!ok) break;
             tc_fence_after();
             if (J > 0) flush(false);
@@ -666,7 +729,10 @@ cudaError_t launch(const S2dCacheView &c, const S2dCacheAttention &a, const Attn
     if (items > 0x7fffffff - 1024) return cudaErrorInvalidValue;
     int sms = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device))) return e;
-    rows_tc_kernel<Q, E, HD><<<(unsigned)std::min<int64_t>(items, sms), kTcThreads, smem, s>>>(mk, mv, c, a, p, (int)items);
+    AttnPlan q = p;
+    if (items <= sms) q.next_item = nullptr;  // one item each
+    if (q.next_item && (e = cudaMemsetAsync(q.next_item, 0, sizeof(int), s))) return e;
+    rows_tc_kernel<Q, E, HD><<<(unsigned)std::min<int64_t>(items, sms), kTcThreads, smem, s>>>(mk, mv, c, a, q, (int)items);
     return cudaGetLastError();
 }
 
