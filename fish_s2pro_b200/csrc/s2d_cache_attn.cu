@@ -61,6 +61,14 @@ __device__ __forceinline__ void store_out(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_out(__half *p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void store_out(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
+__device__ __forceinline__ void store_out4(float *p, const float (&x)[4]) {
+    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+template <typename E>
+__device__ __forceinline__ void store_out4(E *p, const float (&x)[4]) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<E>(x[0], x[1]), pack2<E>(x[2], x[3]));
+}
+
 // All threads of the cluster's CTAs (of the CTA where it is alone).
 __device__ __forceinline__ void cluster_sync(int size) {
     if (size == 1) {
@@ -73,7 +81,7 @@ __device__ __forceinline__ void cluster_sync(int size) {
 // *p in the shared memory of CTA `rank` of the cluster
 template <typename T>
 __device__ __forceinline__ T cluster_get(const T *p, int rank, int size) {
-    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two words");
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8 || sizeof(T) == 16, "one, two or four words");
     if (size == 1) return *p;
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
@@ -82,6 +90,10 @@ __device__ __forceinline__ T cluster_get(const T *p, int rank, int size) {
         uint32_t x;
         asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
         memcpy(&v, &x, 4);
+    } else if constexpr (sizeof(T) == 16) {
+        uint4 x;
+        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+        memcpy(&v, &x, 16);
     } else {
         uint2 x;
         asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(at) : "memory");
@@ -132,6 +144,8 @@ __device__ __forceinline__ void load_q(const Q *row, float scale, int t, uint32_
         }
     }
 }
+
+constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots
 
 // Single tokens: the rep <= 8 query heads of one (sequence, KV head) against
 // the sequence's own slots, shared by the CTAs of a cluster (chunks of 16
@@ -282,23 +296,25 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
     // what every part counts in the row's softmax: ranks, then prefix parts
     for (int row = warp; row < n_rows; row += NW) {
         const int64_t id = (int64_t)b * a.heads + head0 + row;
-        float2 mine = make_float2(-INFINITY, 0.f);
+        const float2 none = make_float2(-INFINITY, 0.f);
+        float2 mine = none, pre[kMaxParts / 32];
+#pragma unroll
+        for (int i = 0; i < kMaxParts / 32; ++i) pre[i] = lane + 32 * i < p.parts ? __ldcg(&p.ml[id * p.parts + lane + 32 * i]) : none;
         if (lane < S) mine = cluster_get(&s_ml[row], lane, S);
         float m = mine.x;
-        for (int k = lane; k < p.parts; k += 32) m = fmaxf(m, __ldcg(&p.ml[id * p.parts + k]).x);
+#pragma unroll
+        for (int i = 0; i < kMaxParts / 32; ++i) m = fmaxf(m, pre[i].x);
         m = warp_max(m);
         const float f = lane < S ? part_factor(mine.x, mine.y, m) : 0.f;
-        float l = lane < S ? f * mine.y : 0.f;
-        for (int k = lane; k < p.parts; k += 32) {
-            const float2 e = __ldcg(&p.ml[id * p.parts + k]);
-            const float fk = part_factor(e.x, e.y, m);
-            s_pre[row * p.parts + k] = fk;
-            l = fmaf(e.y, fk, l);
-        }
+        float l = lane < S ? f * mine.y : 0.f, fp[kMaxParts / 32];
+#pragma unroll
+        for (int i = 0; i < kMaxParts / 32; ++i) fp[i] = part_factor(pre[i].x, pre[i].y, m), l = fmaf(pre[i].y, fp[i], l);
         l = warp_sum(l);
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
         if (lane < S) s_rank[row][lane] = f * inv;
-        for (int k = lane; k < p.parts; k += 32) s_pre[row * p.parts + k] *= inv;
+#pragma unroll
+        for (int i = 0; i < kMaxParts / 32; ++i)
+            if (lane + 32 * i < p.parts) s_pre[row * p.parts + lane + 32 * i] = fp[i] * inv;
         if (lane == 0) {
             const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
             s_lse[row] = l == 0.f ? 0.f : lse2;
@@ -309,14 +325,26 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
         }
     }
     __syncthreads();
-    // the outputs, shared by the ranks
-    for (int i = rank * 128 + (int)threadIdx.x; i < n_rows * HD; i += S * 128) {
-        const int row = i / HD, d = i % HD;
+    // the outputs, four elements a thread, shared by the ranks
+    for (int i = rank * 128 + (int)threadIdx.x; i < n_rows * (HD / 4); i += S * 128) {
+        const int row = i / (HD / 4), d = i % (HD / 4) * 4;
         const int64_t id = (int64_t)b * a.heads + head0 + row;
-        float sum = 0.f;
-        for (int k = 0; k < S; ++k) sum = fmaf(cluster_get(&s_o[row * HD + d], k, S), s_rank[row][k], sum);
-        for (int k = 0; k < p.parts; ++k) sum = fmaf(__ldcg(p.part + (id * p.parts + k) * HD + d), s_pre[row * p.parts + k], sum);
-        store_out(static_cast<Q *>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + row) * HD + d, sum);
+        float sum[4] = {};
+        auto add = [&](float4 v, float f) {
+            sum[0] = fmaf(v.x, f, sum[0]), sum[1] = fmaf(v.y, f, sum[1]), sum[2] = fmaf(v.z, f, sum[2]), sum[3] = fmaf(v.w, f, sum[3]);
+        };
+        for (int k = 0; k < S; ++k) add(cluster_get(reinterpret_cast<const float4 *>(&s_o[row * HD + d]), k, S), s_rank[row][k]);
+        const float4 *part = reinterpret_cast<const float4 *>(p.part + id * p.parts * HD + d);
+        for (int k0 = 0; k0 < p.parts; k0 += 8) {  // eight parts in flight
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k < p.parts) v[k] = __ldcg(part + (k0 + k) * (HD / 4));
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k < p.parts) add(v[k], s_pre[row * p.parts + k0 + k]);
+        }
+        store_out4(static_cast<Q *>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + row) * HD + d, sum);
     }
     if (keep) {
         float *mass = c.mass + ((int64_t)b * G + g) * c.max_pages * kCachePage;
@@ -464,30 +492,30 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
     p = {};
     p.rep = a.heads / c.kv_heads;
     const int64_t rows = (int64_t)a.tokens * p.rep;
-    // splits that give every SM an item, of at least `least` positions
-    auto cut = [&](int64_t items, int64_t positions, int64_t least) {
-        const int64_t want = kSms / std::max<int64_t>(items, 1);
-        return (int)std::max<int64_t>(1, std::min<int64_t>({want, (positions + least - 1) / least, 64}));
+    // splits that give `fill` items to fill, of at least `least` positions
+    auto cut = [&](int64_t items, int64_t positions, int64_t least, int64_t fill) {
+        const int64_t want = fill / std::max<int64_t>(items, 1);
+        return (int)std::max<int64_t>(1, std::min<int64_t>({want, (positions + least - 1) / least, kMaxParts}));
     };
     const int64_t pooled = (rows + kTcTile - 1) / kTcTile;
     if (!a.q_start) {
         if (a.prefix_len) {
             p.prefix_tiles = (int)pooled;
-            p.prefix_splits = cut(pooled * c.kv_heads, a.prefix_len, 128);
+            p.prefix_splits = cut(pooled * c.kv_heads, a.prefix_len, 128, kSms);
         }
         const int64_t items = (int64_t)a.tokens * c.kv_heads;
         p.own_splits = 1;
-        while (p.own_splits < kMaxCluster && items * p.own_splits < 4 * kSms) p.own_splits *= 2;
+        while (p.own_splits < kMaxCluster && items * p.own_splits < 4 * kSms && c.max_pages > 4 * p.own_splits) p.own_splits *= 2;
         p.parts = p.prefix_splits;
     } else {
         const int64_t own = rows / kTcTile + std::min<int64_t>(c.n_seq, rows);  // sum of ceil(rows of b / 256) is no more
         const bool fill = own * c.kv_heads >= kSms;
         p.own_tiles = (int)own;
-        p.own_splits = fill ? 1 : cut(own * c.kv_heads, (int64_t)c.max_pages * kCachePage, 128);
+        p.own_splits = fill ? 1 : cut(own * c.kv_heads, (int64_t)c.max_pages * kCachePage, 512, 4 * kSms);
         p.fused = a.prefix_len && fill && rows >= (int64_t)c.n_seq * kTcTile / 2;
         if (a.prefix_len && !p.fused) {
             p.prefix_tiles = (int)pooled;
-            p.prefix_splits = cut(pooled * c.kv_heads, a.prefix_len, 128);
+            p.prefix_splits = cut(pooled * c.kv_heads, a.prefix_len, 128, kSms);
         }
         p.parts = p.prefix_splits + p.own_splits;
         if (p.parts == 1) p.parts = 0;  // an item sees all that its rows see

@@ -483,25 +483,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // Q row: its sign takes the scale's, so that the scores' maximum is that of q . k
             const Q *src = static_cast<const Q *>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * HD;
             float qmul = fabsf(a.scale) * kLog2e;
+            // the whole row in flight at once: one round trip of latency
+            uint4 qv[HD * (int)sizeof(Q) / 16];
+#pragma unroll
+            for (int i = 0; i < HD * (int)sizeof(Q) / 16; ++i) qv[i] = real ? reinterpret_cast<const uint4 *>(src)[i] : make_uint4(0, 0, 0, 0);
             if constexpr (Sh::kF32) {
                 float amax = 0.f;
-                for (int i = 0; i < HD / 4; ++i) {
-                    const float4 v = real ? reinterpret_cast<const float4 *>(src)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-                }
+#pragma unroll
+                for (int i = 0; i < HD / 4; ++i)
+                    amax = fmaxf(amax, fmaxf(fmaxf(fabsf(__uint_as_float(qv[i].x)), fabsf(__uint_as_float(qv[i].y))),
+                                             fmaxf(fabsf(__uint_as_float(qv[i].z)), fabsf(__uint_as_float(qv[i].w)))));
                 int ex = 0;
                 frexpf(amax, &ex);
                 ex = max(ex, -100);
                 const float up = copysignf(ldexpf(1.f, 14 - ex), a.scale);
                 qmul *= ldexpf(1.f, ex - 14);
+#pragma unroll
                 for (int i = 0; i < HD / 8; ++i) {
-                    const float4 x = real ? reinterpret_cast<const float4 *>(src)[2 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    const float4 y = real ? reinterpret_cast<const float4 *>(src)[2 * i + 1] : make_float4(0.f, 0.f, 0.f, 0.f);
                     uint32_t hi[4], lo[4];
-                    split2<E>(x.x * up, x.y * up, hi[0], lo[0]);
-                    split2<E>(x.z * up, x.w * up, hi[1], lo[1]);
-                    split2<E>(y.x * up, y.y * up, hi[2], lo[2]);
-                    split2<E>(y.z * up, y.w * up, hi[3], lo[3]);
+                    split2<E>(__uint_as_float(qv[2 * i].x) * up, __uint_as_float(qv[2 * i].y) * up, hi[0], lo[0]);
+                    split2<E>(__uint_as_float(qv[2 * i].z) * up, __uint_as_float(qv[2 * i].w) * up, hi[1], lo[1]);
+                    split2<E>(__uint_as_float(qv[2 * i + 1].x) * up, __uint_as_float(qv[2 * i + 1].y) * up, hi[2], lo[2]);
+                    split2<E>(__uint_as_float(qv[2 * i + 1].z) * up, __uint_as_float(qv[2 * i + 1].w) * up, hi[3], lo[3]);
                     const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]),
@@ -510,11 +513,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             } else {
                 const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll 4
+#pragma unroll
                 for (int i = 0; i < HD / 8; ++i) {
-                    const uint4 v = real ? reinterpret_cast<const uint4 *>(src)[i] : make_uint4(0, 0, 0, 0);
                     const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(qv[i].x ^ flip), "r"(qv[i].y ^ flip), "r"(qv[i].z ^ flip),
+                                 "r"(qv[i].w ^ flip)
                                  : "memory");
                 }
             }
