@@ -491,6 +491,7 @@ int score_pitch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPla
 void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, size_t &bytes) {
     p = {};
     p.rep = a.heads / c.kv_heads;
+    p.rep_inv = p.rep > 1 ? (uint32_t)(((1ull << 32) + p.rep - 1) / p.rep) : 0;
     const int64_t rows = (int64_t)a.tokens * p.rep;
     // splits that give `fill` items to fill, of at least `least` positions
     auto cut = [&](int64_t items, int64_t positions, int64_t least, int64_t fill) {
@@ -505,7 +506,7 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
         }
         const int64_t items = (int64_t)a.tokens * c.kv_heads;
         p.own_splits = 1;
-        while (p.own_splits < kMaxCluster && items * p.own_splits < 4 * kSms && c.max_pages > 4 * p.own_splits) p.own_splits *= 2;
+        while (p.own_splits < kMaxCluster && items * p.own_splits < 4 * kSms && c.max_pages > 8 * p.own_splits) p.own_splits *= 2;
         p.parts = p.prefix_splits;
     } else {
         const int64_t own = rows / kTcTile + std::min<int64_t>(c.n_seq, rows);  // sum of ceil(rows of b / 256) is no more

@@ -52,6 +52,7 @@ __device__ __forceinline__ float part_factor(float pm, float pl, float m) {
 // (m, l) and O with l = sum 2^(s - m), O = sum 2^(s - m) v in base 2.
 struct AttnPlan {
     int rep;                          // query heads per KV head
+    uint32_t rep_inv;                 // ceil(2^32 / rep), 0 for 1: see row_token
     int prefix_tiles, prefix_splits;  // items over the pooled rows and the prefix
     int own_tiles, own_splits;        // at most this many row tiles over all sequences, and position splits
     int fused;                        // own items walk the prefix too
@@ -61,6 +62,9 @@ struct AttnPlan {
     int *next_item;                   // what the tcgen05 CTAs draw further items from
     float *lse2;                      // [tokens][heads] in base 2, for the weigh kernel, or NULL
 };
+
+// row / rep without a division, for rows below 2^28 (rep <= 16).
+__device__ __forceinline__ int row_token(const AttnPlan &p, int row) { return p.rep_inv ? (int)__umulhi((uint32_t)row, p.rep_inv) : row; }
 
 // Tokens that belong to some sequence: [0, this).
 __device__ __forceinline__ int real_tokens(const S2dCacheAttention &a, int n_seq) {

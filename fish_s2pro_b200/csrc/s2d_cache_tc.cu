@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     volatile int *abort_v = &sh.abort;
 
+    grid_dep_launch();  // every CTA is resident: what follows may use what they leave of the GPU
     if (threadIdx.x == 0) {
         for (int i = 0; i < Sh::kSlots; ++i) mb_init(&sh.full[i], 1), mb_init(&sh.empty[i], 1);
         for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_full[i], 4), mb_init(&sh.pv_done[i], 1), mb_init(&sh.q_full[i], 4),
@@ -479,54 +480,65 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!it.get(c, a, p, item) || q >= it.nq) continue;
             const int row = q * kTcRows + r, J = it.J[q];
             const bool real = row < it.rows;
-            const int rr = it.r0 + (real ? row : 0), tok = it.first + rr / p.rep, head = it.g * p.rep + rr % p.rep;
-            // Q row: its sign takes the scale's, so that the scores' maximum is that of q . k
-            const Q *src = static_cast<const Q *>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * HD;
+            const int rr = it.r0 + (real ? row : 0), rt = row_token(p, rr), tok = it.first + rt, head = it.g * p.rep + rr - rt * p.rep;
+            // The warp's 32 query rows, 16 bytes a lane with a row's lanes side by
+            // side, up to sixteen loads in flight at once.  Their sign takes the scale's,
+            // so that the scores' maximum is that of q . k.  Compact loops, here
+            // and below: code that runs once an item comes from L2, at about six
+            // cycles an instruction.
+            constexpr int kLanes = HD * (int)sizeof(Q) / 16, kTogether = 32 / kLanes;  // lanes of a row, rows of a load
             float qmul = fabsf(a.scale) * kLog2e;
-            // the whole row in flight at once: one round trip of latency
-            uint4 qv[HD * (int)sizeof(Q) / 16];
+            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            const int c16 = lane % kLanes;  // 16-byte chunk of the row
+            int my_ex = 0;
+            constexpr int kAtOnce = kLanes < 16 ? kLanes : 16;
+#pragma unroll 1
+            for (int i0 = 0; i0 < kLanes; i0 += kAtOnce) {
+                uint4 qv[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < HD * (int)sizeof(Q) / 16; ++i) qv[i] = real ? reinterpret_cast<const uint4 *>(src)[i] : make_uint4(0, 0, 0, 0);
-            if constexpr (Sh::kF32) {
-                float amax = 0.f;
-#pragma unroll
-                for (int i = 0; i < HD / 4; ++i)
-                    amax = fmaxf(amax, fmaxf(fmaxf(fabsf(__uint_as_float(qv[i].x)), fabsf(__uint_as_float(qv[i].y))),
-                                             fmaxf(fabsf(__uint_as_float(qv[i].z)), fabsf(__uint_as_float(qv[i].w)))));
-                int ex = 0;
-                frexpf(amax, &ex);
-                ex = max(ex, -100);
-                const float up = copysignf(ldexpf(1.f, 14 - ex), a.scale);
-                qmul *= ldexpf(1.f, ex - 14);
-#pragma unroll
-                for (int i = 0; i < HD / 8; ++i) {
-                    uint32_t hi[4], lo[4];
-                    split2<E>(__uint_as_float(qv[2 * i].x) * up, __uint_as_float(qv[2 * i].y) * up, hi[0], lo[0]);
-                    split2<E>(__uint_as_float(qv[2 * i].z) * up, __uint_as_float(qv[2 * i].w) * up, hi[1], lo[1]);
-                    split2<E>(__uint_as_float(qv[2 * i + 1].x) * up, __uint_as_float(qv[2 * i + 1].y) * up, hi[2], lo[2]);
-                    split2<E>(__uint_as_float(qv[2 * i + 1].z) * up, __uint_as_float(qv[2 * i + 1].w) * up, hi[3], lo[3]);
-                    const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]),
-                                 "r"(lo[2]), "r"(lo[3])
-                                 : "memory");
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int w = q * kTcRows + 32 * (warp & 3) + (i0 + i) * kTogether + lane / kLanes, wr = it.r0 + w, wt = row_token(p, wr);
+                    const Q *src = static_cast<const Q *>(a.q) + (int64_t)(it.first + wt) * a.q_stride + (int64_t)(it.g * p.rep + wr - wt * p.rep) * HD;
+                    qv[i] = w < it.rows ? reinterpret_cast<const uint4 *>(src)[c16] : make_uint4(0, 0, 0, 0);
                 }
-            } else {
-                const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-                for (int i = 0; i < HD / 8; ++i) {
-                    const uint32_t at = qdst + (uint32_t)((i >> 3) * Sh::kQHalf) + swizzle(r, i & 7);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(qv[i].x ^ flip), "r"(qv[i].y ^ flip), "r"(qv[i].z ^ flip),
-                                 "r"(qv[i].w ^ flip)
-                                 : "memory");
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int w = 32 * (warp & 3) + (i0 + i) * kTogether + lane / kLanes;  // row of the tile
+                    if constexpr (Sh::kF32) {
+                        // scaled by the power of two that puts the row's largest element near 2^14: the remainders stay normal
+                        // f16 (at most by 2^114, which keeps rows of subnormal numbers finite)
+                        const float x[4] = {__uint_as_float(qv[i].x), __uint_as_float(qv[i].y), __uint_as_float(qv[i].z), __uint_as_float(qv[i].w)};
+                        float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+                        for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                        const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);
+#pragma unroll
+                        for (int k = 0; k < kTogether; ++k) {
+                            const int e = kTogether == 1 ? ex : __shfl_sync(0xffffffffu, ex, k * kLanes);
+                            if (lane == (i0 + i) * kTogether + k) my_ex = e;
+                        }
+                        const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - ex) << 23), a.scale);
+                        uint32_t hi[2], lo[2];
+                        split2<E>(x[0] * up, x[1] * up, hi[0], lo[0]);
+                        split2<E>(x[2] * up, x[3] * up, hi[1], lo[1]);
+                        const uint32_t at = qdst + (uint32_t)((c16 >> 4) * Sh::kQHalf) + swizzle(w, (c16 >> 1) & 7) + (c16 & 1) * 8;
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]) : "memory");
+                    } else {
+                        const uint32_t at = qdst + (uint32_t)((c16 >> 3) * Sh::kQHalf) + swizzle(w, c16 & 7);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(qv[i].x ^ flip), "r"(qv[i].y ^ flip), "r"(qv[i].z ^ flip),
+                                     "r"(qv[i].w ^ flip)
+                                     : "memory");
+                    }
                 }
             }
+            if constexpr (Sh::kF32) qmul *= __uint_as_float((uint32_t)(127 + my_ex - 14) << 23);
             qmul = fmaxf(qmul, 1e-38f);  // a masked score stays -inf when the scale is 0
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mb_arrive(&sh.q_full[q]);
 
-            const int own_limit = min(it.pooled ? 0 : max(0, it.back + rr / p.rep + 1), it.own1) - it.own0;  // own slots of the item that this row sees
+            const int own_limit = min(it.pooled ? 0 : max(0, it.back + rt + 1), it.own1) - it.own0;  // own slots of the item that this row sees
             float mref = -INFINITY, l = 0.f;
             float acc[Sh::kF32 ? HD : 1];
 #pragma unroll
@@ -550,8 +562,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             };
             for (int j = 0; j < J; ++j, ++ns) {
-                ok = warp_wait(&sh.s_full[q], ns & 1, abort_v);
-                if (!ok) break;
+                if (!(ok = warp_wait(&sh.s_full[q], ns & 1, abort_v))) break;
                 tc_fence_after();
                 const int vis = !real ? BN : j < it.jp ? it.pre1 - it.pre0 - j * BN : own_limit - (j - it.jp) * BN;
                 const bool whole = __all_sync(0xffffffffu, vis >= BN);
@@ -559,7 +570,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 float mx;
                 if constexpr (Sh::kF32) {
                     mx = -INFINITY;
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < BN / 32; ++h) {
                         tmem_ld(st + 32 * h, s);
                         tmem_wait_ld();
@@ -607,7 +618,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint64_t qm2 = two(qmul, qmul), nb2 = two(-base, -base);
                 uint64_t sum[2] = {0, 0};
                 if constexpr (Sh::kF32) {
-#pragma unroll
+#pragma unroll 2
                     for (int h = 0; h < BN / 16; ++h) {
                         uint32_t x[16], hi[8], lo[8];
                         tmem_ld16(st + 16 * h, x);
@@ -661,40 +672,66 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (p.lse2) p.lse2[id] = lse2;
                 }
             }
-            float *to_part = p.part + (id * p.parts + part) * HD;
-            Q *to_out = static_cast<Q *>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * HD;
+            // O, scaled, through the warp's own rows of the Q tile (free by now), so
+            // that a global store writes whole rows: kBlocks blocks of 128 bytes a
+            // row, swizzled like Q, as often as an output row of OB bytes takes
+            constexpr int kBlocks = Sh::kHalves * Sh::kSplit;
+            auto store = [&](auto *to_rows, auto row_offset) {
+                using O = std::remove_reference_t<decltype(*to_rows)>;
+                constexpr int kEach = 16 / (int)sizeof(O), kCols = kBlocks * 8 * kEach < HD ? kBlocks * 8 * kEach : HD;  // elements of a chunk; columns of a pass
+                constexpr int kChunks = kCols / kEach, kRows = 32 / (kChunks < 32 ? kChunks : 32);                       // chunks of a row; rows of a store
+#pragma unroll(Sh::kF32 ? HD / kCols : 1)
+                for (int c0 = 0; c0 < HD; c0 += kCols) {
+#pragma unroll(Sh::kF32 ? kCols / 32 : 1)
+                    for (int i = c0; i < c0 + kCols; i += 32) {
+                        float o[32];
+                        if constexpr (Sh::kF32) {
 #pragma unroll
-            for (int i = 0; i < HD; i += 32) {
-                float o[32];
-                if constexpr (Sh::kF32) {
+                            for (int e = 0; e < 32; ++e) o[e] = acc[i + e] * inv;
+                        } else {
+                            uint32_t raw_o[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = acc[i + e] * inv;
-                } else {
-                    uint32_t raw_o[32];
+                            for (int e = 0; e < 32; ++e) raw_o[e] = 0;
+                            if (J > 0) {
+                                tmem_ld(ot + i, raw_o);  // warp-collective
+                                tmem_wait_ld();
+                            }
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) raw_o[e] = 0;
-                    if (J > 0) {
-                        tmem_ld(ot + i, raw_o);  // warp-collective
-                        tmem_wait_ld();
+                            for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(raw_o[e]) * inv;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += kEach) {
+                            const int ch = (i - c0 + e) / kEach;
+                            uint32_t w[4];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                if constexpr (sizeof(O) == 4) w[x] = __float_as_uint(o[e + x]);
+                                else w[x] = pack2<O>(o[e + 2 * x], o[e + 2 * x + 1]);
+                            }
+                            const uint32_t at = qdst + (uint32_t)((ch >> 3) * Sh::kQHalf) + swizzle(r, ch & 7);
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        }
                     }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(raw_o[e]) * inv;
-                }
-                if (real) {
-                    if (parts || Sh::kF32) {
-                        float4 *to = reinterpret_cast<float4 *>(parts ? to_part + i : reinterpret_cast<float *>(to_out + i));
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                    } else {
-                        uint4 *to = reinterpret_cast<uint4 *>(to_out + i);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            to[e] = make_uint4(pack2<E>(o[8 * e], o[8 * e + 1]), pack2<E>(o[8 * e + 2], o[8 * e + 3]), pack2<E>(o[8 * e + 4], o[8 * e + 5]),
-                                               pack2<E>(o[8 * e + 6], o[8 * e + 7]));
+                    __syncwarp();
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += kRows) {
+                        const int mine = 32 * (warp & 3) + i + lane / kChunks, w = q * kTcRows + mine, ch = lane % kChunks;
+                        uint32_t x[4];
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                                     : "r"(qdst + (uint32_t)((ch >> 3) * Sh::kQHalf) + swizzle(mine, ch & 7))
+                                     : "memory");
+                        if (w < it.rows) *reinterpret_cast<uint4 *>(to_rows + row_offset(it.r0 + w) + c0 + ch * kEach) = make_uint4(x[0], x[1], x[2], x[3]);
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
-            }
+            };
+            auto at_row = [&](int wr, int64_t stride, int step) {  // offset of a row's token and head
+                const int wt = row_token(p, wr);
+                return (int64_t)(it.first + wt) * stride + (int64_t)(it.g * p.rep + wr - wt * p.rep) * step;
+            };
+            if (parts) store(p.part + part * HD, [&](int wr) { return at_row(wr, (int64_t)a.heads * p.parts * HD, p.parts * HD); });
+            else store(static_cast<Q *>(a.out), [&](int wr) { return at_row(wr, a.out_stride, HD); });
         }
         if (!ok) *abort_v = 1;
     }
