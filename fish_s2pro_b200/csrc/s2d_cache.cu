@@ -46,126 +46,185 @@ struct RopeTurns {
     uint64_t turn[64];
 };
 
-template <typename T>
-__device__ __forceinline__ float to_float(T x);
-template <>
-__device__ __forceinline__ float to_float(float x) { return x; }
-template <>
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-template <>
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ float from_float(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
+// The table of a rope_base: computed once, as the base is a model's.
+const RopeTurns &rope_turns(double base, int hd) {
+    thread_local RopeTurns r;
+    thread_local double have = 0.0;
+    thread_local int have_hd = 0;
+    if (base != have || hd != have_hd) {
+        const long double two_pi = 6.283185307179586476925286766559005768L;
+        for (int i = 0; i < hd / 2; ++i) {
+            const long double f = powl((long double)base, -2.0L * i / hd) / two_pi;
+            r.turn[i] = (uint64_t)((f - floorl(f)) * 0x1p64L);  // f - floor(f) < 1
+        }
+        have = base, have_hd = hd;
+    }
+    return r;
+}
 
+// 16 bytes of elements of type T as f32, and back.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4 &v, float (&x)[16 / sizeof(T)]) {
+    if constexpr (sizeof(T) == 4) {
+        x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2<T>(w[i]);
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+}
+// N elements of type T from f32, in one store of 8 or 16 bytes.
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
-    T v[N];
-};
+__device__ __forceinline__ void store_pack(T *to, const float (&x)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        static_assert(N == 4, "16 bytes");
+        *reinterpret_cast<float4 *>(to) = make_float4(x[0], x[1], x[2], x[3]);
+    } else if constexpr (N == 4) {
+        *reinterpret_cast<uint2 *>(to) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+    } else {
+        static_assert(N == 8, "16 bytes");
+        *reinterpret_cast<uint4 *>(to) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+    }
+}
 
-// One block per token.  A head row of HD elements is read 16 bytes a thread,
-// so the row's threads are neighbouring lanes of one warp (8 to 32), which
-// sum the squares with shuffles.  A thread keeps its place in the row over
-// all the rows it takes, so its pairs' sines and cosines are computed once
-// per token and serve all H + Hkv heads.
+// A block takes `group` consecutive tokens (at most kGroup): one thread each
+// finds a token's sequence, slot and page, the block computes the tokens' sines
+// and cosines for all their heads, and then every group of L lanes takes head
+// rows of the tokens in turn.  A head row of HD elements is read 16 bytes a
+// lane, so its lanes are neighbours in one warp (8 to 32) and sum the squares
+// with shuffles.
+//
+// HBM bound: every row is read and written once.  What a token needs before
+// its rows (four dependent loads) is paid once for the group, and kAhead rows
+// of a lane are under way at once.
+constexpr int kGroup = 8, kAhead = 4;
+
 template <typename Q, typename E, int HD>
-__global__ void __launch_bounds__(256) append_kernel(const S2dCacheView c, const S2dCacheAppend a, const RopeTurns turns) {
-    constexpr int W = 16 / (int)sizeof(Q), L = HD / W, ROWS = 256 / L;
-    const int t = blockIdx.x, G = c.kv_heads, cap = c.max_pages * kCachePage;
+__global__ void __launch_bounds__(256, 4) append_kernel(const S2dCacheView c, const S2dCacheAppend a, const __grid_constant__ RopeTurns turns, int tokens) {
+    constexpr int W = 16 / (int)sizeof(Q), L = HD / W, kRows = 256 / L;
+    __shared__ __align__(16) float2 s_turn[kGroup][HD / 2];  // (cos, sin) of the tokens' pairs
+    __shared__ __align__(16) float s_gain[2][HD];            // of queries and keys
+    __shared__ int64_t s_at[kGroup], s_side[kGroup];         // a token's cache rows and its positions / mass, of head 0; -1: none
+    __shared__ int s_pos[kGroup];
+    const int G = c.kv_heads, cap = c.max_pages * kCachePage, tid = threadIdx.x;
+    const int last = a.q_start ? min(a.tokens, __ldg(a.q_start + c.n_seq)) : min(a.tokens, c.n_seq);
+    const int t0 = (int)blockIdx.x * tokens, n = min(tokens, last - t0);
     // lengths of every sequence, tokens or none
-    for (int b = t * 256 + (int)threadIdx.x; b < c.n_seq; b += (int)gridDim.x * 256) {
+    for (int b = (int)blockIdx.x * 256 + tid; b < c.n_seq; b += (int)gridDim.x * 256) {
         int first;
-        const int n = cache_tokens(a.q_start, a.tokens, b, first, c.status), p = a.past[b];
+        const int m = cache_tokens(a.q_start, a.tokens, b, first, c.status), p = a.past[b];
         if (p < 0 || p > cap) cache_flag(c.status, S2D_CACHE_BAD_LENGTH);
-        c.lengths[b] = min(cap, min(max(p, 0), cap) + n);
+        c.lengths[b] = min(cap, min(max(p, 0), cap) + m);
     }
-    if (t >= a.tokens) return;
-    // the token's sequence: how many end at or before it
-    int seq = t, i = 0;
+    if (n <= 0) return;
+    int before = t0;  // sequences that end at or before the group's first token
     if (a.q_start) {
-        seq = 0;
-        for (int b0 = 0; b0 < c.n_seq; b0 += 256) {
-            const int b = b0 + (int)threadIdx.x;
-            seq += __syncthreads_count(b < c.n_seq && __ldg(a.q_start + b + 1) <= t);
-        }
-        if (seq >= c.n_seq) return;  // padding
-        i = t - __ldg(a.q_start + seq);
+        before = 0;
+        for (int b0 = 0; b0 < c.n_seq; b0 += 256) before += __syncthreads_count(b0 + tid < c.n_seq && __ldg(a.q_start + min(b0 + tid, c.n_seq - 1) + 1) <= t0);
     }
-    if (seq >= c.n_seq) return;
-    const int slot = __ldg(a.past + seq) + i;
-    const bool fits = i >= 0 && slot >= i && slot < cap;  // slot >= i: past >= 0 and no overflow
-    if (!fits && threadIdx.x == 0) cache_flag(c.status, i < 0 || slot < i ? S2D_CACHE_BAD_LENGTH : S2D_CACHE_FULL);
-    const int pos = __ldg(a.pos + t);
+    if (tid < n) {
+        const int t = t0 + tid;
+        int seq = t, i = 0;
+        if (a.q_start) {
+            seq = before;
+            while (seq < c.n_seq && __ldg(a.q_start + seq + 1) <= t) ++seq;
+            i = seq < c.n_seq ? t - __ldg(a.q_start + seq) : -1;  // an unordered q_start: lengths has set the status
+        }
+        const int past = i >= 0 ? __ldg(a.past + seq) : -1;
+        const bool sane = past >= 0 && past <= cap, fits = sane && i < cap - past;
+        if (!fits) cache_flag(c.status, sane ? S2D_CACHE_FULL : S2D_CACHE_BAD_LENGTH);
+        s_at[tid] = fits ? cache_row(c, c.page_table + (int64_t)seq * c.table_stride, 0, past + i) : -1;
+        s_side[tid] = fits ? (int64_t)seq * G * cap + past + i : -1;
+        s_pos[tid] = __ldg(a.pos + t);
+    }
+    for (int e = tid; e < 2 * HD; e += 256) {
+        const float *gain = e < HD ? a.q_norm : a.k_norm;
+        s_gain[e / HD][e % HD] = gain ? __ldg(gain + e % HD) : 1.f;
+    }
+    __syncthreads();
+    for (int i = tid; i < n * (HD / 2); i += 256) {
+        const int64_t x = (int64_t)((uint64_t)(int64_t)s_pos[i / (HD / 2)] * turns.turn[i % (HD / 2)]);  // [-1/2, 1/2) turn
+        float sn, cs;
+        sincospif((float)x * 0x1p-63f, &sn, &cs);
+        s_turn[i / (HD / 2)][i % (HD / 2)] = make_float2(cs, sn);
+    }
+    for (int i = tid; i < n * G; i += 256) {
+        const int64_t at = s_side[i / G];
+        if (at >= 0 && c.positions) c.positions[at + (int64_t)(i % G) * cap] = s_pos[i / G];
+        if (at >= 0 && c.mass) c.mass[at + (int64_t)(i % G) * cap] = 0.f;
+    }
+    __syncthreads();
 
-    const int group = threadIdx.x / L, lane = threadIdx.x % L, d0 = lane * W;
-    float cs[W / 2], sn[W / 2];
+    const int d0 = tid % L * W, rows = a.heads + 2 * G;
+    const uint32_t mates = (L == 32 ? 0xffffffffu : (1u << L) - 1u) << ((tid & 31) / L * L);  // the row's lanes
+    int tok = 0, row = tid / L;  // this lane group's next row: a query, a key or a value head of a token of the group
+    auto settle = [&]() {
+        while (row >= rows) row -= rows, ++tok;
+    };
+    settle();
+    while (tok < n) {
+        uint4 in[kAhead];
+        int its_tok[kAhead], its_row[kAhead];
 #pragma unroll
-    for (int p = 0; p < W / 2; ++p) {
-        const int64_t turn = (int64_t)((uint64_t)(int64_t)pos * turns.turn[d0 / 2 + p]);  // [-1/2, 1/2) turn
-        sincospif((float)turn * 0x1p-63f, &sn[p], &cs[p]);
-    }
-    const uint32_t mates = (L == 32 ? 0xffffffffu : (1u << L) - 1u) << ((threadIdx.x & 31) / L * L);  // the row's lanes
-    const int rows = a.heads + 2 * G;
-    for (int r = group; r < rows; r += ROWS) {
-        const bool is_q = r < a.heads, is_k = !is_q && r < a.heads + G;
-        const int h = is_q ? r : is_k ? r - a.heads : r - a.heads - G;
-        const Q *src = static_cast<const Q *>(is_q ? a.q : is_k ? a.k : a.v) +
-                       (int64_t)t * (is_q ? a.q_stride : is_k ? a.k_stride : a.v_stride) + (int64_t)h * HD + d0;
-        const Pack<Q, W> in = *reinterpret_cast<const Pack<Q, W> *>(src);
-        float x[W];
-#pragma unroll
-        for (int e = 0; e < W; ++e) x[e] = to_float(in.v[e]);
-        const float *gain = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
-        if (gain) {
-            float ss = 0.f;
-#pragma unroll
-            for (int e = 0; e < W; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mates, ss, o);
-            const float s = rsqrtf(ss * (1.f / HD) + a.eps);
-#pragma unroll
-            for (int e = 0; e < W; ++e) x[e] = x[e] * s * __ldg(gain + d0 + e);
+        for (int k = 0; k < kAhead; ++k) {
+            its_tok[k] = tok, its_row[k] = row;
+            if (tok < n) {
+                const bool is_q = row < a.heads, is_k = row < a.heads + G;
+                const Q *src = static_cast<const Q *>(is_q ? a.q : is_k ? a.k : a.v) + (int64_t)(t0 + tok) * (is_q ? a.q_stride : is_k ? a.k_stride : a.v_stride) +
+                               (row - (is_q ? 0 : is_k ? a.heads : a.heads + G)) * HD + d0;
+                in[k] = *reinterpret_cast<const uint4 *>(src);
+            }
+            row += kRows;
+            settle();
         }
-        if (is_q || is_k) {
 #pragma unroll
-            for (int p = 0; p < W / 2; ++p) {
-                const float u = x[2 * p], w = x[2 * p + 1];
-                x[2 * p] = u * cs[p] - w * sn[p];
-                x[2 * p + 1] = fmaf(u, sn[p], w * cs[p]);
+        for (int k = 0; k < kAhead; ++k) {
+            if (its_tok[k] >= n) break;  // whole rows: the row's lanes together
+            const bool is_q = its_row[k] < a.heads, is_k = !is_q && its_row[k] < a.heads + G;
+            float x[W];
+            unpack16<Q>(in[k], x);
+            if (is_q || is_k) {
+                if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int e = 0; e < W; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+                    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mates, ss, o);
+                    const float norm = rsqrtf(ss * (1.f / HD) + a.eps);
+#pragma unroll
+                    for (int e = 0; e < W; e += 4) {
+                        const float4 gain = *reinterpret_cast<const float4 *>(&s_gain[is_k][d0 + e]);
+                        x[e] *= norm * gain.x, x[e + 1] *= norm * gain.y, x[e + 2] *= norm * gain.z, x[e + 3] *= norm * gain.w;
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < W / 2; p += 2) {
+                    const float4 r = *reinterpret_cast<const float4 *>(&s_turn[its_tok[k]][d0 / 2 + p]);
+                    const float u0 = x[2 * p], w0 = x[2 * p + 1], u1 = x[2 * p + 2], w1 = x[2 * p + 3];
+                    x[2 * p] = u0 * r.x - w0 * r.y, x[2 * p + 1] = fmaf(u0, r.y, w0 * r.x);
+                    x[2 * p + 2] = u1 * r.z - w1 * r.w, x[2 * p + 3] = fmaf(u1, r.w, w1 * r.z);
+                }
+            }
+            if (is_q) {
+                store_pack(static_cast<Q *>(a.q_out) + (int64_t)(t0 + its_tok[k]) * a.q_out_stride + its_row[k] * HD + d0, x);
+            } else if (s_at[its_tok[k]] >= 0) {
+                const int h = its_row[k] - (is_k ? a.heads : a.heads + G);
+                store_pack(static_cast<E *>(is_k ? c.k : c.v) + s_at[its_tok[k]] + (int64_t)h * c.head_stride + d0, x);
             }
         }
-        if (is_q) {
-            Pack<Q, W> o;
-#pragma unroll
-            for (int e = 0; e < W; ++e) o.v[e] = from_float<Q>(x[e]);
-            *reinterpret_cast<Pack<Q, W> *>(static_cast<Q *>(a.q_out) + (int64_t)t * a.q_out_stride + (int64_t)h * HD + d0) = o;
-        } else if (fits) {
-            const int64_t at = cache_row(c, c.page_table + (int64_t)seq * c.table_stride, h, slot);
-            if (at < 0) continue;
-            Pack<E, W> o;
-#pragma unroll
-            for (int e = 0; e < W; ++e) o.v[e] = from_float<E>(x[e]);
-            *reinterpret_cast<Pack<E, W> *>(static_cast<E *>(is_k ? c.k : c.v) + at + d0) = o;
-        }
     }
-    if (fits)
-        for (int g = threadIdx.x; g < G; g += 256) {
-            const int64_t at = ((int64_t)seq * G + g) * cap + slot;
-            if (c.positions) c.positions[at] = pos;
-            if (c.mass) c.mass[at] = 0.f;
-        }
 }
 
 template <typename Q, typename E>
 cudaError_t append_launch(const S2dCacheView &c, const S2dCacheAppend &a, const RopeTurns &r, cudaStream_t s) {
-    const unsigned blocks = (unsigned)std::max(1, a.tokens);
-    if (c.head_dim == 64) append_kernel<Q, E, 64><<<blocks, 256, 0, s>>>(c, a, r);
-    else append_kernel<Q, E, 128><<<blocks, 256, 0, s>>>(c, a, r);
+    // groups only where there are more tokens than blocks that run at once
+    const int tokens = std::max(1, std::min(kGroup, a.tokens / (148 * 4)));
+    const unsigned blocks = (unsigned)std::max(1, (a.tokens + tokens - 1) / tokens);
+    if (c.head_dim == 64) append_kernel<Q, E, 64><<<blocks, 256, 0, s>>>(c, a, r, tokens);
+    else append_kernel<Q, E, 128><<<blocks, 256, 0, s>>>(c, a, r, tokens);
     return cudaGetLastError();
 }
 
@@ -173,24 +232,25 @@ cudaError_t append_launch(const S2dCacheView &c, const S2dCacheAppend &a, const 
 // evict
 // ---------------------------------------------------------------------------
 
-constexpr int kEvictThreads = 1024;
-
-// f32 -> u32 with the same order; NaN as -inf, -0 as 0.
+// f32 -> u32 with the same order; NaN as -inf, -0 as 0.  Never all ones.
 __device__ __forceinline__ uint32_t ordered(float x) {
     if (x != x) x = -INFINITY;
     const uint32_t b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__device__ __forceinline__ int block_max(int v, int *sh) {
-    v = __reduce_max_sync(0xffffffffu, v);
+// The block's maximum or sum of a value, in every thread.
+template <int WARPS, typename F>
+__device__ __forceinline__ int block_reduce(int v, int *sh, F warp_op, int none) {
+    v = warp_op(v);
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = __reduce_max_sync(0xffffffffu, sh[threadIdx.x & 31]);
+    v = warp_op((threadIdx.x & 31) < WARPS ? sh[threadIdx.x & 31] : none);
     __syncthreads();
     return v;
 }
 // Exclusive prefix sum over the block's threads; total receives the sum.
+template <int WARPS>
 __device__ __forceinline__ int block_scan(int v, int *sh, int &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int in = v;
@@ -201,7 +261,7 @@ __device__ __forceinline__ int block_scan(int v, int *sh, int &total) {
     }
     if (lane == 31) sh[warp] = in;
     __syncthreads();
-    int w = sh[lane];
+    int w = lane < WARPS ? sh[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, w, o);
@@ -213,94 +273,258 @@ __device__ __forceinline__ int block_scan(int v, int *sh, int &total) {
     return before + in - v;
 }
 
-// One block per (sequence, KV head): the budget-th largest key by a radix
-// select of four 8-bit digits, then the freed slots and the rows to move
-// listed in ascending order (block scans over the slots in order), then the
-// moves.  A row is read from a slot >= budget and written to a slot < budget,
-// so no move reads what another writes.
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const S2dCacheView c, const S2dCacheEvict a, int32_t *lists) {
+// counts[0 .. n), n <= N, replaced by their exclusive prefix sums; total receives the sum.
+template <int THREADS, int N>
+__device__ __forceinline__ void scan_counts(int *counts, int n, int *sh, int &total) {
+    constexpr int PER = (N + THREADS - 1) / THREADS;
+    int mine = 0, run[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = (int)threadIdx.x * PER + i;
+        run[i] = mine;
+        mine += at < n ? counts[at] : 0;
+    }
+    const int before = block_scan<THREADS / 32>(mine, sh, total);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = (int)threadIdx.x * PER + i;
+        if (at < n) counts[at] = before + run[i];
+    }
+    __syncthreads();
+}
+
+// One (sequence, KV head) per block, or per cluster of blocks that all choose
+// and then share the moves.  A slot's key is its mass in an order that unsigned
+// comparison follows, or all ones where it is recent.
+//
+//  choose  the smallest key that stays, by a radix select in digits of 11 bits
+//          (histogram in shared memory, scan from the top), and how many of
+//          the slots that equal it stay, the lowest first;
+//  list    the freed slots below the budget and the kept rows above it, both
+//          ascending: a ballot per warp and KPT slots a thread, then one scan
+//          over the warps' counts;
+//  move    row i of the second list into slot i of the first.  A row is read
+//          from a slot >= budget and written to one < budget, so no move reads
+//          what another writes.
+//
+// Up to THREADS * KPT slots the keys stay in registers (read once); longer
+// caches read them again in each of the passes.  The moves are HBM bound, so
+// kMoves 16-byte units of a thread are under way at once.
+constexpr int kDigit = 11, kMoves = 8;
+
+template <int THREADS, int KPT>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const S2dCacheView c, const S2dCacheEvict a, int32_t *lists, int share) {
+    constexpr int WARPS = THREADS / 32, ROUND = THREADS * KPT, BINS = 1 << kDigit, PER = BINS / THREADS;
+    static_assert(KPT <= 32 && WARPS * KPT <= 1024 && PER >= 1, "counts of a round fit the scan");
     __shared__ int sh[32];
-    __shared__ int hist[256];
+    __shared__ int hist[BINS];  // and the warps' counts of a round
+    __shared__ longlong2 s_move[THREADS];  // (to, from) elements of rows to move
     __shared__ uint32_t s_digit;
-    __shared__ int s_need;
-    const int G = c.kv_heads, b = blockIdx.x / G, g = blockIdx.x % G, cap = c.max_pages * kCachePage;
+    __shared__ int s_need, s_in;
+    const int G = c.kv_heads, pair = (int)blockIdx.x / share, part = (int)blockIdx.x % share, b = pair / G, g = pair % G, tid = threadIdx.x;
+    const int cap = c.max_pages * kCachePage, lane = tid & 31, warp = tid >> 5;
     const int n = cache_length(c, b), budget = a.budget;
-    if (g == 0 && threadIdx.x == 0 && a.past) a.past[b] = min(n, budget);
-    if (n <= budget) return;
+    if (g == 0 && part == 0 && tid == 0 && a.past) a.past[b] = min(n, budget);
+    if (n <= budget) return;  // the whole cluster
     int32_t *pos = c.positions + ((int64_t)b * G + g) * cap;
     float *mass = c.mass + ((int64_t)b * G + g) * cap;
     const int32_t *table = c.page_table + (int64_t)b * c.table_stride;
+    const int rounds = (n + ROUND - 1) / ROUND;
+    // slot of a thread's i-th key in a round
+    auto slot = [&](int r, int i) { return r * ROUND + i * THREADS + tid; };
 
+    // keys of a thread that a round uses
+    auto used = [&](int r) { return min(KPT, (n - r * ROUND + THREADS - 1) / THREADS); };
+
+    uint32_t key[KPT];
     int newest = INT32_MIN;
-    for (int j = threadIdx.x; j < n; j += kEvictThreads) newest = max(newest, pos[j]);
-    newest = block_max(newest, sh);
+    for (int r = 0; r < rounds; ++r)
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            if (i >= used(r)) break;
+            const int j = slot(r, i), x = j < n ? pos[j] : INT32_MIN;
+            key[i] = (uint32_t)x;  // the position, for now
+            newest = max(newest, x);
+        }
+    newest = block_reduce<WARPS>(newest, sh, [](int v) { return __reduce_max_sync(0xffffffffu, v); }, INT32_MIN);
     const int64_t edge = (int64_t)newest - a.recent;
-    // More recent slots than the budget (positions that repeat): only they
-    // can stay, by their mass.  Otherwise all of them stay.
     int recents = 0;
-    for (int j = threadIdx.x; j < n; j += kEvictThreads) recents += (int64_t)pos[j] > edge;
-    int all_recents;
-    block_scan(recents, sh, all_recents);
-    const bool crowded = all_recents > budget;
-    auto key = [&](int j) {
-        const bool late = (int64_t)pos[j] > edge;
+    for (int r = 0; r < rounds; ++r)
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            if (i >= used(r)) break;
+            const int j = slot(r, i);
+            if (j < n && (int64_t)(rounds > 1 ? pos[j] : (int)key[i]) > edge) ++recents;
+        }
+    recents = block_reduce<WARPS>(recents, sh, [](int v) { return __reduce_add_sync(0xffffffffu, v); }, 0);
+    // More recent slots than the budget (positions that repeat): only they can
+    // stay, by their mass.  Otherwise all of them stay.
+    const bool crowded = recents > budget;
+    auto key_of = [&](int j, int position) {
+        const bool late = (int64_t)position > edge;
         return late == crowded ? ordered(mass[j]) : late ? 0xffffffffu : 0u;
     };
-
-    // digits of the budget-th largest key, from the top; need: how many of
-    // the keys that share the digits so far are kept
-    uint32_t prefix = 0;
-    int need = budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-        __syncthreads();
-        for (int j = threadIdx.x; j < n; j += kEvictThreads) {
-            const uint32_t k = key(j);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255u], 1);
+    if (rounds == 1) {
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            if (i >= used(0)) break;
+            key[i] = slot(0, i) < n ? key_of(slot(0, i), (int)key[i]) : 0u;
         }
-        __syncthreads();
-        int total;
-        const int digit = 255 - (int)threadIdx.x;  // descending over the threads
-        const int mine = threadIdx.x < 256 ? hist[digit] : 0;
-        const int above = block_scan(mine, sh, total);
-        if (threadIdx.x < 256 && above < need && above + mine >= need) s_digit = (uint32_t)digit, s_need = need - above;
-        __syncthreads();
-        prefix |= s_digit << shift;
-        need = s_need;
-        __syncthreads();
+    }
+    auto load = [&](int r) {
+        if (rounds == 1) return;
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            if (i >= used(r)) break;
+            const int j = slot(r, i);
+            key[i] = j < n ? key_of(j, pos[j]) : 0u;
+        }
+    };
+
+    // the digits of the smallest key that stays, from the top; need: how many
+    // of the keys that share its digits so far stay
+    uint32_t least = crowded ? 0u : 0xffffffffu;
+    int need = crowded ? budget : budget - recents;
+    if (need > 0) {
+        uint32_t prefix = 0;
+        for (int shift = 32; shift > 0;) {
+            const int from = shift, width = min(kDigit, shift);
+            shift -= width;
+            for (int i = tid; i < BINS; i += THREADS) hist[i] = 0;
+            __syncthreads();
+            for (int r = 0; r < rounds; ++r) {
+                load(r);
+#pragma unroll
+                for (int i = 0; i < KPT; ++i) {
+                    if (i >= used(r)) break;
+                    const uint32_t k = key[i];
+                    if (slot(r, i) < n && k != 0xffffffffu && (from == 32 || (k >> from) == (prefix >> from)))
+                        atomicAdd(&hist[(k >> shift) & ((1u << width) - 1u)], 1);
+                }
+            }
+            __syncthreads();
+            int mine = 0, total;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) mine += hist[BINS - 1 - tid * PER - i];  // bins from the top, PER a thread
+            int above = block_scan<WARPS>(mine, sh, total);
+            if (above < need && above + mine >= need) {
+#pragma unroll 1
+                for (int i = 0; i < PER; ++i) {
+                    const int bin = BINS - 1 - tid * PER - i, in = hist[bin];
+                    if (above + in >= need) {
+                        s_digit = (uint32_t)bin, s_need = need - above, s_in = in;
+                        break;
+                    }
+                    above += in;
+                }
+            }
+            __syncthreads();
+            prefix |= s_digit << shift;
+            need = s_need;
+            least = prefix;
+            if (s_in == need) {  // all of them stay: every key from here on
+                least = prefix - 1, need = 0;
+                break;
+            }
+            __syncthreads();
+        }
     }
 
-    // slots in order: equals are kept while they are among the first `need`
+    // lists, round by round
     const int most = min(budget, cap - budget);
     int32_t *holes = lists + (int64_t)blockIdx.x * 2 * most, *rows = holes + most;
     int equals = 0, n_holes = 0, n_rows = 0;
-    for (int j0 = 0; j0 < n; j0 += kEvictThreads) {
-        const int j = j0 + (int)threadIdx.x;
-        const uint32_t k = j < n ? key(j) : 0u;
-        const bool same = j < n && k == prefix;
-        int total;
-        const int eq = equals + block_scan(same, sh, total);
-        equals += total;
-        const bool keep = j < n && (k > prefix || (same && eq < need));
-        const bool hole = j < budget && !keep, row = j >= budget && keep;
-        const int at = block_scan(hole | (row << 16), sh, total);
-        if (hole) holes[n_holes + (at & 0xffff)] = j;
-        if (row) rows[n_rows + (at >> 16)] = j;
-        n_holes += total & 0xffff, n_rows += total >> 16;
+    for (int r = 0; r < rounds; ++r) {
+        load(r);
+        uint32_t keep = 0;  // bit i: the thread's i-th slot of the round stays
+        if (need > 0) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) {
+                if (i >= used(r)) break;
+                const uint32_t same = __ballot_sync(0xffffffffu, slot(r, i) < n && key[i] == least);
+                if (lane == 0) hist[i * WARPS + warp] = __popc(same);
+            }
+            __syncthreads();
+            int total = 0;
+            scan_counts<THREADS, WARPS * KPT>(hist, used(r) * WARPS, sh, total);
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) {
+                if (i >= used(r)) break;
+                const bool is = slot(r, i) < n && key[i] == least;
+                const uint32_t same = __ballot_sync(0xffffffffu, is);
+                const int rank = equals + hist[i * WARPS + warp] + __popc(same & ((1u << lane) - 1u));
+                if (is && rank < need) keep |= 1u << i;
+            }
+            equals += total;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            if (i >= used(r)) break;
+            const int j = slot(r, i);
+            if (j < n && (key[i] > least || key[i] == 0xffffffffu)) keep |= 1u << i;
+            const uint32_t hole = __ballot_sync(0xffffffffu, j < budget && !((keep >> i) & 1u)), row = __ballot_sync(0xffffffffu, j >= budget && ((keep >> i) & 1u));
+            if (lane == 0) hist[i * WARPS + warp] = __popc(hole) | __popc(row) << 16;
+        }
+        __syncthreads();
+        int total = 0;
+        scan_counts<THREADS, WARPS * KPT>(hist, used(r) * WARPS, sh, total);
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            if (i >= used(r)) break;
+            const int j = slot(r, i);
+            const bool hole = j < budget && !((keep >> i) & 1u), row = j >= budget && ((keep >> i) & 1u);
+            const uint32_t h = __ballot_sync(0xffffffffu, hole), w = __ballot_sync(0xffffffffu, row), below = (1u << lane) - 1u;
+            const int at = hist[i * WARPS + warp];
+            if (hole) holes[n_holes + (at & 0xffff) + __popc(h & below)] = j;
+            if (row) rows[n_rows + (int)((uint32_t)at >> 16) + __popc(w & below)] = j;
+        }
+        n_holes += total & 0xffff, n_rows += (int)((uint32_t)total >> 16);
     }
-    __syncthreads();
+    // every block of the cluster has read the positions and the mass that the
+    // moves change (and this block has written its lists)
+    if (share > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
 
-    const int units = c.head_dim / 8;  // 16-byte units of a row
-    for (int i = threadIdx.x; i < n_rows * 2 * units; i += kEvictThreads) {
-        const int m = i / (2 * units), u = i % (2 * units);
-        const int64_t to = cache_row(c, table, g, holes[m]), from = cache_row(c, table, g, rows[m]);
-        if (to < 0 || from < 0) continue;
-        uint16_t *base = static_cast<uint16_t *>(u < units ? c.k : c.v) + (u % units) * 8;
-        *reinterpret_cast<uint4 *>(base + to) = *reinterpret_cast<const uint4 *>(base + from);
-    }
-    for (int m = threadIdx.x; m < n_rows; m += kEvictThreads) {
-        pos[holes[m]] = pos[rows[m]];
-        mass[holes[m]] = mass[rows[m]];
+    // THREADS rows at a time: a thread works out where one goes, then all copy
+    const int units = c.head_dim / 4, half = units / 2;  // 16-byte units of a slot's key and value rows (powers of two)
+    const int shift = 31 - __clz(units);
+    const int row0 = (int)((int64_t)n_rows * part / share), row1 = (int)((int64_t)n_rows * (part + 1) / share);
+    for (int m0 = row0; m0 < row1; m0 += THREADS) {
+        const int m = m0 + tid;
+        if (m < row1) {
+            const int to = holes[m], from = rows[m];
+            const int64_t x = cache_row(c, table, g, to), y = cache_row(c, table, g, from);
+            s_move[tid] = x < 0 || y < 0 ? make_longlong2(-1, -1) : make_longlong2(x, y);
+            pos[to] = pos[from];
+            mass[to] = mass[from];
+        }
+        __syncthreads();
+        const int count = min(THREADS, row1 - m0) * units;
+        for (int i0 = tid; i0 < count; i0 += kMoves * THREADS) {
+            uint4 v[kMoves];
+            int64_t to[kMoves];
+#pragma unroll
+            for (int k = 0; k < kMoves; ++k) {
+                const int i = i0 + k * THREADS, u = i & (units - 1);  // the same for all k: THREADS is a multiple of units
+                to[k] = -1;
+                if (i >= count) continue;
+                const longlong2 at = s_move[i >> shift];
+                to[k] = at.x;
+                if (at.x >= 0) v[k] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(u < half ? c.k : c.v) + at.y + (u & (half - 1)) * 8);
+            }
+            const int u = i0 & (units - 1);
+            uint16_t *base = static_cast<uint16_t *>(u < half ? c.k : c.v) + (u & (half - 1)) * 8;
+#pragma unroll
+            for (int k = 0; k < kMoves; ++k)
+                if (to[k] >= 0) *reinterpret_cast<uint4 *>(base + to[k]) = v[k];
+        }
+        __syncthreads();
     }
 }
 
@@ -309,6 +533,21 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const S2dCacheView
 size_t evict_list(const S2dCacheView &c, const S2dCacheEvict &a) {
     const int64_t cap = (int64_t)c.max_pages * kCachePage;
     return (size_t)std::max<int64_t>(0, std::min<int64_t>(a.budget, cap - a.budget));
+}
+
+// Threads of a block: 16 of a sequence's slots each, in registers, or 32 with
+// the most threads; several smaller blocks run on an SM together.
+int evict_threads(const S2dCacheView &c) {
+    const int64_t cap = (int64_t)c.max_pages * kCachePage;
+    return cap <= 256 * 16 ? 256 : cap <= 512 * 16 ? 512 : 1024;
+}
+// Blocks that share the moves of one (sequence, KV head): as many (up to 8) as
+// run at once.
+int evict_share(const S2dCacheView &c) {
+    const int64_t pairs = (int64_t)c.n_seq * c.kv_heads, most = 148 * (1024 / evict_threads(c));
+    int share = 1;
+    while (share < 8 && pairs * share * 2 <= most) share *= 2;
+    return share;
 }
 
 const char *evict_fault(const S2dCacheView *c, const S2dCacheEvict *a) {
@@ -334,6 +573,12 @@ const char *append_fault(const S2dCacheView *c, const S2dCacheAppend *a) {
         return "q, k and v must have the cache's type, or F32 with an F16 cache";
     const int w = a->type == S2D_TYPE_F32 ? 4 : 8;
     const int64_t qrow = (int64_t)a->heads * c->head_dim;
+    if (a->tokens > 0 && (a->q != a->q_out || a->q_stride != a->q_out_stride)) {
+        const size_t es = a->type == S2D_TYPE_F32 ? 4 : 2;
+        if (overlap(a->q, es * ((size_t)std::max<int64_t>(a->q_stride, 0) * (a->tokens - 1) + qrow), a->q_out,
+                    es * ((size_t)std::max<int64_t>(a->q_out_stride, 0) * (a->tokens - 1) + qrow)))
+            return "q_out must be q itself or not overlap it";
+    }
     if (a->q_stride % w || a->k_stride % w || a->v_stride % w || a->q_out_stride % w || !cache_aligned16(a->q) ||
         !cache_aligned16(a->k) || !cache_aligned16(a->v) || !cache_aligned16(a->q_out))
         return "misaligned buffer: rows of q, k, v and q_out must be 16-byte aligned";
@@ -354,13 +599,7 @@ using namespace s2d;
 extern "C" int32_t s2d_cache_append(const S2dCacheView *view, const S2dCacheAppend *args, void *stream, char *err,
                                     size_t err_cap) {
     if (const char *f = append_fault(view, args)) return cache_fail(err, err_cap, S2D_EINVAL, f);
-    RopeTurns r;
-    const int hd = view->head_dim;
-    const long double two_pi = 6.283185307179586476925286766559005768L;
-    for (int i = 0; i < hd / 2; ++i) {
-        const long double f = powl((long double)args->rope_base, -2.0L * i / hd) / two_pi;
-        r.turn[i] = (uint64_t)((f - floorl(f)) * 0x1p64L);  // f - floor(f) < 1
-    }
+    const RopeTurns &r = rope_turns(args->rope_base, view->head_dim);
     DeviceGuard guard(view->device);
     if (guard.error) return cache_cuda(err, err_cap, "cache append: device", guard.error);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -374,7 +613,7 @@ extern "C" int32_t s2d_cache_evict_workspace(const S2dCacheView *view, const S2d
                                              size_t err_cap) {
     if (const char *f = evict_fault(view, args)) return cache_fail(err, err_cap, S2D_EINVAL, f);
     if (!bytes) return cache_fail(err, err_cap, S2D_EINVAL, "bytes is null");
-    *bytes = sizeof(int32_t) * 2 * evict_list(*view, *args) * (size_t)view->n_seq * view->kv_heads;
+    *bytes = sizeof(int32_t) * 2 * evict_list(*view, *args) * (size_t)view->n_seq * view->kv_heads * evict_share(*view);
     return S2D_OK;
 }
 
@@ -386,9 +625,17 @@ extern "C" int32_t s2d_cache_evict(const S2dCacheView *view, const S2dCacheEvict
         return cache_fail(err, err_cap, S2D_EINVAL, "workspace is null, too small or not 256-byte aligned");
     DeviceGuard guard(view->device);
     if (guard.error) return cache_cuda(err, err_cap, "cache evict: device", guard.error);
-    evict_kernel<<<(unsigned)view->n_seq * (unsigned)view->kv_heads, kEvictThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        *view, *args, static_cast<int32_t *>(args->workspace));
-    return cache_cuda(err, err_cap, "cache evict", cudaGetLastError());
+    const int threads = evict_threads(*view), share = evict_share(*view);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)view->n_seq * (unsigned)view->kv_heads * (unsigned)share), cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)share, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr, cfg.numAttrs = 1;
+    int32_t *lists = static_cast<int32_t *>(args->workspace);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, threads == 256 ? evict_kernel<256, 16> : threads == 512 ? evict_kernel<512, 16> : evict_kernel<1024, 32>, *view, *args, lists, share);
+    return cache_cuda(err, err_cap, "cache evict", e);
 }
 
 extern "C" int32_t s2d_cache_status(const S2dCacheView *view, int32_t *bits, void *stream, char *err, size_t err_cap) {

@@ -10,28 +10,6 @@ namespace s2d {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <typename E>
-__device__ __forceinline__ uint32_t pack2(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <typename E>
-__device__ __forceinline__ float2 unpack2(uint32_t v);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
-}
 // (x, y) = hi + lo, both of the cache's type
 template <typename E>
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
