@@ -8,6 +8,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/s2d_cache.h"
 #include "s2d_common.cuh"
 
@@ -103,6 +105,17 @@ inline int32_t cache_cuda(char *err, size_t cap, const char *what, cudaError_t e
     if (!e) return S2D_OK;
     if (err && cap) snprintf(err, cap, "%s: %s", what, cudaGetErrorString(e));
     return S2D_ECUDA;
+}
+
+// Raises a kernel's dynamic shared memory limit to `bytes`, once per device.
+// `done` is the kernel's own; every caller asks for the same size.
+template <typename K>
+inline cudaError_t smem_limit(std::atomic<uint64_t> &done, K kernel, int device, int bytes) {
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (!e) done.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 // nullptr if the view can be used, else what is wrong with it.

@@ -541,8 +541,8 @@ template <typename Q, typename E, int HD>
 cudaError_t token_launch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
     const int pitch = score_pitch(c, a, p);
     const size_t smem = token_smem(c, p, pitch);
-    // the limit, not this call's size: calls of other threads may launch in between
-    cudaError_t e = cudaFuncSetAttribute(token_kernel<Q, E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTokenSmemMost);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = smem_limit(done, token_kernel<Q, E, HD>, c.device, kTokenSmemMost);
     if (e) return e;
     const int64_t blocks = (int64_t)a.tokens * c.kv_heads * ((p.rep + 7) / 8) * p.own_splits;
     if (blocks > 0x7fffffff) return cudaErrorInvalidValue;

@@ -763,7 +763,8 @@ cudaError_t launch(const S2dCacheView &c, const S2dCacheAttention &a, const Attn
     CUtensorMap mk, mv;
     if (!page_map(&mk, c, c.k) || !page_map(&mv, c, c.v)) return cudaErrorInvalidValue;
     constexpr int smem = TcShape<Q, HD>::kSmem;
-    cudaError_t e = cudaFuncSetAttribute(rows_tc_kernel<Q, E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = smem_limit(done, rows_tc_kernel<Q, E, HD>, c.device, smem);
     if (e) return e;
     const int64_t items = ((int64_t)p.prefix_tiles * p.prefix_splits + (int64_t)p.own_tiles * p.own_splits) * c.kv_heads;
     if (items > 0x7fffffff - 1024) return cudaErrorInvalidValue;

@@ -110,7 +110,7 @@ class PagedKvCache:
 
     def __init__(self, k, v, page_table, lengths, positions=None, mass=None):
         import torch
-        self._torch = torch
+        self._torch, self._int32 = torch, torch.int32
         if k.dim() != 4 or k.shape[2] != PAGE or v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype:
             raise _bad("k and v must be alike, [n_pages, kv_heads, 64, head_dim]")
         if k.dtype not in (torch.float16, torch.bfloat16):
@@ -120,6 +120,10 @@ class PagedKvCache:
         self.device = k.device
         if self.device.type != "cuda":
             raise _bad("the cache must be on a CUDA device")
+        self._index = self.device.index
+        # torch.cuda.current_stream(index).cuda_stream without the Stream object
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda index: torch.cuda.current_stream(index).cuda_stream)
         self.n_pages, self.kv_heads, _, self.head_dim = k.shape
         self.n_seq, self.max_pages = page_table.shape if page_table.dim() == 2 else (0, 0)
         self._ints("page_table", page_table, None)
@@ -152,28 +156,28 @@ class PagedKvCache:
         self._lib = cache_lib()
 
     def _dense(self, name, t, dtype, shape):
-        if t.dtype != dtype or t.device != self.device:
+        if t.dtype != dtype or t.get_device() != self._index:
             raise _bad(f"{name} must be {dtype} on {self.device}")
-        if shape is not None and (tuple(t.shape) != shape or not t.is_contiguous()):
-            raise _bad(f"{name} must be contiguous of shape {shape}, got {tuple(t.shape)}")
+        if shape is not None and (t.shape != shape or not t.is_contiguous()):
+            raise _bad(f"{name} must be contiguous of shape {tuple(shape)}, got {tuple(t.shape)}")
         return t.data_ptr()
 
     def _ints(self, name, t, shape):
-        return self._dense(name, t, self._torch.int32, shape)
+        return self._dense(name, t, self._int32, shape)
 
     def _rows(self, name, t, heads=None):
         """Token rows [tokens, heads, head_dim] with contiguous heads: (pointer, token stride)."""
         s = t.shape
-        if t.dim() != 3 or s[2] != self.head_dim or (heads is not None and s[1] != heads):
+        if len(s) != 3 or s[2] != self.head_dim or (heads is not None and s[1] != heads):
             raise _bad(f"{name} must be [tokens, {heads or 'heads'}, {self.head_dim}], got {tuple(s)}")
-        st = t.stride()
-        if s[0] and (st[2] != 1 or (st[1] != s[2] and s[1] > 1)):
+        step, st1, st2 = t.stride()
+        if s[0] and (st2 != 1 or (st1 != s[2] and s[1] > 1)):
             raise _bad(f"the heads of a token of {name} must be contiguous")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise _bad(f"{name} must be on {self.device}")
         if t.requires_grad and self._torch.is_grad_enabled():
             raise _bad(f"{name} requires a gradient: the cache operators have no backward pass")
-        return t.data_ptr(), st[0] if s[0] > 1 else s[1] * s[2]
+        return t.data_ptr(), step if s[0] > 1 else s[1] * s[2]
 
     def _type(self, name, t):
         code = self._types.get(t.dtype)
@@ -183,7 +187,7 @@ class PagedKvCache:
         return code
 
     def _stream(self):
-        return self._torch.cuda.current_stream(self.device).cuda_stream
+        return self._raw_stream(self._index)
 
     def _call(self, rc: int) -> None:
         if rc != 0:
@@ -217,7 +221,7 @@ class PagedKvCache:
         if k.shape[0] != tokens or v.shape[0] != tokens:
             raise _bad("q, k and v must have the same tokens")
         if out is None:
-            out = self._torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = q.new_empty(q.shape)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise _bad("out must be like q")
         op, os_ = self._rows("out", out)
@@ -246,11 +250,11 @@ class PagedKvCache:
         tokens, heads = q.shape[0], q.shape[1]
         torch = self._torch
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = q.new_empty(q.shape)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise _bad("out must be like q")
         op, os_ = self._rows("out", out)
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if return_lse else None
+        lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
         prefix = None
         if prefix_len:
             if prefix_pages is None or prefix_pages.dim() != 1 or prefix_len < 0 or prefix_pages.shape[0] * PAGE < prefix_len:
@@ -269,7 +273,7 @@ class PagedKvCache:
             need = self._sizes[key] = n.value
         if need:
             # from the caching allocator: stream-ordered, and a captured graph gets its own
-            work = torch.empty(need, dtype=torch.uint8, device=self.device)
+            work = q.new_empty(need, dtype=torch.uint8)
             a.workspace, a.workspace_bytes = work.data_ptr(), need
         self._call(self._lib.s2d_cache_attention(self._view_ref, _c.byref(a), self._stream(), self._err, 256))
         return (out, lse) if return_lse else out
@@ -289,7 +293,7 @@ class PagedKvCache:
             self._call(self._lib.s2d_cache_evict_workspace(self._view_ref, _c.byref(a), _c.byref(n), self._err, 256))
             need = self._sizes[key] = n.value
         if need:
-            work = self._torch.empty(need, dtype=self._torch.uint8, device=self.device)
+            work = self.lengths.new_empty(need, dtype=self._torch.uint8)
             a.workspace, a.workspace_bytes = work.data_ptr(), need
         self._call(self._lib.s2d_cache_evict(self._view_ref, _c.byref(a), self._stream(), self._err, 256))
 
