@@ -386,64 +386,6 @@ __global__ void __launch_bounds__(128) join_kernel(const S2dCacheView c, const S
     }
 }
 
-// mass[b][g][slot] += sum over the rows that see the slot of 2^(s - lse2): the
-// scores again, as S^T = K Q^T, so that a slot's weights lie in one quad's
-// registers and are added in the order of the rows.  A block takes 64 slots,
-// a warp 16 of them.
-template <typename Q, typename E, int HD>
-__global__ void __launch_bounds__(128) weigh_kernel(const S2dCacheView c, const S2dCacheAttention a, const AttnPlan p) {
-    const int G = c.kv_heads, b = blockIdx.y, g = blockIdx.z, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
-    int first;
-    const int n = cache_length(c, b), nt = cache_tokens(a.q_start, a.tokens, b, first, c.status);
-    const int j0 = (int)blockIdx.x * kCachePage + (threadIdx.x >> 5) * 16;
-    if (j0 >= n || nt == 0) return;
-    const int64_t at = cache_row(c, c.page_table + (int64_t)b * c.table_stride, g, j0);
-    if (at < 0) return;
-    const uint16_t *k = static_cast<const uint16_t *>(c.k) + at;
-    uint32_t ka[HD / 16][4];  // slots j0 + gl and j0 + gl + 8
-#pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = gl + 8 * (i & 1);
-            ka[kk][i] = j0 + row < n ? *reinterpret_cast<const uint32_t *>(k + (int64_t)row * HD + 16 * kk + 8 * (i >> 1) + 2 * t) : 0u;
-        }
-    float sum[2] = {};
-    const int rows = nt * p.rep;
-    // rows before this one see none of the block's slots
-    const int skip = max(0, j0 - (n - nt)) * p.rep / 8 * 8;
-    for (int r0 = skip; r0 < rows; r0 += 8) {
-        const int r = r0 + gl;  // the lane loads query row r as column gl of B
-        uint32_t qa[HD / 16][4];
-        float qmul;
-        load_q<Q, E, HD>(r < rows ? static_cast<const Q *>(a.q) + (int64_t)(first + r / p.rep) * a.q_stride + (int64_t)(g * p.rep + r % p.rep) * HD : nullptr,
-                         a.scale, t, qa, qmul);
-        const float mine = r < rows ? p.lse2[(int64_t)(first + r / p.rep) * a.heads + g * p.rep + r % p.rep] : -INFINITY;
-        float s[4] = {};
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-            mma<E>(s, ka[kk], qa[kk][0], qa[kk][2]);
-            if constexpr (sizeof(Q) == 4) mma<E>(s, ka[kk], qa[kk][1], qa[kk][3]);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int col = 2 * t + e;
-            const float lse2 = __shfl_sync(0xffffffffu, mine, col * 4), qm = __shfl_sync(0xffffffffu, qmul, col * 4);
-            const int seen = n - nt + (r0 + col) / p.rep + 1;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (lse2 != -INFINITY && j0 + gl + 8 * i < seen) sum[i] += exp2f(fmaf(s[2 * i + e], qm, -lse2));
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        const int j = j0 + gl + 8 * i;
-        if (t == 0 && j < n) c.mass[((int64_t)b * G + g) * c.max_pages * kCachePage + j] += sum[i];
-    }
-}
-
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 const char *attention_fault(const S2dCacheView *c, const S2dCacheAttention *a) {
@@ -569,8 +511,7 @@ cudaError_t attention_launch(const S2dCacheView &c, const S2dCacheAttention &a, 
         e = cudaGetLastError();
     }
     if (e || !p.lse2) return e;
-    weigh_kernel<Q, E, HD><<<dim3((unsigned)c.max_pages, (unsigned)c.n_seq, (unsigned)c.kv_heads), 128, 0, s>>>(c, a, p);
-    return cudaGetLastError();
+    return launch_weigh_tc(c, a, p, s);
 }
 
 template <typename Q, typename E>

@@ -76,7 +76,10 @@ __device__ __forceinline__ void find_tile(const S2dCacheView &c, const S2dCacheA
     b = -1;
 }
 
-// s2d_cache_tc.cu: the items of `p` on tcgen05.
+// s2d_cache_tc.cu: the items of `p` on tcgen05, and the weights of its rows by
+// computing their scores again (from p.lse2).
 cudaError_t launch_rows_tc(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s);
+
+cudaError_t launch_weigh_tc(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s);
 
 }  // namespace s2d

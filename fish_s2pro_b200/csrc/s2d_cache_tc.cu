@@ -745,6 +745,179 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
+// ---------------------------------------------------------------------------
+// weights of many rows
+// ---------------------------------------------------------------------------
+
+// mass[b][g][slot] += sum over the rows that see the slot of 2^(s - lse2), the
+// scores computed again with the slots as rows: S^T = K Q^T, so that a slot is
+// a TMEM lane and one thread adds its weights, in the order of the rows.
+//
+// A CTA keeps 256 slots' keys in shared memory (two tiles of 128, one for each
+// warpgroup) and takes the sequence's query rows 128 at a time.  Its phases
+// follow one another; with 16-bit queries two CTAs share an SM and fill each
+// other's waits.
+constexpr int kWeighSlots = 256;
+
+template <typename Q, int HD>
+struct WeighShape {
+    static constexpr bool kF32 = sizeof(Q) == 4;
+    static constexpr int kHalves = HD / 64, kSplit = kF32 ? 2 : 1;
+    static constexpr int kQHalf = kTcRows * 128, kQ = kHalves * kSplit * kQHalf;  // query rows: a column block; all
+    static constexpr int kKHalf = kTcRows * 128, kK = kHalves * kKHalf;           // a tile of keys
+    static constexpr int kSmem = kQ + 2 * kK + 1024;
+};
+
+template <typename Q, typename E, int HD>
+__global__ void __launch_bounds__(256) weigh_tc_kernel(const __grid_constant__ CUtensorMap mk, const S2dCacheView c, const S2dCacheAttention a,
+                                                       const AttnPlan p) {
+    using Sh = WeighShape<Q, HD>;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t k_full, s_full;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    __shared__ __align__(16) float2 s_row[kTcRows];  // a row's (multiplier of its scores, lse2); lse2 inf: no weight
+    __shared__ int s_seen[kTcRows];                  // slots that a row sees
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t sbase = su32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y, g = blockIdx.z, p0 = (int)blockIdx.x * kWeighSlots;
+    int first;
+    const int n = cache_length(c, b), nt = cache_tokens(a.q_start, a.tokens, b, first, c.status);
+    if (p0 >= n || nt == 0) return;
+    const int back = n - nt, rows = nt * p.rep;
+    volatile int *abort_v = &s_abort;
+    if (threadIdx.x == 0) {
+        mb_init(&k_full, 1), mb_init(&s_full, 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&s_tmem)), "r"(2 * kTcRows));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const int n_pages = min(kWeighSlots / kCachePage, (n - p0 + kCachePage - 1) / kCachePage);
+    if (threadIdx.x == 0) {
+        mb_expect_tx(&k_full, (uint32_t)(n_pages * Sh::kHalves * kCachePage * 128));
+        const int32_t *table = c.page_table + (int64_t)b * c.table_stride + p0 / kCachePage;
+        for (int i = 0; i < n_pages; ++i) {
+            int page = __ldg(table + i);
+            if ((uint32_t)page >= (uint32_t)c.n_pages) {
+                cache_flag(c.status, S2D_CACHE_BAD_PAGE);
+                page = 0;
+            }
+            for (int h = 0; h < Sh::kHalves; ++h)
+                tma_page(smem + Sh::kQ + (i >> 1) * Sh::kK + h * Sh::kKHalf + (i & 1) * kCachePage * 128, &mk, 64 * h, g, page, &k_full);
+        }
+    }
+    const int tile = warp >> 2, slot = p0 + tile * kTcRows + 32 * (warp & 3) + lane;  // this thread's slot
+    const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(tile * kTcRows);
+    constexpr uint32_t id_s = idesc_f16_f32(kTcRows, kTcRows) | (std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
+    float sum = 0.f;
+    bool ok = true;
+    uint32_t turn = 0;
+    // row tiles before this see none of the CTA's slots
+    for (int r0 = (int)min((int64_t)rows, (int64_t)max(0, p0 - back) * p.rep) / kTcRows * kTcRows; r0 < rows && ok; r0 += kTcRows, ++turn) {
+        // 128 query rows: 16 a warp, 16 bytes a lane
+        constexpr int kLanes = HD * (int)sizeof(Q) / 16, kTogether = 32 / kLanes, kLoads = 16 / kTogether;
+        const int c16 = lane % kLanes;
+        uint4 qv[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int w = r0 + 16 * warp + i * kTogether + lane / kLanes, wt = row_token(p, w);
+            const Q *src = static_cast<const Q *>(a.q) + (int64_t)(first + wt) * a.q_stride + (int64_t)(g * p.rep + w - wt * p.rep) * HD;
+            qv[i] = w < rows ? reinterpret_cast<const uint4 *>(src)[c16] : make_uint4(0, 0, 0, 0);
+        }
+        if (threadIdx.x < kTcRows) {
+            const int w = r0 + (int)threadIdx.x, wt = row_token(p, w);
+            float l = INFINITY;
+            if (w < rows) l = p.lse2[(int64_t)(first + wt) * a.heads + g * p.rep + w - wt * p.rep];
+            s_row[threadIdx.x].y = l == -INFINITY ? INFINITY : l;
+            if (!Sh::kF32) s_row[threadIdx.x].x = a.scale * kLog2e;
+            s_seen[threadIdx.x] = w < rows ? back + wt + 1 : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int w = 16 * warp + i * kTogether + lane / kLanes;
+            if constexpr (Sh::kF32) {
+                const float x[4] = {__uint_as_float(qv[i].x), __uint_as_float(qv[i].y), __uint_as_float(qv[i].z), __uint_as_float(qv[i].w)};
+                float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+                for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);  // as in the kernel above
+                const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+                if (c16 == 0) s_row[w].x = a.scale * kLog2e * __uint_as_float((uint32_t)(127 + ex - 14) << 23);
+                uint32_t hi[2], lo[2];
+                split2<E>(x[0] * up, x[1] * up, hi[0], lo[0]);
+                split2<E>(x[2] * up, x[3] * up, hi[1], lo[1]);
+                const uint32_t at = sbase + (uint32_t)((c16 >> 4) * Sh::kQHalf) + swizzle(w, (c16 >> 1) & 7) + (c16 & 1) * 8;
+                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
+                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]) : "memory");
+            } else {
+                const uint32_t at = sbase + (uint32_t)((c16 >> 3) * Sh::kQHalf) + swizzle(w, c16 & 7);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(qv[i].x), "r"(qv[i].y), "r"(qv[i].z), "r"(qv[i].w) : "memory");
+            }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 0) {
+            const uint32_t one = elect();
+            if (turn == 0 && !warp_wait(&k_full, 0, abort_v)) *abort_v = 1;
+            tc_fence_after();
+            if (!*abort_v) {
+                const int tiles = n - p0 > kTcRows ? 2 : 1;
+                for (int t = 0; t < tiles; ++t)
+#pragma unroll
+                    for (int part = Sh::kSplit - 1; part >= 0; --part)  // the remainders first: their sums are small
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            const uint32_t half = (uint32_t)(kk >> 2), off = (uint32_t)((kk & 3) * 32);
+                            umma_ss(one, tmem + (uint32_t)(t * kTcRows), desc_k_sw128(sbase + Sh::kQ + (uint32_t)t * Sh::kK + half * Sh::kKHalf + off),
+                                    desc_k_sw128(sbase + (uint32_t)(part * Sh::kHalves * Sh::kQHalf) + half * Sh::kQHalf + off), id_s,
+                                    (uint32_t)(part != Sh::kSplit - 1 || kk > 0));
+                        }
+                commit_one(one, &s_full);
+            }
+        }
+        ok = warp_wait(&s_full, turn & 1, abort_v);
+        if (!ok) *abort_v = 1;
+        tc_fence_after();
+        if (ok && p0 + tile * kTcRows < n) {
+            // 128 rows that all see the tile's slots, or not
+            const bool whole = r0 + kTcRows <= rows && s_seen[0] >= min(n, p0 + (tile + 1) * kTcRows);
+#pragma unroll 1
+            for (int h = 0; h < kTcRows / 32; ++h) {
+                uint32_t x[32];
+                tmem_ld(st + 32 * h, x);
+                tmem_wait_ld();
+                float part[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float4 r = *reinterpret_cast<const float4 *>(&s_row[32 * h + i]);
+                    const float w0 = ex2(fmaf(__uint_as_float(x[i]), r.x, -r.y)), w1 = ex2(fmaf(__uint_as_float(x[i + 1]), r.z, -r.w));
+                    part[0] += whole || slot < s_seen[32 * h + i] ? w0 : 0.f;
+                    part[1] += whole || slot < s_seen[32 * h + i + 1] ? w1 : 0.f;
+                }
+                sum += part[0] + part[1];
+            }
+        }
+        tc_fence_before();
+        __syncthreads();  // the rows and the scores are used up
+    }
+    if (turn == 0) (void)warp_wait(&k_full, 0, abort_v);  // no copy may still be landing when the CTA leaves
+    if (ok && slot < n) c.mass[((int64_t)b * c.kv_heads + g) * c.max_pages * kCachePage + slot] += sum;
+    if (threadIdx.x == 0 && *abort_v) cache_flag(c.status, S2D_CACHE_ABORTED);
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kTcRows));
+    }
+}
+
 // The pool as [page][head][position][element], boxes of one page's 64
 // positions x 64 elements with 128-byte swizzle.
 bool page_map(CUtensorMap *m, const S2dCacheView &c, void *base) {
@@ -777,7 +950,27 @@ cudaError_t launch(const S2dCacheView &c, const S2dCacheAttention &a, const Attn
     return cudaGetLastError();
 }
 
+template <typename Q, typename E, int HD>
+cudaError_t weigh(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
+    CUtensorMap mk;
+    if (!page_map(&mk, c, c.k)) return cudaErrorInvalidValue;
+    constexpr int smem = WeighShape<Q, HD>::kSmem;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = smem_limit(done, weigh_tc_kernel<Q, E, HD>, c.device, smem);
+    if (e) return e;
+    const dim3 grid((unsigned)((c.max_pages * kCachePage + kWeighSlots - 1) / kWeighSlots), (unsigned)c.n_seq, (unsigned)c.kv_heads);
+    weigh_tc_kernel<Q, E, HD><<<grid, 256, smem, s>>>(mk, c, a, p);
+    return cudaGetLastError();
+}
+
 }  // namespace
+
+cudaError_t launch_weigh_tc(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
+    const bool wide = c.head_dim == 128;
+    if (a.type == S2D_TYPE_F32) return wide ? weigh<float, __half, 128>(c, a, p, s) : weigh<float, __half, 64>(c, a, p, s);
+    if (a.type == S2D_TYPE_F16) return wide ? weigh<__half, __half, 128>(c, a, p, s) : weigh<__half, __half, 64>(c, a, p, s);
+    return wide ? weigh<__nv_bfloat16, __nv_bfloat16, 128>(c, a, p, s) : weigh<__nv_bfloat16, __nv_bfloat16, 64>(c, a, p, s);
+}
 
 cudaError_t launch_rows_tc(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
     const bool wide = c.head_dim == 128;
