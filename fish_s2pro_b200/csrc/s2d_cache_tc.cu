@@ -8,7 +8,8 @@
 //   P = 2^(s - m)    one thread per row, S read from TMEM, P written over it
 //   O += P V         P from TMEM, V from shared memory (MN-major), O in TMEM
 // The two row tiles alternate: while one is in its softmax, the tensor core
-// runs the products of the other.  One CTA per SM draws items from a counter,
+// runs the products of the other; an item of one row tile is walked by both
+// warpgroups in the same way, tile by tile in turn.  One CTA per SM draws items from a counter,
 // the longest first; one item's first loads run under the last one's epilogue.
 //
 // 16-bit queries: Q as it is, P rounded once to the cache's type (its relative
@@ -192,19 +193,22 @@ struct TcShape {
 };
 
 struct TcShared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2], item_full[2], item_empty[2];
+    uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2], item_full[2], item_empty[2], pair_full, pair_free;
     int item[2];
+    float2 ml[kTcRows];  // the second warpgroup's (m, l), where both take one row tile
     uint32_t tmem;
     int abort;
 };
 
 // What an item is: its rows, its positions, where its results go.
-template <int BN>
+template <int BN, bool DUAL>
 struct TcItem {
     int g, split, b, first, rows, r0, back;  // back: own slots before the sequence's first token
     int pre0, pre1, own0, own1;              // prefix positions and own slots of the item
-    int jp, J[2], nq;                        // prefix tiles; tiles of the row tiles; row tiles
-    bool pooled;
+    int jp, tiles, J[2];                     // prefix tiles; all tiles; those of each warpgroup
+    int last_q;                              // last row tile
+    // one row tile only: both warpgroups take it, with the even and the odd tiles (if the ring holds two tiles' loads)
+    bool pooled, dual;
 
     // own slots that rows [0, n) of the item see together
     __device__ __forceinline__ int seen(int n, int rep) const { return pooled ? 0 : max(0, back + (r0 + n - 1) / rep + 1); }
@@ -214,7 +218,7 @@ struct TcItem {
     // The fields of the MMA warp's loops, known to be alike in all lanes.
     __device__ __forceinline__ void uniform() {
         auto u = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
-        pre0 = u(pre0), pre1 = u(pre1), own0 = u(own0), own1 = u(own1), jp = u(jp), nq = u(nq), J[0] = u(J[0]), J[1] = u(J[1]);
+        pre0 = u(pre0), pre1 = u(pre1), own0 = u(own0), own1 = u(own1), jp = u(jp), tiles = u(tiles), last_q = u(last_q), dual = u(dual), J[0] = u(J[0]), J[1] = u(J[1]);
     }
 
     // false: nothing to do.  Called by whole warps.
@@ -243,15 +247,15 @@ struct TcItem {
         }
         if (rows <= 0) return false;
         rows = min(rows, kTcItemRows);
-        J[0] = J[1] = 0;
-        r0 = tile * kTcItemRows, nq = rows > kTcRows ? 2 : 1;
+        r0 = tile * kTcItemRows, last_q = rows > kTcRows, dual = DUAL && !last_q;
         if (!pooled) {
             const int span = seen(rows, p.rep), tiles = (span + BN - 1) / BN, per = (tiles + splits - 1) / splits;
             own0 = min(span, split * per * BN), own1 = min(span, own0 + per * BN);
         }
         jp = (pre1 - pre0 + BN - 1) / BN;
-        J[nq - 1] = jp + (own1 - own0 + BN - 1) / BN;
-        if (nq == 2) J[0] = jp + max(0, (min(seen(kTcRows, p.rep), own1) - own0 + BN - 1) / BN);
+        tiles = jp + (own1 - own0 + BN - 1) / BN;
+        J[0] = dual ? (tiles + 1) / 2 : !last_q ? tiles : jp + max(0, (min(seen(kTcRows, p.rep), own1) - own0 + BN - 1) / BN);
+        J[1] = dual ? tiles / 2 : last_q ? tiles : 0;
         return true;
     }
 };
@@ -277,6 +281,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < Sh::kSlots; ++i) mb_init(&sh.full[i], 1), mb_init(&sh.empty[i], 1);
         for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_full[i], 4), mb_init(&sh.pv_done[i], 1), mb_init(&sh.q_full[i], 4),
             mb_init(&sh.item_full[i], 1), mb_init(&sh.item_empty[i], 9);
+        mb_init(&sh.pair_full, 4), mb_init(&sh.pair_free, 4);
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (threadIdx.x == 0) cache_flag(c.status, S2D_CACHE_ABORTED);
         return;
     }
-    TcItem<BN> it;
+    TcItem<BN, (Sh::kSlots >= 5)> it;
 
     // The CTA's n-th item: its own block's, then what the loader drew from the
     // counter, through a ring of two.  For the MMA and softmax warps.
@@ -337,8 +342,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (!real) continue;
                 const int32_t *own_table = c.page_table + (int64_t)it.b * c.table_stride;
                 int ids = 0, have = -1;  // page ids 32 * have + lane of the current segment
-                const int J = it.J[it.nq - 1];
-                for (int j = 0; j < J && ok; ++j) {
+                for (int j = 0; j < it.tiles && ok; ++j) {
                     const bool own = j >= it.jp;
                     if (j == it.jp) have = -1;
                     const int32_t *table = own ? own_table : a.prefix_pages;
@@ -408,12 +412,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                  desc_k_sw128(k + half * Sh::kKvHalf + off), id_s, (uint32_t)(part != Sh::kSplit - 1 || kk > 0));
                     }
                 commit_one(one, &sh.s_full[q]);
-                if (q == it.nq - 1) commit_one(one, &sh.empty[load % Sh::kSlots]);
+                if (q == it.last_q || it.dual) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
             auto issue_pv = [&](int q, int j) {
                 const int load = 2 * (kv + j) + 1;
                 const uint32_t v = slot_base(load), d = tmem + Sh::kO + (uint32_t)(q * HD), pt = tmem + (uint32_t)(q * BN);
-                const bool fresh = Sh::kF32 ? j % Sh::kFlush == 0 : j == 0;
+                const int jj = it.dual ? j >> 1 : j;  // the warpgroup's own count
+                const bool fresh = Sh::kF32 ? jj % Sh::kFlush == 0 : jj == 0;
 #pragma unroll
                 for (int part = 0; part < Sh::kSplit; ++part)
 #pragma unroll
@@ -422,25 +427,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         umma_ts(one, d, pt + (uint32_t)(Sh::kF32 ? kk * 16 + part * 8 : kk * 8), desc_mn_sw128(v + (uint32_t)kk * 2048u, Sh::kKvHalf), id_o,
                                 (uint32_t)(!fresh || part || kk));
                 commit_one(one, &sh.pv_done[q]);
-                if (q == it.nq - 1) commit_one(one, &sh.empty[load % Sh::kSlots]);
+                if (q == it.last_q || it.dual) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
             for (int n = 0, item; ok && (ok = take(n, item)) && item < items; ++n) {
                 if (!it.get(c, a, p, item)) continue;
                 it.uniform();
-                const int nq = it.nq, J = it.J[nq - 1];
-                            for (int q = 0; q < nq && ok; ++q) {
+                const int J = it.tiles, step = it.dual ? 2 : 1;  // step: to the warpgroup's next tile
+                for (int q = 0; q < (it.dual ? 2 : it.last_q + 1) && ok; ++q) {
                     ok = wait(&sh.q_full[q], nitem[q]++ & 1);
                     tc_fence_after();
-                    if (ok && it.J[q] > 0 && (ok = slot_wait(2 * kv))) issue_s(q, 0);
+                    const int j = it.dual ? q : 0;
+                    if (ok && it.J[q] > 0 && (ok = slot_wait(2 * (kv + j)))) issue_s(q, j);
                 }
                 for (int j = 0; j < J && ok; ++j) {
                     const int load = 2 * (kv + j) + 1;
                     bool v_ready = false;
-                    for (int q = 0; q < nq && ok; ++q) {
-                        if (j >= it.J[q]) continue;
+                    for (int q = 0; q < 2 && ok; ++q) {
+                        if (it.dual ? (j & 1) != q : j >= it.J[q]) continue;
                         if (!(ok = wait(&sh.p_full[q], np[q]++ & 1))) break;
                         tc_fence_after();
-                        const bool more = j + 1 < it.J[q];
+                        const bool more = it.dual ? j + 2 < J : j + 1 < it.J[q];
                         if (!v_ready) {
                             if (!(ok = slot_wait(load))) break;
                             v_ready = true;
@@ -458,8 +464,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         issue_pv(q, j);
                         if (more) {
-                            if (!(ok = slot_wait(load + 1))) break;
-                            issue_s(q, j + 1);
+                            if (!(ok = slot_wait(2 * (kv + j + step)))) break;
+                            issue_s(q, j + step);
                         }
                     }
                 }
@@ -474,11 +480,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t st = lane_t + (uint32_t)(q * BN), ot = lane_t + Sh::kO + (uint32_t)(q * HD);
         const uint32_t qdst = sbase + (uint32_t)q * Sh::kQTile;
-        uint32_t ns = 0;  // S tiles taken so far; P V tiles done are as many
+        uint32_t ns = 0, nd = 0;  // S tiles taken so far (P V tiles done are as many); items shared by both warpgroups
         bool ok = true;
         for (int n = 0, item; ok && (ok = take(n, item)) && item < items; ++n) {
-            if (!it.get(c, a, p, item) || q >= it.nq) continue;
-            const int row = q * kTcRows + r, J = it.J[q];
+            if (!it.get(c, a, p, item) || (!it.dual && q > it.last_q)) continue;
+            const int tile0 = it.dual ? 0 : q * kTcRows, row = tile0 + r, J = it.J[q];  // tile0: the warpgroup's first row
             const bool real = row < it.rows;
             const int rr = it.r0 + (real ? row : 0), rt = row_token(p, rr), tok = it.first + rt, head = it.g * p.rep + rr - rt * p.rep;
             // The warp's 32 query rows, 16 bytes a lane with a row's lanes side by
@@ -497,7 +503,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint4 qv[kAtOnce];
 #pragma unroll
                 for (int i = 0; i < kAtOnce; ++i) {
-                    const int w = q * kTcRows + 32 * (warp & 3) + (i0 + i) * kTogether + lane / kLanes, wr = it.r0 + w, wt = row_token(p, wr);
+                    const int w = tile0 + 32 * (warp & 3) + (i0 + i) * kTogether + lane / kLanes, wr = it.r0 + w, wt = row_token(p, wr);
                     const Q *src = static_cast<const Q *>(a.q) + (int64_t)(it.first + wt) * a.q_stride + (int64_t)(it.g * p.rep + wr - wt * p.rep) * HD;
                     qv[i] = w < it.rows ? reinterpret_cast<const uint4 *>(src)[c16] : make_uint4(0, 0, 0, 0);
                 }
@@ -561,7 +567,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
             };
-            for (int j = 0; j < J; ++j, ++ns) {
+            for (int jj = 0; jj < J; ++jj, ++ns) {
+                const int j = it.dual ? 2 * jj + q : jj;
                 if (!(ok = warp_wait(&sh.s_full[q], ns & 1, abort_v))) break;
                 tc_fence_after();
                 const int vis = !real ? BN : j < it.jp ? it.pre1 - it.pre0 - j * BN : own_limit - (j - it.jp) * BN;
@@ -588,15 +595,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const bool up = mx > mref + 14.f;
                 const float mnew = up ? mx - 6.f : mref;
                 const float corr = up && mref > -INFINITY ? ex2(mref - mnew) : 1.f;
-                const bool rescale = j > 0 && __any_sync(0xffffffffu, corr != 1.f);
-                if (j > 0) {
+                const bool rescale = jj > 0 && __any_sync(0xffffffffu, corr != 1.f);
+                if (jj > 0) {
                     // P and O are free once P V of the last tile is done
                     ok = warp_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v);
                     if (!ok) break;
                     tc_fence_after();
                 }
                 if constexpr (Sh::kF32) {
-                    if (j > 0 && (rescale || j % Sh::kFlush == 0)) flush(j % Sh::kFlush != 0);
+                    if (jj > 0 && (rescale || jj % Sh::kFlush == 0)) flush(jj % Sh::kFlush != 0);
                     if (rescale) {
 #pragma unroll
                         for (int i = 0; i < HD; ++i) acc[i] *= corr;
@@ -659,6 +666,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!ok) break;
             tc_fence_after();
             if (J > 0) flush(false);
+            float mine = 1.f, other = 0.f;  // what this warpgroup's and the other's O count
+            if (it.dual) {
+                // the second warpgroup's part goes to the first, which shares its TMEM lanes: O is there (f32: put there), (m, l)
+                // through shared memory
+                if (q == 1) {
+                    if constexpr (Sh::kF32) {
+#pragma unroll
+                        for (int i = 0; i < HD; i += 32) {
+                            uint32_t o[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(acc[i + e]);
+                            tmem_st32(ot + i, o);
+                        }
+                        tmem_wait_st();
+                    }
+                    sh.ml[r] = make_float2(mref, l);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mb_arrive(&sh.pair_full);
+                    // until the first has read it
+                    if (!(ok = warp_wait(&sh.pair_free, nd++ & 1, abort_v))) break;
+                    continue;
+                }
+                if (!(ok = warp_wait(&sh.pair_full, nd++ & 1, abort_v))) break;
+                tc_fence_after();
+                const float2 b = sh.ml[r];
+                const float m = fmaxf(mref, b.x);
+                mine = part_factor(mref, l, m), other = part_factor(b.x, b.y, m);
+                l = l * mine + b.y * other, mref = m;
+            }
             const int64_t id = (int64_t)tok * a.heads + head;
             const bool parts = p.parts > 0;
             const int part = it.pooled ? it.split : p.prefix_splits + it.split;
@@ -687,7 +724,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         float o[32];
                         if constexpr (Sh::kF32) {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = acc[i + e] * inv;
+                            for (int e = 0; e < 32; ++e) o[e] = acc[i + e] * (mine * inv);
                         } else {
                             uint32_t raw_o[32];
 #pragma unroll
@@ -697,7 +734,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 tmem_wait_ld();
                             }
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(raw_o[e]) * inv;
+                            for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(raw_o[e]) * (mine * inv);
+                        }
+                        if (it.dual && it.J[1] > 0) {
+                            uint32_t two_o[32];
+                            tmem_ld(ot + HD + i, two_o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = fmaf(__uint_as_float(two_o[e]), other * inv, o[e]);
                         }
 #pragma unroll
                         for (int e = 0; e < 32; e += kEach) {
@@ -715,11 +759,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     __syncwarp();
 #pragma unroll 4
                     for (int i = 0; i < 32; i += kRows) {
-                        const int mine = 32 * (warp & 3) + i + lane / kChunks, w = q * kTcRows + mine, ch = lane % kChunks;
+                        const int tr = 32 * (warp & 3) + i + lane / kChunks, w = tile0 + tr, ch = lane % kChunks;
                         uint32_t x[4];
                         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                                      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                                     : "r"(qdst + (uint32_t)((ch >> 3) * Sh::kQHalf) + swizzle(mine, ch & 7))
+                                     : "r"(qdst + (uint32_t)((ch >> 3) * Sh::kQHalf) + swizzle(tr, ch & 7))
                                      : "memory");
                         if (w < it.rows) *reinterpret_cast<uint4 *>(to_rows + row_offset(it.r0 + w) + c0 + ch * kEach) = make_uint4(x[0], x[1], x[2], x[3]);
                     }
@@ -732,6 +776,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             };
             if (parts) store(p.part + part * HD, [&](int wr) { return at_row(wr, (int64_t)a.heads * p.parts * HD, p.parts * HD); });
             else store(static_cast<Q *>(a.out), [&](int wr) { return at_row(wr, a.out_stride, HD); });
+            if (it.dual) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&sh.pair_free);
+            }
         }
         if (!ok) *abort_v = 1;
     }
