@@ -12,6 +12,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include <algorithm>
 
 namespace s2d {
@@ -56,10 +58,6 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-__device__ __forceinline__ void store_out(float *p, float x) { *p = x; }
-__device__ __forceinline__ void store_out(__half *p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void store_out(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
 __device__ __forceinline__ void store_out4(float *p, const float (&x)[4]) {
     *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
@@ -145,7 +143,7 @@ __device__ __forceinline__ void load_q(const Q *row, float scale, int t, uint32_
     }
 }
 
-constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots
+constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots: parts of a row are at most as many and two
 
 // Single tokens: the rep <= 8 query heads of one (sequence, KV head) against
 // the sequence's own slots, shared by the CTAs of a cluster (chunks of 16
@@ -154,9 +152,8 @@ constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots
 // the remainders of what the cache's type rounds (f32 queries, and the weights
 // of every type), so the sums have f32's precision at no extra MMA.
 //
-// The CTAs' parts meet through distributed shared memory, together with the
-// prefix's parts from the workspace: the call needs no kernel to join them.
-// When weighing, the scores stay in shared memory until the row's sum over
+// The CTAs' parts meet through distributed shared memory; without a prefix the
+// call needs no kernel to join them.  When weighing, the scores stay in shared memory until the row's sum over
 // prefix and own slots is known, and each CTA adds its slots' weights to the
 // mass: the keys are read once and no score leaves the SM.
 template <typename Q, typename E, int HD>
@@ -290,7 +287,13 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
         if (d == 0) s_ml[row] = make_float2(m, l);
         s_o[row * HD + d] = sum;
     }
-    if (p.parts) grid_dep_wait();  // the prefix's parts are in the workspace
+    // With a prefix and kept scores the row's sum is needed here: wait for the
+    // prefix's parts.  With a prefix alone the own part goes to the workspace
+    // like the others, for the join kernel: no block holds its SM until the
+    // prefix is done, but the last one, so that the grid ends after it.
+    const bool late = p.parts && !keep;
+    const int parts = late ? 0 : p.parts;  // prefix parts that are joined here
+    if (p.parts && (keep || blockIdx.x == gridDim.x - 1)) grid_dep_wait();
     cluster_sync(S);
 
     // what every part counts in the row's softmax: ranks, then prefix parts
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
         const float2 none = make_float2(-INFINITY, 0.f);
         float2 mine = none, pre[kMaxParts / 32];
 #pragma unroll
-        for (int i = 0; i < kMaxParts / 32; ++i) pre[i] = lane + 32 * i < p.parts ? __ldcg(&p.ml[id * p.parts + lane + 32 * i]) : none;
+        for (int i = 0; i < kMaxParts / 32; ++i) pre[i] = lane + 32 * i < parts ? __ldcg(&p.ml[id * p.parts + lane + 32 * i]) : none;
         if (lane < S) mine = cluster_get(&s_ml[row], lane, S);
         float m = mine.x;
 #pragma unroll
@@ -310,15 +313,16 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
 #pragma unroll
         for (int i = 0; i < kMaxParts / 32; ++i) fp[i] = part_factor(pre[i].x, pre[i].y, m), l = fmaf(pre[i].y, fp[i], l);
         l = warp_sum(l);
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
+        const float inv = late ? 1.f : l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
         if (lane < S) s_rank[row][lane] = f * inv;
 #pragma unroll
         for (int i = 0; i < kMaxParts / 32; ++i)
-            if (lane + 32 * i < p.parts) s_pre[row * p.parts + lane + 32 * i] = fp[i] * inv;
+            if (lane + 32 * i < parts) s_pre[row * p.parts + lane + 32 * i] = fp[i] * inv;
         if (lane == 0) {
             const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
             s_lse[row] = l == 0.f ? 0.f : lse2;
-            if (rank == 0) {
+            if (late && rank == 0) p.ml[id * p.parts + p.parts - 1] = make_float2(m, l);
+            if (!late && rank == 0) {
                 if (a.lse) a.lse[id] = lse2 * kLn2;
                 if (p.lse2) p.lse2[id] = lse2;
             }
@@ -335,16 +339,17 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
         };
         for (int k = 0; k < S; ++k) add(cluster_get(reinterpret_cast<const float4 *>(&s_o[row * HD + d]), k, S), s_rank[row][k]);
         const float4 *part = reinterpret_cast<const float4 *>(p.part + id * p.parts * HD + d);
-        for (int k0 = 0; k0 < p.parts; k0 += 8) {  // eight parts in flight
+        for (int k0 = 0; k0 < parts; k0 += 8) {  // eight parts in flight
             float4 v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (k0 + k < p.parts) v[k] = __ldcg(part + (k0 + k) * (HD / 4));
+                if (k0 + k < parts) v[k] = __ldcg(part + (k0 + k) * (HD / 4));
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (k0 + k < p.parts) add(v[k], s_pre[row * p.parts + k0 + k]);
+                if (k0 + k < parts) add(v[k], s_pre[row * p.parts + k0 + k]);
         }
-        store_out4(static_cast<Q *>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + row) * HD + d, sum);
+        if (late) store_out4(p.part + (id * p.parts + p.parts - 1) * HD + d, sum);
+        else store_out4(static_cast<Q *>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + row) * HD + d, sum);
     }
     if (keep) {
         float *mass = c.mass + ((int64_t)b * G + g) * c.max_pages * kCachePage;
@@ -357,28 +362,53 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
     cluster_sync(S);  // no CTA leaves while another may read its part
 }
 
-// One warp per (token, head): joins its parts in their order.
+// One warp per (token, head): joins its parts, eight in flight, in their order.
 template <typename Q, int HD>
 __global__ void __launch_bounds__(128) join_kernel(const S2dCacheView c, const S2dCacheAttention a, const AttnPlan p) {
+    constexpr int V = HD / 32;  // elements of a lane
+    using Vec = std::conditional_t<V == 4, float4, float2>;
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
+    grid_dep_wait();
     if (id >= (int64_t)real_tokens(a, c.n_seq) * a.heads) return;
     const int64_t tok = id / a.heads;
     const int head = (int)(id % a.heads);
-    const float2 *ml = p.ml + id * p.parts;
-    const float *part = p.part + id * p.parts * HD;
-    float m = -INFINITY, l = 0.f, o[HD / 32] = {};
-    for (int k = 0; k < p.parts; ++k) m = fmaxf(m, ml[k].x);
-    for (int k = 0; k < p.parts; ++k) {
-        const float f = part_factor(ml[k].x, ml[k].y, m);
-        l = fmaf(ml[k].y, f, l);
+    const Vec *part = reinterpret_cast<const Vec *>(p.part + id * p.parts * HD) + lane;
+    float m = -INFINITY;
+    for (int k = lane; k < p.parts; k += 32) m = fmaxf(m, p.ml[id * p.parts + k].x);
+    m = warp_max(m);
+    float l = 0.f, o[V] = {};
+    for (int k0 = 0; k0 < p.parts; k0 += 32) {
+        // lane k holds part k0 + k's share
+        const float2 e = k0 + lane < p.parts ? p.ml[id * p.parts + k0 + lane] : make_float2(-INFINITY, 0.f);
+        const float f = part_factor(e.x, e.y, m);
+        l += warp_sum(e.y * f);
+        for (int k1 = 0; k1 < min(32, p.parts - k0); k1 += 8) {
+            Vec v[8];
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(part[k * HD + lane + 32 * i], f, o[i]);
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k1 + k < p.parts) v[k] = part[(int64_t)(k0 + k1 + k) * 32];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, k1 + k);
+                if (k0 + k1 + k < p.parts) {
+                    const float *x = reinterpret_cast<const float *>(&v[k]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] = fmaf(x[i], fk, o[i]);
+                }
+            }
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
-    Q *out = static_cast<Q *>(a.out) + tok * a.out_stride + (int64_t)head * HD;
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) store_out(out + lane + 32 * i, o[i] * inv);
+    for (int i = 0; i < V; ++i) o[i] *= inv;
+    Q *out = static_cast<Q *>(a.out) + tok * a.out_stride + (int64_t)head * HD + V * lane;
+    if constexpr (V == 4) {
+        store_out4(out, o);
+    } else {
+        if constexpr (sizeof(Q) == 4) *reinterpret_cast<float2 *>(out) = make_float2(o[0], o[1]);
+        else *reinterpret_cast<uint32_t *>(out) = pack2<Q>(o[0], o[1]);
+    }
     if (lane == 0) {
         const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
         if (a.lse) a.lse[id] = lse2 * kLn2;
@@ -450,6 +480,7 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
         p.own_splits = 1;
         while (p.own_splits < kMaxCluster && items * p.own_splits < 4 * kSms && c.max_pages > 8 * p.own_splits) p.own_splits *= 2;
         p.parts = p.prefix_splits;
+        if (p.parts && !score_pitch(c, a, p)) ++p.parts;  // the own part goes with them
     } else {
         const int64_t own = rows / kTcTile + std::min<int64_t>(c.n_seq, rows);  // sum of ceil(rows of b / 256) is no more
         const bool fill = own * c.kv_heads >= kSms;
@@ -504,12 +535,9 @@ template <typename Q, typename E, int HD>
 cudaError_t attention_launch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
     cudaError_t e = cudaSuccess;
     if (p.prefix_tiles || p.own_tiles) e = launch_rows_tc(c, a, p, s);
-    if (!e && !a.q_start) {
-        e = token_launch<Q, E, HD>(c, a, p, s);
-    } else if (!e && p.parts) {
-        join_kernel<Q, HD><<<(unsigned)(((int64_t)a.tokens * a.heads + 3) / 4), 128, 0, s>>>(c, a, p);
-        e = cudaGetLastError();
-    }
+    if (!e && !a.q_start) e = token_launch<Q, E, HD>(c, a, p, s);
+    if (!e && p.parts && (a.q_start || !score_pitch(c, a, p)))
+        e = s2d_launch(join_kernel<Q, HD>, dim3((unsigned)(((int64_t)a.tokens * a.heads + 3) / 4)), dim3(128), 0, s, true, c, a, p);
     if (e || !p.lse2) return e;
     return launch_weigh_tc(c, a, p, s);
 }
