@@ -41,6 +41,10 @@ template <>
 __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
 }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 __device__ __forceinline__ void cache_flag(int32_t *status, int bits) {
     if (status) atomicOr(status, bits);
 }

@@ -83,6 +83,15 @@ __device__ __forceinline__ void commit_one(uint32_t one, uint64_t *bar) {
 }
 #define S2D_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define S2D_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void lds16(uint32_t addr, float (&x)[4]) {
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void sts16(uint32_t addr, const uint32_t (&x)[4]) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+}
 // One thread of the warp, the same one each time.
 __device__ __forceinline__ uint32_t elect() {
     uint32_t yes;
@@ -488,57 +497,64 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const bool real = row < it.rows;
             const int rr = it.r0 + (real ? row : 0), rt = row_token(p, rr), tok = it.first + rt, head = it.g * p.rep + rr - rt * p.rep;
             // The warp's 32 query rows, 16 bytes a lane with a row's lanes side by
-            // side, up to sixteen loads in flight at once.  Their sign takes the scale's,
-            // so that the scores' maximum is that of q . k.  Compact loops, here
-            // and below: code that runs once an item comes from L2, at about six
-            // cycles an instruction.
+            // side, all in flight at once.  Compact loops, here and below: code
+            // that runs once an item comes from L2, at about six cycles an
+            // instruction.
             constexpr int kLanes = HD * (int)sizeof(Q) / 16, kTogether = 32 / kLanes;  // lanes of a row, rows of a load
-            float qmul = fabsf(a.scale) * kLog2e;
-            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            auto q_slot = [&](int w, int slot) { return qdst + (uint32_t)((slot >> 3) * Sh::kQHalf) + swizzle(32 * (warp & 3) + w, slot & 7); };
             const int c16 = lane % kLanes;  // 16-byte chunk of the row
-            int my_ex = 0;
-            constexpr int kAtOnce = kLanes < 16 ? kLanes : 16;
-#pragma unroll 1
-            for (int i0 = 0; i0 < kLanes; i0 += kAtOnce) {
-                uint4 qv[kAtOnce];
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const int w = tile0 + 32 * (warp & 3) + (i0 + i) * kTogether + lane / kLanes, wr = it.r0 + w, wt = row_token(p, wr);
-                    const Q *src = static_cast<const Q *>(a.q) + (int64_t)(it.first + wt) * a.q_stride + (int64_t)(it.g * p.rep + wr - wt * p.rep) * HD;
-                    qv[i] = w < it.rows ? reinterpret_cast<const uint4 *>(src)[c16] : make_uint4(0, 0, 0, 0);
+            // 16-bit: chunk c to its place.  f32: chunks 2k and 2k + 1 to where their elements' hi and lo will be.
+            const int to_slot = Sh::kF32 ? (c16 & 1) * (kLanes / 2) + (c16 >> 1) : c16;
+#pragma unroll 4
+            for (int i = 0; i < kLanes; ++i) {
+                const int w = i * kTogether + lane / kLanes, wr = it.r0 + tile0 + 32 * (warp & 3) + w, wt = row_token(p, wr);
+                const bool is = tile0 + 32 * (warp & 3) + w < it.rows;
+                const Q *src = static_cast<const Q *>(a.q);
+                if (is) src += (int64_t)(it.first + wt) * a.q_stride + (int64_t)(it.g * p.rep + wr - wt * p.rep) * HD + c16 * (16 / (int)sizeof(Q));
+                cp_async16(q_slot(w, to_slot), src, is);
+            }
+            cp_commit();
+            cp_wait<0>();
+            __syncwarp();
+            // Scores are taken with |scale|: the rows' sign takes the scale's, so
+            // that their maximum is that of q . k.
+            float qmul = fabsf(a.scale) * kLog2e;
+            if constexpr (Sh::kF32) {
+                // a thread splits its row into hi + lo, scaled by the power of two that puts its largest element near 2^14: the
+                // remainders stay normal f16 (at most by 2^114, which keeps rows of subnormal numbers finite)
+                float amax = 0.f;
+#pragma unroll 4
+                for (int k = 0; k < kLanes; ++k) {
+                    float x[4];
+                    lds16(q_slot(lane, k), x);
+                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
                 }
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const int w = 32 * (warp & 3) + (i0 + i) * kTogether + lane / kLanes;  // row of the tile
-                    if constexpr (Sh::kF32) {
-                        // scaled by the power of two that puts the row's largest element near 2^14: the remainders stay normal
-                        // f16 (at most by 2^114, which keeps rows of subnormal numbers finite)
-                        const float x[4] = {__uint_as_float(qv[i].x), __uint_as_float(qv[i].y), __uint_as_float(qv[i].z), __uint_as_float(qv[i].w)};
-                        float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-                        for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                        const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);
-#pragma unroll
-                        for (int k = 0; k < kTogether; ++k) {
-                            const int e = kTogether == 1 ? ex : __shfl_sync(0xffffffffu, ex, k * kLanes);
-                            if (lane == (i0 + i) * kTogether + k) my_ex = e;
-                        }
-                        const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - ex) << 23), a.scale);
-                        uint32_t hi[2], lo[2];
-                        split2<E>(x[0] * up, x[1] * up, hi[0], lo[0]);
-                        split2<E>(x[2] * up, x[3] * up, hi[1], lo[1]);
-                        const uint32_t at = qdst + (uint32_t)((c16 >> 4) * Sh::kQHalf) + swizzle(w, (c16 >> 1) & 7) + (c16 & 1) * 8;
-                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
-                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]) : "memory");
-                    } else {
-                        const uint32_t at = qdst + (uint32_t)((c16 >> 3) * Sh::kQHalf) + swizzle(w, c16 & 7);
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(qv[i].x ^ flip), "r"(qv[i].y ^ flip), "r"(qv[i].z ^ flip),
-                                     "r"(qv[i].w ^ flip)
-                                     : "memory");
-                    }
+                const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);
+                const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - ex) << 23), a.scale);
+                qmul *= __uint_as_float((uint32_t)(127 + ex - 14) << 23);
+#pragma unroll 2
+                for (int k = 0; k < kLanes / 2; ++k) {
+                    float x[4], y[4];
+                    uint32_t hi[4], lo[4];
+                    lds16(q_slot(lane, k), x);
+                    lds16(q_slot(lane, kLanes / 2 + k), y);
+                    split2<E>(x[0] * up, x[1] * up, hi[0], lo[0]);
+                    split2<E>(x[2] * up, x[3] * up, hi[1], lo[1]);
+                    split2<E>(y[0] * up, y[1] * up, hi[2], lo[2]);
+                    split2<E>(y[2] * up, y[3] * up, hi[3], lo[3]);
+                    sts16(q_slot(lane, k), hi);
+                    sts16(q_slot(lane, kLanes / 2 + k), lo);
+                }
+            } else if (a.scale < 0.f) {
+#pragma unroll 1
+                for (int k = 0; k < kLanes; ++k) {
+                    float x[4];
+                    lds16(q_slot(lane, k), x);
+                    const uint32_t y[4] = {__float_as_uint(x[0]) ^ 0x80008000u, __float_as_uint(x[1]) ^ 0x80008000u, __float_as_uint(x[2]) ^ 0x80008000u,
+                                           __float_as_uint(x[3]) ^ 0x80008000u};
+                    sts16(q_slot(lane, k), y);
                 }
             }
-            if constexpr (Sh::kF32) qmul *= __uint_as_float((uint32_t)(127 + my_ex - 14) << 23);
             qmul = fmaxf(qmul, 1e-38f);  // a masked score stays -inf when the scale is 0
             fence_proxy_async_smem();
             __syncwarp();
@@ -752,20 +768,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 if constexpr (sizeof(O) == 4) w[x] = __float_as_uint(o[e + x]);
                                 else w[x] = pack2<O>(o[e + 2 * x], o[e + 2 * x + 1]);
                             }
-                            const uint32_t at = qdst + (uint32_t)((ch >> 3) * Sh::kQHalf) + swizzle(r, ch & 7);
-                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                            sts16(q_slot(lane, ch), w);
                         }
                     }
                     __syncwarp();
 #pragma unroll 4
                     for (int i = 0; i < 32; i += kRows) {
                         const int tr = 32 * (warp & 3) + i + lane / kChunks, w = tile0 + tr, ch = lane % kChunks;
-                        uint32_t x[4];
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                                     : "r"(qdst + (uint32_t)((ch >> 3) * Sh::kQHalf) + swizzle(tr, ch & 7))
-                                     : "memory");
-                        if (w < it.rows) *reinterpret_cast<uint4 *>(to_rows + row_offset(it.r0 + w) + c0 + ch * kEach) = make_uint4(x[0], x[1], x[2], x[3]);
+                        float x[4];
+                        lds16(q_slot(tr - 32 * (warp & 3), ch), x);
+                        if (w < it.rows) *reinterpret_cast<uint4 *>(to_rows + row_offset(it.r0 + w) + c0 + ch * kEach) =
+                            make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
                     }
                     __syncwarp();
                 }
