@@ -97,48 +97,54 @@ __device__ __forceinline__ T cluster_get(const T *p, int rank, int size) {
     return v;
 }
 
-// The query row of a lane's MMA row (g = lane / 4), as A fragments: rows g
-// hold q (its rounding to the cache's type if q is f32), rows g + 8 the f32
-// remainder.  f32 rows are scaled by the power of two that puts their largest
-// element near 2^14, so that the remainder stays a normal f16; qmul takes it
-// out of the scores again, along with scale * log2(e).
+// The query row of a lane's MMA row (g = lane / 4, t = lane % 4), as A
+// fragments: rows g hold q (its rounding to the cache's type if q is f32), rows
+// g + 8 the f32 remainder.  f32 rows are scaled by the power of two that puts
+// their largest element near 2^14, so that the remainder stays a normal f16
+// (at most by 2^114, which keeps rows of subnormal numbers finite); qmul takes
+// it out of the scores again, along with scale * log2(e).
 template <typename Q, typename E, int HD>
-__device__ __forceinline__ void load_q(const Q *row, float scale, int t, uint32_t (&qa)[HD / 16][4], float &qmul) {
-    if constexpr (sizeof(Q) == 4) {
-        float qv[HD / 16][4], amax = 0.f;
+struct QueryRow {
+    uint2 raw[HD / 16][2];  // elements 16 k + 2 t and 16 k + 2 t + 8 with the next, under way (f32: two words; else one)
+
+    __device__ __forceinline__ void load(const Q *row, int t) {
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-            float2 v0 = make_float2(0.f, 0.f), v1 = v0;
-            if (row) {
-                v0 = *reinterpret_cast<const float2 *>(row + 16 * k + 2 * t);
-                v1 = *reinterpret_cast<const float2 *>(row + 16 * k + 2 * t + 8);
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const Q *at = row + 16 * k + 8 * i + 2 * t;
+                raw[k][i] = make_uint2(0u, 0u);
+                if (!row) continue;
+                if constexpr (sizeof(Q) == 4) raw[k][i] = *reinterpret_cast<const uint2 *>(at);
+                else raw[k][i].x = *reinterpret_cast<const uint32_t *>(at);
             }
-            qv[k][0] = v0.x, qv[k][1] = v0.y, qv[k][2] = v1.x, qv[k][3] = v1.y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(qv[k][e]));
-        }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        int ex = 0;
-        frexpf(amax, &ex);
-        ex = max(ex, -100);  // 2^(14 - ex) stays finite for the smallest rows
-        const float up = ldexpf(1.f, 14 - ex);
-        qmul = scale * kLog2e * ldexpf(1.f, ex - 14);
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-            split2<E>(qv[k][0] * up, qv[k][1] * up, qa[k][0], qa[k][1]);
-            split2<E>(qv[k][2] * up, qv[k][3] * up, qa[k][2], qa[k][3]);
-        }
-    } else {
+    }
+    __device__ __forceinline__ void fragments(float scale, uint32_t (&qa)[HD / 16][4], float &qmul) const {
         qmul = scale * kLog2e;
+        if constexpr (sizeof(Q) == 4) {
+            float amax = 0.f;
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-            qa[k][0] = row ? *reinterpret_cast<const uint32_t *>(row + 16 * k + 2 * t) : 0u;
-            qa[k][2] = row ? *reinterpret_cast<const uint32_t *>(row + 16 * k + 2 * t + 8) : 0u;
-            qa[k][1] = qa[k][3] = 0u;
+            for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(raw[k][i].x)), fabsf(__uint_as_float(raw[k][i].y))));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);
+            const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+            qmul *= __uint_as_float((uint32_t)(127 + ex - 14) << 23);
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    split2<E>(__uint_as_float(raw[k][i].x) * up, __uint_as_float(raw[k][i].y) * up, qa[k][2 * i], qa[k][2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) qa[k][2 * i] = raw[k][i].x, qa[k][2 * i + 1] = 0u;
         }
     }
-}
+};
 
 constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots: parts of a row are at most as many and two
 
@@ -170,21 +176,35 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
     item /= groups;
     const int g = item % G, b = item / G;
     const int head0 = g * p.rep + grp * R, n_rows = min(R, p.rep - grp * R);
-    const int n = cache_length(c, b), nch = (n + KC - 1) / KC, per = (nch + S - 1) / S;
-    const int ch0 = min(nch, rank * per), ch1 = min(nch, ch0 + per);
     const int32_t *table = c.page_table + (int64_t)b * c.table_stride;
     const bool keep = score_pitch > 0;
+    // what the first copies and scores wait for, all under way together: the
+    // length, 32 page ids (id `lane` of a window, read again as the window
+    // moves on), the query rows
+    int ids = __ldg(table + min(lane, c.max_pages - 1)), window = 0;
+    QueryRow<Q, E, HD> query;
+    query.load(gl < n_rows ? static_cast<const Q *>(a.q) + (int64_t)b * a.q_stride + (int64_t)(head0 + gl) * HD : nullptr, t);
+    const int n = cache_length(c, b), nch = (n + KC - 1) / KC, per = (nch + S - 1) / S;
+    const int ch0 = min(nch, rank * per), ch1 = min(nch, ch0 + per);
 
     uint8_t *ring = sm + (size_t)warp * 2 * STAGE;
     auto issue = [&](int ch, int stage) {
         uint8_t *kt = ring + (size_t)stage * STAGE, *vt = kt + KC * PITCH;
-        const int64_t at = cache_row(c, table, g, ch * KC);  // a chunk never spans two pages
-        const int have = at < 0 ? 0 : min(KC, n - ch * KC);
-        const char *ks = static_cast<const char *>(c.k) + 2 * max(at, (int64_t)0), *vs = static_cast<const char *>(c.v) + 2 * max(at, (int64_t)0);
+        const int at_page = ch * KC / kCachePage;  // a chunk never spans two pages
+        if (at_page / 32 != window) {
+            window = at_page / 32;
+            ids = __ldg(table + min(window * 32 + lane, c.max_pages - 1));
+        }
+        const int page = __shfl_sync(0xffffffffu, ids, at_page & 31);
+        const bool good = (uint32_t)page < (uint32_t)c.n_pages;
+        if (!good) cache_flag(c.status, S2D_CACHE_BAD_PAGE);
+        const int have = good ? min(KC, n - ch * KC) : 0;
+        const int64_t at = (int64_t)(good ? page : 0) * c.page_stride + (int64_t)g * c.head_stride + (int64_t)(ch * KC % kCachePage) * HD;
+        const char *ks = static_cast<const char *>(c.k) + 2 * at, *vs = static_cast<const char *>(c.v) + 2 * at;
 #pragma unroll
         for (int i = 0; i < KC * UNITS / 32; ++i) {
             const int u = lane + 32 * i, row = u / UNITS, cc = u % UNITS;
-            const int64_t src = (int64_t)(row < have ? row : 0) * (HD * 2) + cc * 16;
+            const int src = (row < have ? row : 0) * (HD * 2) + cc * 16;
             cp_async16(kt + row * PITCH + cc * 16, ks + src, row < have);
             cp_async16(vt + row * PITCH + cc * 16, vs + src, row < have);
         }
@@ -195,7 +215,7 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
     if (ch < ch1) have = issue(ch, 0);
     uint32_t qa[HD / 16][4];
     float qmul;
-    load_q<Q, E, HD>(gl < n_rows ? static_cast<const Q *>(a.q) + (int64_t)b * a.q_stride + (int64_t)(head0 + gl) * HD : nullptr, a.scale, t, qa, qmul);
+    query.fragments(a.scale, qa, qmul);
 
     float o[NO][4];
 #pragma unroll

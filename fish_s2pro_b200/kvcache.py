@@ -139,6 +139,7 @@ class PagedKvCache:
             raise _bad("every buffer must be on the cache's device")
         self.k, self.v, self.page_table, self.lengths, self.positions, self.mass = k, v, page_table, lengths, positions, mass
         self.dtype = k.dtype
+        self._scale = 1.0 / math.sqrt(self.head_dim)
         self._types = {k.dtype: 1 if k.dtype == torch.float16 else 30}
         if k.dtype == torch.float16:
             self._types[torch.float32] = 0
@@ -178,6 +179,15 @@ class PagedKvCache:
         if t.requires_grad and self._torch.is_grad_enabled():
             raise _bad(f"{name} requires a gradient: the cache operators have no backward pass")
         return t.data_ptr(), step if s[0] > 1 else s[1] * s[2]
+
+    def _like_q(self, q, out):
+        """The output for q, new if none is given: (tensor, pointer, token stride)."""
+        if out is None:
+            out = q.new_empty(q.shape)
+            return out, out.data_ptr(), q.shape[1] * q.shape[2]
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise _bad("out must be like q")
+        return (out, *self._rows("out", out))
 
     def _type(self, name, t):
         code = self._types.get(t.dtype)
@@ -220,11 +230,7 @@ class PagedKvCache:
         vp, vs = self._rows("v", v, self.kv_heads)
         if k.shape[0] != tokens or v.shape[0] != tokens:
             raise _bad("q, k and v must have the same tokens")
-        if out is None:
-            out = q.new_empty(q.shape)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise _bad("out must be like q")
-        op, os_ = self._rows("out", out)
+        out, op, os_ = self._like_q(q, out)
         gains = [None if t is None else self._dense(n, t, self._torch.float32, (self.head_dim,))
                  for n, t in (("q_norm", q_norm), ("k_norm", k_norm))]
         a = _Append(qp, kp, vp, qs, ks, vs, op, os_, gains[0], gains[1], self._ints("pos", pos, (tokens,)),
@@ -249,11 +255,7 @@ class PagedKvCache:
         qp, qs = self._rows("q", q)
         tokens, heads = q.shape[0], q.shape[1]
         torch = self._torch
-        if out is None:
-            out = q.new_empty(q.shape)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise _bad("out must be like q")
-        op, os_ = self._rows("out", out)
+        out, op, os_ = self._like_q(q, out)
         lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
         prefix = None
         if prefix_len:
@@ -262,7 +264,7 @@ class PagedKvCache:
             prefix = self._ints("prefix_pages", prefix_pages, tuple(prefix_pages.shape))
         a = _Attention(qp, qs, op, os_, lse.data_ptr() if return_lse else None, self._starts(q_start, tokens), prefix,
                        prefix_len, tokens, heads, ty, 1 if weigh else 0,
-                       1.0 / math.sqrt(self.head_dim) if scale is None else scale, None, 0)
+                       self._scale if scale is None else scale, None, 0)
         key = (tokens, heads, prefix_len, ty, weigh, q_start is None)
         need = self._sizes.get(key)
         if need is None:
