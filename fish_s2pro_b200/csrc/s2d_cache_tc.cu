@@ -202,7 +202,7 @@ struct TcShape {
 };
 
 struct TcShared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2], item_full[2], item_empty[2], pair_full, pair_free;
+    uint64_t full[8], empty[8], s_full[2], p_half[2][2], pv_done[2], q_full[2], item_full[2], item_empty[2], pair_full, pair_free;
     int item[2];
     float2 ml[kTcRows];  // the second warpgroup's (m, l), where both take one row tile
     uint32_t tmem;
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     grid_dep_launch();  // every CTA is resident: what follows may use what they leave of the GPU
     if (threadIdx.x == 0) {
         for (int i = 0; i < Sh::kSlots; ++i) mb_init(&sh.full[i], 1), mb_init(&sh.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_full[i], 4), mb_init(&sh.pv_done[i], 1), mb_init(&sh.q_full[i], 4),
+        for (int i = 0; i < 2; ++i) mb_init(&sh.s_full[i], 1), mb_init(&sh.p_half[i][0], 4), mb_init(&sh.p_half[i][1], 4), mb_init(&sh.pv_done[i], 1), mb_init(&sh.q_full[i], 4),
             mb_init(&sh.item_full[i], 1), mb_init(&sh.item_empty[i], 9);
         mb_init(&sh.pair_full, 4), mb_init(&sh.pair_free, 4);
         sh.abort = 0;
@@ -423,18 +423,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 commit_one(one, &sh.s_full[q]);
                 if (q == it.last_q || it.dual) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
-            auto issue_pv = [&](int q, int j) {
+            auto issue_pv = [&](int q, int j, int half) {  // half: of the tile's positions
                 const int load = 2 * (kv + j) + 1;
-                const uint32_t v = slot_base(load), d = tmem + Sh::kO + (uint32_t)(q * HD), pt = tmem + (uint32_t)(q * BN);
+                const uint32_t v = slot_base(load) + (uint32_t)(half * (BN / 32) * 2048), d = tmem + Sh::kO + (uint32_t)(q * HD);
+                const uint32_t pt = tmem + (uint32_t)(q * BN + half * (Sh::kF32 ? BN / 2 : BN / 4));
                 const int jj = it.dual ? j >> 1 : j;  // the warpgroup's own count
                 const bool fresh = Sh::kF32 ? jj % Sh::kFlush == 0 : jj == 0;
 #pragma unroll
                 for (int part = 0; part < Sh::kSplit; ++part)
 #pragma unroll
-                    for (int kk = 0; kk < BN / 16; ++kk)
+                    for (int kk = 0; kk < BN / 32; ++kk)
                         // 16-bit: 8 columns a step; f32: 8 of hi and 8 of lo over the 16 that S leaves
                         umma_ts(one, d, pt + (uint32_t)(Sh::kF32 ? kk * 16 + part * 8 : kk * 8), desc_mn_sw128(v + (uint32_t)kk * 2048u, Sh::kKvHalf), id_o,
-                                (uint32_t)(!fresh || part || kk));
+                                (uint32_t)(!fresh || part || kk || half));
+                if (half == 0) return;
                 commit_one(one, &sh.pv_done[q]);
                 if (q == it.last_q || it.dual) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     bool v_ready = false;
                     for (int q = 0; q < 2 && ok; ++q) {
                         if (it.dual ? (j & 1) != q : j >= it.J[q]) continue;
-                        if (!(ok = wait(&sh.p_full[q], np[q]++ & 1))) break;
+                        if (!(ok = wait(&sh.p_half[q][0], np[q] & 1))) break;
                         tc_fence_after();
                         const bool more = it.dual ? j + 2 < J : j + 1 < it.J[q];
                         if (!v_ready) {
@@ -471,7 +473,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 __syncwarp();
                             }
                         }
-                        issue_pv(q, j);
+                        issue_pv(q, j, 0);
+                        if (!(ok = wait(&sh.p_half[q][1], np[q]++ & 1))) break;
+                        tc_fence_after();
+                        issue_pv(q, j, 1);
                         if (more) {
                             if (!(ok = slot_wait(2 * (kv + j + step)))) break;
                             issue_s(q, j + step);
@@ -612,14 +617,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const float mnew = up ? mx - 6.f : mref;
                 const float corr = up && mref > -INFINITY ? ex2(mref - mnew) : 1.f;
                 const bool rescale = jj > 0 && __any_sync(0xffffffffu, corr != 1.f);
-                if (jj > 0) {
-                    // P and O are free once P V of the last tile is done
-                    ok = warp_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v);
-                    if (!ok) break;
+                const bool flushes = Sh::kF32 && jj > 0 && (rescale || jj % Sh::kFlush == 0);
+                if (rescale || flushes) {
+                    // O holds the tiles before this once P V of the last one is done
+                    if (!(ok = warp_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v))) break;
                     tc_fence_after();
                 }
                 if constexpr (Sh::kF32) {
-                    if (jj > 0 && (rescale || jj % Sh::kFlush == 0)) flush(jj % Sh::kFlush != 0);
+                    if (flushes) flush(jj % Sh::kFlush != 0);
                     if (rescale) {
 #pragma unroll
                         for (int i = 0; i < HD; ++i) acc[i] *= corr;
@@ -640,6 +645,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const float base = mref == -INFINITY ? 0.f : mref;  // nothing seen yet: every score is -inf
                 const uint64_t qm2 = two(qmul, qmul), nb2 = two(-base, -base);
                 uint64_t sum[2] = {0, 0};
+                // half of P is written: P V of its positions may run under the other half's softmax
+                auto hand_over = [&](int half) {
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mb_arrive(&sh.p_half[q][half]);
+                };
                 if constexpr (Sh::kF32) {
 #pragma unroll 2
                     for (int h = 0; h < BN / 16; ++h) {
@@ -656,6 +668,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         tmem_st8(st + 16 * h, hi);
                         tmem_st8(st + 16 * h + 8, lo);
+                        if (h % (BN / 32) == BN / 32 - 1) hand_over(h / (BN / 32));
                     }
                 } else {
 #pragma unroll
@@ -669,14 +682,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             w[i] = pack2<E>(w0, w1);
                         }
                         tmem_st32(st + 32 * h, w);
+                        hand_over(h);
                     }
                 }
                 const float2 total = untwo(add2(sum[0], sum[1]));
                 l += total.x + total.y;
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mb_arrive(&sh.p_full[q]);
             }
             if (ok && J > 0) ok = warp_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v);
             if (!ok) break;
