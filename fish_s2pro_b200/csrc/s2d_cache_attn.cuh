@@ -50,32 +50,6 @@ __device__ __forceinline__ int real_tokens(const S2dCacheAttention &a, int n_seq
     return max(0, min(n, a.tokens));
 }
 
-// The sequence and its row tile behind own tile `tile` (tiles of `rows` rows,
-// the sequences' tiles one after the other); b = -1 when there is none.
-// Called by a whole warp.
-__device__ __forceinline__ void find_tile(const S2dCacheView &c, const S2dCacheAttention &a, int rep, int rows, int &tile, int &b) {
-    const int lane = threadIdx.x & 31;
-    for (int b0 = 0; b0 < c.n_seq; b0 += 32) {
-        int first, n = 0;
-        if (b0 + lane < c.n_seq) n = (int)(((int64_t)cache_tokens(a.q_start, a.tokens, b0 + lane, first, c.status) * rep + rows - 1) / rows);
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += x;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, sum > tile);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            tile -= __shfl_sync(0xffffffffu, sum - n, l);
-            b = b0 + l;
-            return;
-        }
-        tile -= __shfl_sync(0xffffffffu, sum, 31);
-    }
-    b = -1;
-}
-
 // s2d_cache_tc.cu: the items of `p` on tcgen05, and the weights of its rows by
 // computing their scores again (from p.lse2).
 cudaError_t launch_rows_tc(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s);

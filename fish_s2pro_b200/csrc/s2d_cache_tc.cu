@@ -201,13 +201,73 @@ struct TcShape {
     static_assert(kSlots >= 3, "K and V of a tile and the next K");
 };
 
+// Where an item lies.
+struct TcPlace {
+    int some;       // 0: no further item
+    int pooled, g, split, tile, b;  // own items: row tile `tile` of sequence b
+    int half;                       // 0 or 1: that half of the row tile's rows; -1: all
+};
+
 struct TcShared {
     uint64_t full[8], empty[8], s_full[2], p_half[2][2], pv_done[2], q_full[2], item_full[2], item_empty[2], pair_full, pair_free;
-    int item[2];
+    TcPlace item[2];
     float2 ml[kTcRows];  // the second warpgroup's (m, l), where both take one row tile
     uint32_t tmem;
     int abort;
 };
+
+// The k-th own row tile when all sequences' tiles are ordered by the own slots
+// they see, in steps of 128, the most first: CTAs that draw in this order end
+// nearly together.
+// A tile's slots follow from its sequence's length, so the step of the k-th is
+// found by bisection over the count of tiles that see as much.  By one warp.
+// k < 0: the number of own row tiles.
+__device__ __noinline__ int find_own_tile(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, int k, int &b) {
+    const int lane = threadIdx.x & 31;
+    // tiles of sequence i that see at least x steps; they are its last ones
+    auto count = [&](int i, int x, int &tiles) {
+        int first;
+        const int nt = cache_tokens(a.q_start, a.tokens, i, first, c.status);
+        tiles = (nt * p.rep + kTcItemRows - 1) / kTcItemRows;
+        const int64_t need = (int64_t)(x - 1) * 128 - (cache_length(c, i) - nt);  // first token that sees so much
+        return x <= 0 || need <= 0 ? tiles : need >= nt ? 0 : tiles - (int)(need * p.rep / kTcItemRows);
+    };
+    auto total = [&](int x) {
+        int sum = 0, tiles;
+        for (int i = lane; i < c.n_seq; i += 32) sum += count(i, x, tiles);
+        return __reduce_add_sync(0xffffffffu, sum);
+    };
+    if (k < 0) return total(0);
+    // Items of split positions are short: any order will do, and the bisection
+    // costs more than it saves (weigh window 122.4 us with it, 120.5 without).
+    const bool sorted = p.own_splits == 1;
+    int lo = 0, hi = sorted ? c.max_pages * kCachePage / 128 + 1 : 0;  // total(lo) > k (it is for 0); total(hi + 1) = 0
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (total(mid) > k) lo = mid;
+        else hi = mid - 1;
+    }
+    const int above = sorted ? lo + 1 : INT32_MAX;  // among those that see exactly lo steps (unsorted: all), by sequence
+    if (sorted) k -= total(above);
+    for (int b0 = 0; b0 < c.n_seq; b0 += 32) {
+        int tiles = 0, more = 0, n = 0;
+        if (b0 + lane < c.n_seq) more = count(b0 + lane, above, tiles), n = count(b0 + lane, lo, tiles) - more;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, sum > k);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            b = b0 + l;
+            return __shfl_sync(0xffffffffu, tiles - more - 1, l) - (k - __shfl_sync(0xffffffffu, sum - n, l));
+        }
+        k -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return 0;
+}
 
 // What an item is: its rows, its positions, where its results go.
 template <int BN, bool DUAL>
@@ -230,33 +290,25 @@ struct TcItem {
         pre0 = u(pre0), pre1 = u(pre1), own0 = u(own0), own1 = u(own1), jp = u(jp), tiles = u(tiles), last_q = u(last_q), dual = u(dual), J[0] = u(J[0]), J[1] = u(J[1]);
     }
 
-    // false: nothing to do.  Called by whole warps.
-    __device__ bool get(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, int item) {
-        const int G = c.kv_heads, prefix_items = p.prefix_tiles * p.prefix_splits * G;
-        pooled = item < prefix_items;
-        // own tiles from the back: a sequence's later tiles see more positions
-        if (!pooled) item = p.own_tiles * p.own_splits * G - 1 - (item - prefix_items);
-        g = item % G;
-        item /= G;
-        const int splits = pooled ? p.prefix_splits : p.own_splits;
-        split = item % splits;
-        int tile = item / splits;
-        b = first = back = pre0 = pre1 = own0 = own1 = 0;
+    // false: nothing to do.
+    __device__ bool get(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, const TcPlace &at) {
+        pooled = at.pooled, g = at.g, split = at.split, b = at.b;
+        const int tile = at.tile, splits = pooled ? p.prefix_splits : p.own_splits;
+        first = back = pre0 = pre1 = own0 = own1 = 0;
         if (pooled) {
             rows = real_tokens(a, c.n_seq) * p.rep - tile * kTcItemRows;
             const int tiles = (a.prefix_len + BN - 1) / BN, per = (tiles + splits - 1) / splits;
             pre0 = min(a.prefix_len, split * per * BN), pre1 = min(a.prefix_len, pre0 + per * BN);
         } else {
-            find_tile(c, a, p.rep, kTcItemRows, tile, b);
-            if (b < 0) return false;
             const int nt = cache_tokens(a.q_start, a.tokens, b, first, c.status);
             back = cache_length(c, b) - nt;
             rows = nt * p.rep - tile * kTcItemRows;
             if (p.fused) pre1 = a.prefix_len;
         }
+        r0 = tile * kTcItemRows + max(0, at.half) * kTcRows, rows -= max(0, at.half) * kTcRows;
         if (rows <= 0) return false;
-        rows = min(rows, kTcItemRows);
-        r0 = tile * kTcItemRows, last_q = rows > kTcRows, dual = DUAL && !last_q;
+        rows = min(rows, at.half >= 0 ? kTcRows : kTcItemRows);
+        last_q = rows > kTcRows, dual = DUAL && !last_q;
         if (!pooled) {
             const int span = seen(rows, p.rep), tiles = (span + BN - 1) / BN, per = (tiles + splits - 1) / splits;
             own0 = min(span, split * per * BN), own1 = min(span, own0 + per * BN);
@@ -272,7 +324,7 @@ struct TcItem {
 template <typename Q, typename E, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
     rows_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const S2dCacheView c,
-                   const S2dCacheAttention a, const AttnPlan p, const int items) {
+                   const S2dCacheAttention a, const AttnPlan p) {
     using Sh = TcShape<Q, HD>;
     constexpr int BN = Sh::BN;
     extern __shared__ uint8_t raw[];
@@ -311,19 +363,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     TcItem<BN, (Sh::kSlots >= 5)> it;
 
-    // The CTA's n-th item: its own block's, then what the loader drew from the
-    // counter, through a ring of two.  For the MMA and softmax warps.
-    auto take = [&](int n, int &item) {
-        if (n == 0) {
-            item = (int)blockIdx.x;
-            return true;
-        }
+    // The CTA's n-th item, which the loader draws and places, through a ring of
+    // two; false at the end.  For the MMA and softmax warps.
+    auto take = [&](int n, TcPlace &at, bool &ok) {
         const int s = n & 1;
-        if (!warp_wait(&sh.item_full[s], ((n - 1) >> 1) & 1, abort_v)) return false;
-        item = *const_cast<volatile int *>(&sh.item[s]);
+        if (!(ok = warp_wait(&sh.item_full[s], (n >> 1) & 1, abort_v))) return false;
+        at = sh.item[s];
         __syncwarp();
         if (lane == 0) mb_arrive(&sh.item_empty[s]);
-        return true;
+        return at.some != 0;
     };
     // Registers: 168 a thread at launch (three warps on a scheduler); warps
     // 8-11 give theirs to the softmax warps: 2 x 216 + 72 = 3 x 168.
@@ -333,25 +381,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ---- loader: K then V of every tile of every item ----
             int issued = 0;
             bool ok = true;
-            for (int n = 0, item = blockIdx.x; item < items && ok;) {
-                // draw the next item while this one's tiles are loaded
-                int next = items;
-                if (p.next_item) {
-                    if (lane == 0) next = (int)gridDim.x + atomicAdd(p.next_item, 1);
-                    next = __shfl_sync(0xffffffffu, next, 0);
+            const int G = c.kv_heads, prefix_items = p.prefix_tiles * p.prefix_splits * G;
+            TcPlace next = {};
+            // Own items of whole row tiles, and behind them the last few, where
+            // they are at most half a round of the CTAs, as halves: 616 items on
+            // 148 SMs would else end with 24 SMs at work on a fifth.  Not more
+            // of them: a half reads as many keys and values.
+            const int tiles = p.own_tiles ? find_own_tile(c, a, p, -1, next.b) * p.own_splits * G : 0;
+            const int odd = tiles % (int)gridDim.x, whole = Sh::kSlots >= 5 && odd <= (int)gridDim.x / 2 ? tiles - odd : tiles;
+            const int items = prefix_items + whole + 2 * (tiles - whole);
+            // places item `item` in `next` and hands it to the others as the n-th
+            auto put = [&](int n, int item) {
+                next.some = item < items;
+                if (next.some) {
+                    next.pooled = item < prefix_items;
+                    if (!next.pooled) item -= prefix_items;
+                    next.half = next.pooled || item < whole ? -1 : (item - whole) & 1;
+                    if (next.half >= 0) item = whole + (item - whole) / 2;
+                    next.g = item % G, item /= G;
+                    const int splits = next.pooled ? p.prefix_splits : p.own_splits;
+                    next.split = item % splits, next.tile = item / splits;
+                    if (!next.pooled) next.tile = find_own_tile(c, a, p, next.tile, next.b);
                 }
-                const int s = ++n & 1, use = (n - 1) >> 1;
-                if (use > 0 && !(ok = warp_wait(&sh.item_empty[s], (use - 1) & 1, abort_v))) break;
+                const int s = n & 1, use = n >> 1;
+                if (use > 0 && !warp_wait(&sh.item_empty[s], (use - 1) & 1, abort_v)) return false;
                 if (lane == 0) {
-                    *const_cast<volatile int *>(&sh.item[s]) = next;
+                    sh.item[s] = next;
                     mb_arrive(&sh.item_full[s]);
                 }
-                const bool real = it.get(c, a, p, item);
-                item = next;
-                if (!real) continue;
-                const int32_t *own_table = c.page_table + (int64_t)it.b * c.table_stride;
+                __syncwarp();
+                return true;
+            };
+            ok = put(0, (int)blockIdx.x);
+            for (int n = 0; ok && next.some; ++n) {
+                const TcPlace at = next;
+                // the next item is drawn here, and placed once this one's loads are issued
+                int item = items;
+                if (p.next_item && lane == 0) item = (int)gridDim.x + atomicAdd(p.next_item, 1);
+                const bool real = it.get(c, a, p, at);
+                const int32_t *own_table = c.page_table + (int64_t)it.b * c.table_stride;  // pooled: unused
                 int ids = 0, have = -1;  // page ids 32 * have + lane of the current segment
-                for (int j = 0; j < it.tiles && ok; ++j) {
+                for (int j = 0; real && j < it.tiles && ok; ++j) {
                     const bool own = j >= it.jp;
                     if (j == it.jp) have = -1;
                     const int32_t *table = own ? own_table : a.prefix_pages;
@@ -393,6 +463,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         ++issued;
                     }
                 }
+                if (ok) ok = put(n + 1, __shfl_sync(0xffffffffu, item, 0));
             }
             if (!ok) *abort_v = 1;
             // no copy may still be landing when the CTA leaves
@@ -440,8 +511,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 commit_one(one, &sh.pv_done[q]);
                 if (q == it.last_q || it.dual) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
-            for (int n = 0, item; ok && (ok = take(n, item)) && item < items; ++n) {
-                if (!it.get(c, a, p, item)) continue;
+            TcPlace at;
+            for (int n = 0; ok && take(n, at, ok); ++n) {
+                if (!it.get(c, a, p, at)) continue;
                 it.uniform();
                 const int J = it.tiles, step = it.dual ? 2 : 1;  // step: to the warpgroup's next tile
                 for (int q = 0; q < (it.dual ? 2 : it.last_q + 1) && ok; ++q) {
@@ -496,8 +568,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t qdst = sbase + (uint32_t)q * Sh::kQTile;
         uint32_t ns = 0, nd = 0;  // S tiles taken so far (P V tiles done are as many); items shared by both warpgroups
         bool ok = true;
-        for (int n = 0, item; ok && (ok = take(n, item)) && item < items; ++n) {
-            if (!it.get(c, a, p, item) || (!it.dual && q > it.last_q)) continue;
+        TcPlace at;
+            for (int n = 0; ok && take(n, at, ok); ++n) {
+            if (!it.get(c, a, p, at) || (!it.dual && q > it.last_q)) continue;
             const int tile0 = it.dual ? 0 : q * kTcRows, row = tile0 + r, J = it.J[q];  // tile0: the warpgroup's first row
             const bool real = row < it.rows;
             const int rr = it.r0 + (real ? row : 0), rt = row_token(p, rr), tok = it.first + rt, head = it.g * p.rep + rr - rt * p.rep;
@@ -855,7 +928,11 @@ __global__ void __launch_bounds__(256) weigh_tc_kernel(const __grid_constant__ C
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y, g = blockIdx.z, p0 = (int)blockIdx.x * kWeighSlots;
     int first;
     const int n = cache_length(c, b), nt = cache_tokens(a.q_start, a.tokens, b, first, c.status);
-    if (p0 >= n || nt == 0) return;
+    if (p0 >= n || nt == 0) {
+        // the grid must not end before the one that it was launched behind
+        if (blockIdx.x + blockIdx.y + blockIdx.z == 0) grid_dep_wait();
+        return;
+    }
     const int back = n - nt, rows = nt * p.rep;
     volatile int *abort_v = &s_abort;
     if (threadIdx.x == 0) {
@@ -889,7 +966,7 @@ __global__ void __launch_bounds__(256) weigh_tc_kernel(const __grid_constant__ C
     const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(tile * kTcRows);
     constexpr uint32_t id_s = idesc_f16_f32(kTcRows, kTcRows) | (std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
     float sum = 0.f;
-    bool ok = true;
+    bool ok = true, waited = false;
     uint32_t turn = 0;
     // row tiles before this see none of the CTA's slots
     for (int r0 = (int)min((int64_t)rows, (int64_t)max(0, p0 - back) * p.rep) / kTcRows * kTcRows; r0 < rows && ok; r0 += kTcRows, ++turn) {
@@ -903,10 +980,11 @@ __global__ void __launch_bounds__(256) weigh_tc_kernel(const __grid_constant__ C
             const Q *src = static_cast<const Q *>(a.q) + (int64_t)(first + wt) * a.q_stride + (int64_t)(g * p.rep + w - wt * p.rep) * HD;
             qv[i] = w < rows ? reinterpret_cast<const uint4 *>(src)[c16] : make_uint4(0, 0, 0, 0);
         }
+        if (!waited) grid_dep_wait(), waited = true;  // the rows' sums are there
         if (threadIdx.x < kTcRows) {
             const int w = r0 + (int)threadIdx.x, wt = row_token(p, w);
             float l = INFINITY;
-            if (w < rows) l = p.lse2[(int64_t)(first + wt) * a.heads + g * p.rep + w - wt * p.rep];
+            if (w < rows) l = __ldcg(&p.lse2[(int64_t)(first + wt) * a.heads + g * p.rep + w - wt * p.rep]);
             s_row[threadIdx.x].y = l == -INFINITY ? INFINITY : l;
             if (!Sh::kF32) s_row[threadIdx.x].x = a.scale * kLog2e;
             s_seen[threadIdx.x] = w < rows ? back + wt + 1 : 0;
@@ -980,6 +1058,7 @@ __global__ void __launch_bounds__(256) weigh_tc_kernel(const __grid_constant__ C
         tc_fence_before();
         __syncthreads();  // the rows and the scores are used up
     }
+    if (!waited) grid_dep_wait();
     if (turn == 0) (void)warp_wait(&k_full, 0, abort_v);  // no copy may still be landing when the CTA leaves
     if (ok && slot < n) c.mass[((int64_t)b * c.kv_heads + g) * c.max_pages * kCachePage + slot] += sum;
     if (threadIdx.x == 0 && *abort_v) cache_flag(c.status, S2D_CACHE_ABORTED);
@@ -1011,14 +1090,15 @@ cudaError_t launch(const S2dCacheView &c, const S2dCacheAttention &a, const Attn
     static std::atomic<uint64_t> done{0};
     cudaError_t e = smem_limit(done, rows_tc_kernel<Q, E, HD>, c.device, smem);
     if (e) return e;
-    const int64_t items = ((int64_t)p.prefix_tiles * p.prefix_splits + (int64_t)p.own_tiles * p.own_splits) * c.kv_heads;
+    // at most: own_tiles is a bound, and any of them may be two halves
+    const int64_t items = ((int64_t)p.prefix_tiles * p.prefix_splits + 2 * (int64_t)p.own_tiles * p.own_splits) * c.kv_heads;
     if (items > 0x7fffffff - 1024) return cudaErrorInvalidValue;
     int sms = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device))) return e;
     AttnPlan q = p;
     if (items <= sms) q.next_item = nullptr;  // one item each
     if (q.next_item && (e = cudaMemsetAsync(q.next_item, 0, sizeof(int), s))) return e;
-    rows_tc_kernel<Q, E, HD><<<(unsigned)std::min<int64_t>(items, sms), kTcThreads, smem, s>>>(mk, mv, c, a, q, (int)items);
+    rows_tc_kernel<Q, E, HD><<<(unsigned)std::min<int64_t>(items, sms), kTcThreads, smem, s>>>(mk, mv, c, a, q);
     return cudaGetLastError();
 }
 
@@ -1031,8 +1111,8 @@ cudaError_t weigh(const S2dCacheView &c, const S2dCacheAttention &a, const AttnP
     const cudaError_t e = smem_limit(done, weigh_tc_kernel<Q, E, HD>, c.device, smem);
     if (e) return e;
     const dim3 grid((unsigned)((c.max_pages * kCachePage + kWeighSlots - 1) / kWeighSlots), (unsigned)c.n_seq, (unsigned)c.kv_heads);
-    weigh_tc_kernel<Q, E, HD><<<grid, 256, smem, s>>>(mk, c, a, p);
-    return cudaGetLastError();
+    // its first keys and queries are loaded while the rows' sums are still computed
+    return s2d_launch(weigh_tc_kernel<Q, E, HD>, grid, dim3(256), smem, s, true, mk, c, a, p);
 }
 
 }  // namespace
