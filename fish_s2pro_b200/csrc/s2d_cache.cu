@@ -28,12 +28,6 @@ const char *cache_view_fault(const S2dCacheView *c) {
 
 namespace {
 
-// [a, a + na) and [b, b + nb) share a byte
-bool overlap(const void *a, size_t na, const void *b, size_t nb) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a && b && x < y + nb && y < x + na;
-}
-
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
@@ -556,7 +550,7 @@ const char *evict_fault(const S2dCacheView *c, const S2dCacheEvict *a) {
     if (!c->positions || !c->mass) return "eviction needs the cache's positions and mass";
     if (a->budget < 1) return "budget must be at least 1";
     if (a->recent < 0 || a->recent > a->budget) return "recent must be in [0, budget]";
-    if (overlap(a->past, sizeof(int32_t) * c->n_seq, c->lengths, sizeof(int32_t) * c->n_seq))
+    if (cache_overlap(a->past, sizeof(int32_t) * c->n_seq, c->lengths, sizeof(int32_t) * c->n_seq))
         return "past and lengths must not overlap";
     return nullptr;
 }
@@ -575,7 +569,7 @@ const char *append_fault(const S2dCacheView *c, const S2dCacheAppend *a) {
     const int64_t qrow = (int64_t)a->heads * c->head_dim;
     if (a->tokens > 0 && (a->q != a->q_out || a->q_stride != a->q_out_stride)) {
         const size_t es = a->type == S2D_TYPE_F32 ? 4 : 2;
-        if (overlap(a->q, es * ((size_t)std::max<int64_t>(a->q_stride, 0) * (a->tokens - 1) + qrow), a->q_out,
+        if (cache_overlap(a->q, es * ((size_t)std::max<int64_t>(a->q_stride, 0) * (a->tokens - 1) + qrow), a->q_out,
                     es * ((size_t)std::max<int64_t>(a->q_out_stride, 0) * (a->tokens - 1) + qrow)))
             return "q_out must be q itself or not overlap it";
     }
@@ -586,7 +580,7 @@ const char *append_fault(const S2dCacheView *c, const S2dCacheAppend *a) {
         return "token strides must not be negative, and rows of q_out must not overlap";
     if (!(a->rope_base > 0.0) || !std::isfinite(a->rope_base)) return "rope_base must be positive and finite";
     if (!(a->eps >= 0.f)) return "eps must not be negative";
-    if (overlap(a->past, sizeof(int32_t) * c->n_seq, c->lengths, sizeof(int32_t) * c->n_seq))
+    if (cache_overlap(a->past, sizeof(int32_t) * c->n_seq, c->lengths, sizeof(int32_t) * c->n_seq))
         return "past and lengths must not overlap";
     return nullptr;
 }

@@ -124,6 +124,11 @@ inline cudaError_t smem_limit(std::atomic<uint64_t> &done, K kernel, int device,
 
 // nullptr if the view can be used, else what is wrong with it.
 const char *cache_view_fault(const S2dCacheView *c);
+// [a, a + na) and [b, b + nb) share a byte
+inline bool cache_overlap(const void *a, size_t na, const void *b, size_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && x < y + nb && y < x + na;
+}
 inline bool cache_aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
 }  // namespace s2d

@@ -404,3 +404,299 @@ def test_decode_loop_keeps_its_budget(torch):
             assert np.array_equal(got_pos[b, :, :n], pos_ref[b, :, :n])
         seen += 1
     s.c.check()
+
+
+# ---------------------------------------------------------------------------
+# how the calls are used: streams, graphs, long pools, many sequences, bad tables
+# ---------------------------------------------------------------------------
+
+
+def test_attention_on_another_stream(torch):
+    """Enqueued on torch's current stream, behind that stream's work, whatever ran on the default one."""
+    s = Case(torch, "f32", 8, 2, 128, [200, 90], None, 300, seed=31)
+    side = torch.cuda.Stream()
+    q, zero = s.q.clone(), torch.zeros_like(s.q)
+    s.q = zero
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        zero.copy_(q)
+        out, lse = s.attend()
+    side.synchronize()
+    s.compare(out, lse)
+
+
+@pytest.mark.parametrize("ty,tokens", [("f32", None), ("bf16", None), ("bf16", [40, 7, 130])])
+def test_attention_in_graphs_that_run_together(torch, ty, tokens):
+    """Two captured calls over different queries, replayed at the same time on two streams, many times: each has a workspace of
+    its own, and every replay gives what the eager call gave, bit for bit."""
+    s = Case(torch, ty, 32, 8, 128, [300, 700, 130], tokens, 900, seed=32)
+    qs = [s.q.clone(), s.q.flip(0).contiguous()]
+    eager = []
+    for q in qs:
+        s.q = q
+        eager.append([x.clone() for x in s.attend()])
+    graphs, outs = [], []
+    for q in qs:
+        s.q = q
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s.attend())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for (out, lse), (want, want_lse) in zip(outs, eager):
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    s.c.check()
+
+
+def test_decode_step_in_a_graph(torch):
+    """append, attention with weights, evict and the position counter captured once; replays carry the lengths on, on the device.
+    The same steps run eagerly on a copy give the same bits."""
+    from fish_s2pro_b200 import PagedKvCache
+    a = Case(torch, "f16", 8, 2, 64, [10, 30, 33], None, 100, spare=1, seed=33)
+    states = []
+    for _ in range(2):
+        k, v, mass, pos = (x.clone() for x in (a.c.k, a.c.v, a.mass, a.positions))
+        mass.nan_to_num_(0.0)
+        c = PagedKvCache(k, v, a.c.page_table, a.ints(a.lengths), positions=pos, mass=mass)
+        states.append(dict(c=c, past=a.ints(a.lengths), pos=a.ints(100 + a.lengths), q=a.q.clone()))
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    new = [torch.randn(3, 2, 64, dtype=torch.float16, device="cuda", generator=gen) for _ in range(2)]
+
+    def step(s):
+        q = s["c"].append(s["q"], new[0], new[1], s["pos"], s["past"])
+        out = s["c"].attention(q, prefix_pages=a.prefix_pages, prefix_len=100, weigh=True)
+        s["c"].evict(32, 4, s["past"])
+        s["pos"].add_(1)
+        return out
+
+    eager = [step(states[0]).clone() for _ in range(9)]
+    g = torch.cuda.CUDAGraph()
+    kept = {x: states[1][x].clone() for x in ("past", "pos")}
+    with torch.cuda.graph(g):
+        out = step(states[1])
+    for x, v in kept.items():
+        assert torch.equal(states[1][x], v)  # capturing ran nothing
+    for want in eager:
+        g.replay()
+        assert torch.equal(out, want)
+    for x in ("k", "v", "mass", "positions", "lengths"):
+        u, w = (getattr(s["c"], x) for s in states)
+        assert torch.equal(u.nan_to_num(0.0) if u.is_floating_point() else u, w.nan_to_num(0.0) if w.is_floating_point() else w)
+    assert torch.equal(states[0]["past"], states[1]["past"]) and states[0]["past"].tolist() == [19, 32, 32]
+
+
+@pytest.mark.parametrize("tokens", [None, [9, 140]])
+def test_pool_past_2_to_the_32_elements(torch, tokens):
+    """Pages whose rows lie more than 2^32 elements into the pool: append, attention with weights and eviction there."""
+    from fish_s2pro_b200 import PagedKvCache
+    s = Case(torch, "f16", 8, 2, 128, [70, 300], tokens, 130, seed=34)
+    n = s.c.n_pages
+    per_page = 2 * PAGE * 128
+    far = 2 ** 32 // per_page + 1000
+    k, v = (torch.empty(far + n, 2, PAGE, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    k[far:], v[far:] = s.c.k, s.c.v
+    c = PagedKvCache(k, v, s.c.page_table + far, s.c.lengths, positions=s.positions, mass=s.mass)
+    s.c = c
+    s.prefix_pages = s.prefix_pages + far
+    out, lse = s.attend(weigh=True)
+    s.compare(out, lse, weigh=True)
+    before = [x[far:].clone() for x in (k, v)]
+    mass0, pos0 = s.mass.cpu().numpy(), s.positions.cpu().numpy()
+    c.evict(64, 8, s.ints([0, 0]))
+    c.check()
+    for b, n_b in enumerate(s.lengths):
+        for g in range(2):
+            to, fro = ref.evict(pos0[b, g], mass0[b, g], int(n_b), 64, 8)
+            for i, j in zip(to, fro):
+                for x in before:
+                    x[s.table[b, i // PAGE], g, i % PAGE] = x[s.table[b, j // PAGE], g, j % PAGE]
+    assert all(torch.equal(x[far:].view(torch.int16), y.view(torch.int16)) for x, y in zip((k, v), before))
+    q = torch.randn(2, 8, 128, dtype=torch.float16, device="cuda")
+    kn = torch.randn(2, 2, 128, dtype=torch.float16, device="cuda")
+    c.append(q, kn, kn, s.ints([1, 2]), s.ints([5, 60]), eps=0.0)
+    c.check()
+    assert torch.equal(v[far + int(s.table[0, 0]), :, 5], kn[0]) and torch.equal(v[far + int(s.table[1, 0]), :, 60], kn[1])
+
+
+def test_many_sequences(torch):
+    """A thousand short sequences, some empty, some without a token of theirs; the same page under two of them."""
+    rng = np.random.default_rng(35)
+    lengths = rng.integers(0, 90, 1000)
+    tokens = np.minimum(lengths, rng.integers(0, 4, 1000)).astype(int)
+    s = Case(torch, "bf16", 6, 2, 64, lengths.tolist(), tokens.tolist(), 80, seed=35, pad=2)
+    s.table[17] = s.table[500]  # sequence 17 reads 500's pages
+    n = int(min(lengths[17], lengths[500]))
+    s.lengths[17] = n
+    if tokens[17] > n:
+        tokens[17] = n
+    s.c.page_table[17] = s.c.page_table[500]
+    s.c.lengths[17] = n
+    s.mass0[17] = 0.5
+    s.mass[17] = 0.5
+    out, lse = s.attend(weigh=True)
+    s.compare(out, lse, weigh=True)
+
+
+def test_results_do_not_change_from_call_to_call(torch):
+    """Weights and outputs are summed in a fixed order: repeated calls give the same bits."""
+    for tokens in (None, [300, 20, 77]):
+        s = Case(torch, "f32", 16, 4, 128, [900, 20, 400], tokens, 1500, seed=36)
+        first = None
+        for _ in range(5):
+            s.mass.zero_()
+            out, lse = s.attend(weigh=True)
+            got = [out.clone(), lse.clone(), s.mass.clone()]
+            first = first or got
+            assert all(torch.equal(x, y) for x, y in zip(first, got))
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("page", [-1, "n_pages", 2 ** 31 - 1, -2 ** 31])
+def test_bad_pages_are_reported_and_stay_in_their_sequence(torch, page, ragged):
+    from fish_s2pro_b200 import S2dError
+    s = Case(torch, "f16", 8, 2, 128, [130, 150, 70], [3, 60, 2] if ragged else None, 100, seed=37)
+    want, *_ = s.expected()
+    s.c.page_table[1, 1] = s.c.n_pages if page == "n_pages" else page
+    mass0 = s.mass.clone()
+    out, lse = s.attend(weigh=True)
+    with pytest.raises(S2dError, match="page id outside the pool"):
+        s.c.check()
+    s.c.check()  # cleared
+    rows = np.r_[: s.starts[1], s.starts[2]: s.starts[3]]
+    assert np.max(np.abs(out.double().cpu().numpy()[rows] - want[rows])) < 1e-2
+    assert torch.all(s.mass[[0, 2]].nan_to_num(0) >= mass0[[0, 2]].nan_to_num(0))
+    before = s.c.k.clone().view(torch.int16)
+    s.positions.copy_(torch.from_numpy(s.pos0))
+    s.mass.copy_(torch.from_numpy(s.mass0))
+    s.c.evict(100, 10, s.ints([0, 0, 0]))
+    with pytest.raises(S2dError, match="page id outside the pool"):
+        s.c.check()
+    untouched = np.setdiff1d(np.arange(s.c.n_pages), s.table[:2].reshape(-1))
+    assert torch.equal(s.c.k.view(torch.int16)[untouched], before[untouched])
+    q = torch.zeros(3, 8, 128, dtype=torch.float16, device="cuda")
+    kn = torch.ones(3, 2, 128, dtype=torch.float16, device="cuda")
+    before = s.c.v.clone().view(torch.int16)
+    s.c.append(q, kn, kn, s.ints([1, 2, 3]), s.ints([130, 64, 70]))
+    with pytest.raises(S2dError, match="page id outside the pool"):
+        s.c.check()
+    changed = (s.c.v.view(torch.int16) != before).any(-1).any(-1).any(-1).nonzero().flatten().tolist()
+    assert sorted(changed) == sorted(int(s.table[b, n // PAGE]) for b, n in ((0, 130), (2, 70)))
+
+
+@pytest.mark.parametrize("length", [-1, 2 ** 31 - 1, -2 ** 31, 193])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_bad_lengths_are_reported(torch, length, ragged):
+    """Lengths outside the page table (three pages here): held inside it."""
+    from fish_s2pro_b200 import S2dError
+    s = Case(torch, "f16", 8, 2, 128, [130, 150, 70], [3, 60, 2] if ragged else None, 100, seed=38)
+    want, *_ = s.expected()
+    s.c.lengths[1] = length
+    out, lse = s.attend(weigh=True)
+    with pytest.raises(S2dError, match="out of range"):
+        s.c.check()
+    rows = np.r_[: s.starts[1], s.starts[2]: s.starts[3]]
+    assert np.max(np.abs(out.double().cpu().numpy()[rows] - want[rows])) < 1e-2
+    s.c.evict(100, 10, s.ints([0, 0, 0]))
+    with pytest.raises(S2dError, match="out of range"):
+        s.c.check()
+
+
+@pytest.mark.parametrize("starts", [[0, 40, 20, 60], [0, -3, 20, 60], [0, 20, 100, 60], [-5, 20, 40, 60], [7, 20, 40, 60], [0, 20, 40, 1000], [0, 0, 0, -1]])
+def test_bad_starts_touch_nothing_else(torch, starts):
+    """q_start out of order or out of range: reported where it is (a first entry above 0 just leaves rows out), no row past the
+    tokens written."""
+    from fish_s2pro_b200 import S2dError
+    s = Case(torch, "bf16", 8, 2, 64, [130, 150, 70], [20, 20, 20], 100, seed=39)
+    s.q_start = s.ints(starts)
+    wide = torch.full((70, 8, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    s.attend(weigh=True, out=wide[:60])
+    assert torch.all(wide[60:] == 5.0)
+    if starts != [7, 20, 40, 60]:
+        with pytest.raises(S2dError, match="out of range"):
+            s.c.check()
+    kn = torch.zeros(60, 2, 64, dtype=torch.bfloat16, device="cuda")
+    s.c.append(s.q, kn, kn, s.ints(range(60)), s.ints([130, 150, 70]), q_start=s.q_start, out=wide[:60])
+    assert torch.all(wide[60:] == 5.0)
+    with pytest.raises(S2dError):
+        s.c.check()
+
+
+def test_append_to_a_full_sequence_and_bad_past(torch):
+    from fish_s2pro_b200 import S2dError
+    for past, message in ((190, "past the last slot"), (192, "past the last slot"), (193, "out of range"), (-1, "out of range"), (2 ** 31 - 1, "out of range")):
+        s = Case(torch, "f16", 8, 2, 64, [64, 192, 64], [2, 5, 2], 0, seed=40)
+        kn = torch.ones(9, 2, 64, dtype=torch.float16, device="cuda")
+        before = s.c.v.clone()
+        s.c.append(s.q, kn, kn, s.ints(range(9)), s.ints([10, past, 20]), q_start=s.q_start)
+        with pytest.raises(S2dError, match=message):
+            s.c.check()
+        assert s.c.lengths.tolist() == [12, min(192, max(past, 0) + 5) if past < 2 ** 31 - 1 else 192, 22]
+        after = s.c.v
+        assert torch.all(after[int(s.table[0, 0]), :, 10:12] == 1) and torch.all(after[int(s.table[2, 0]), :, 20:22] == 1)
+        tail = after[int(s.table[1, 2])]
+        if past == 190:
+            assert torch.all(tail[:, 62:] == 1)
+            tail = tail[:, :62]
+            assert torch.equal(tail, before[int(s.table[1, 2])][:, :62])
+        else:
+            assert all(torch.equal(after[int(p)], before[int(p)]) for p in s.table[1])
+
+
+def test_refusals(torch):
+    from fish_s2pro_b200 import PagedKvCache, S2dError
+    s = Case(torch, "f16", 8, 2, 64, [30, 40], None, 70, seed=41)
+    c, q = s.c, s.q
+    kn = torch.zeros(2, 2, 64, dtype=torch.float16, device="cuda")
+    pos, past = s.ints([1, 2]), s.ints([1, 2])
+    pool = torch.zeros(4, 2, PAGE, 64, dtype=torch.float16, device="cuda")
+    table, lengths = s.ints([[0, 1], [2, 3]]), s.ints([1, 1])
+    calls = [
+        lambda: PagedKvCache(pool.float(), pool.float(), table, lengths),
+        lambda: PagedKvCache(pool, pool[:, :1], table, lengths),
+        lambda: PagedKvCache(pool.transpose(1, 2), pool.transpose(1, 2), table, lengths),
+        lambda: PagedKvCache(pool.cpu(), pool.cpu(), table, lengths),
+        lambda: PagedKvCache(pool, pool, table.long(), lengths),
+        lambda: PagedKvCache(pool, pool, table, lengths[:1]),
+        lambda: PagedKvCache(pool, pool, table, lengths, mass=torch.zeros(2, 2, 64, device="cuda")),
+        lambda: c.attention(q.float().double()),
+        lambda: c.attention(q.bfloat16()),
+        lambda: c.attention(q[:, :7]),
+        lambda: c.attention(q.cpu()),
+        lambda: c.attention(q.transpose(0, 1)),
+        lambda: c.attention(torch.cat([q, q])),                      # four tokens, two sequences, no q_start
+        lambda: c.attention(q, q_start=s.ints([0, 1])),
+        lambda: c.attention(q, q_start=torch.tensor([0, 1, 2], device="cuda")),
+        lambda: c.attention(q, prefix_pages=s.prefix_pages, prefix_len=129),
+        lambda: c.attention(q, prefix_len=3),
+        lambda: c.attention(q, prefix_pages=s.prefix_pages, prefix_len=-1),
+        lambda: c.attention(q, scale=float("nan")),
+        lambda: c.attention(q, out=q[:, :4]),
+        lambda: c.attention(q, out=q),
+        lambda: c.attention(q.detach().clone().requires_grad_()),
+        lambda: c.attention(q, out=torch.empty(2 * 8 * 64 + 1, dtype=torch.float16, device="cuda")[1:].view(2, 8, 64)),  # misaligned
+        lambda: c.append(q, kn, kn.float(), pos, past),
+        lambda: c.append(q, kn[:1], kn, pos, past),
+        lambda: c.append(q, kn, kn, pos.long(), past),
+        lambda: c.append(q, kn, kn, pos, c.lengths),
+        lambda: c.append(q, kn, kn, pos, past, q_norm=torch.ones(32, device="cuda")),
+        lambda: c.append(q, kn, kn, pos, past, rope_base=0.0),
+        lambda: c.append(q, kn, kn, pos, past, eps=-1.0),
+        lambda: c.evict(0, 0),
+        lambda: c.evict(10, 11),
+        lambda: c.evict(10, -1),
+        lambda: c.evict(10, 1, c.lengths),
+        lambda: PagedKvCache(pool, pool, table, lengths).evict(1, 0),
+        lambda: PagedKvCache(pool, pool, table, lengths).attention(q, weigh=True),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(S2dError) as e:
+            call()
+        assert e.value.code == -1, i
+    c.check()
