@@ -511,7 +511,7 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
         const int64_t own = rows / kTcTile + std::min<int64_t>(c.n_seq, rows);  // sum of ceil(rows of b / 256) is no more
         const bool fill = own * c.kv_heads >= kSms;
         p.own_tiles = (int)own;
-        p.own_splits = fill ? 1 : cut(own * c.kv_heads, (int64_t)c.max_pages * kCachePage, 512, 4 * kSms);
+        p.own_splits = fill ? 1 : cut(own * c.kv_heads, (int64_t)c.max_pages * kCachePage, 512, 3 * kSms);
         p.fused = a.prefix_len && fill && rows >= (int64_t)c.n_seq * kTcTile / 2;
         if (a.prefix_len && !p.fused) {
             p.prefix_tiles = (int)pooled;

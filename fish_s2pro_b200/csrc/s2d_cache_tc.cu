@@ -275,9 +275,9 @@ struct TcItem {
     int g, split, b, first, rows, r0, back;  // back: own slots before the sequence's first token
     int pre0, pre1, own0, own1;              // prefix positions and own slots of the item
     int jp, tiles, J[2];                     // prefix tiles; all tiles; those of each warpgroup
-    int last_q;                              // last row tile
-    // one row tile only: both warpgroups take it, with the even and the odd tiles (if the ring holds two tiles' loads)
-    bool pooled, dual;
+    // one row tile only: both warpgroups take it, with the even and the odd tiles (if the ring holds two tiles' loads), or
+    // the first alone
+    bool pooled, dual, solo;
 
     // own slots that rows [0, n) of the item see together
     __device__ __forceinline__ int seen(int n, int rep) const { return pooled ? 0 : max(0, back + (r0 + n - 1) / rep + 1); }
@@ -287,7 +287,7 @@ struct TcItem {
     // The fields of the MMA warp's loops, known to be alike in all lanes.
     __device__ __forceinline__ void uniform() {
         auto u = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
-        pre0 = u(pre0), pre1 = u(pre1), own0 = u(own0), own1 = u(own1), jp = u(jp), tiles = u(tiles), last_q = u(last_q), dual = u(dual), J[0] = u(J[0]), J[1] = u(J[1]);
+        pre0 = u(pre0), pre1 = u(pre1), own0 = u(own0), own1 = u(own1), jp = u(jp), tiles = u(tiles), dual = DUAL && u(dual), solo = !DUAL && u(solo), J[0] = u(J[0]), J[1] = u(J[1]);
     }
 
     // false: nothing to do.
@@ -308,15 +308,15 @@ struct TcItem {
         r0 = tile * kTcItemRows + max(0, at.half) * kTcRows, rows -= max(0, at.half) * kTcRows;
         if (rows <= 0) return false;
         rows = min(rows, at.half >= 0 ? kTcRows : kTcItemRows);
-        last_q = rows > kTcRows, dual = DUAL && !last_q;
+        dual = DUAL && rows <= kTcRows, solo = !DUAL && rows <= kTcRows;
         if (!pooled) {
             const int span = seen(rows, p.rep), tiles = (span + BN - 1) / BN, per = (tiles + splits - 1) / splits;
             own0 = min(span, split * per * BN), own1 = min(span, own0 + per * BN);
         }
         jp = (pre1 - pre0 + BN - 1) / BN;
         tiles = jp + (own1 - own0 + BN - 1) / BN;
-        J[0] = dual ? (tiles + 1) / 2 : !last_q ? tiles : jp + max(0, (min(seen(kTcRows, p.rep), own1) - own0 + BN - 1) / BN);
-        J[1] = dual ? tiles / 2 : last_q ? tiles : 0;
+        J[0] = dual ? (tiles + 1) / 2 : solo ? tiles : jp + max(0, (min(seen(kTcRows, p.rep), own1) - own0 + BN - 1) / BN);
+        J[1] = dual ? tiles / 2 : solo ? 0 : tiles;
         return true;
     }
 };
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                  desc_k_sw128(k + half * Sh::kKvHalf + off), id_s, (uint32_t)(part != Sh::kSplit - 1 || kk > 0));
                     }
                 commit_one(one, &sh.s_full[q]);
-                if (q == it.last_q || it.dual) commit_one(one, &sh.empty[load % Sh::kSlots]);
+                if (q == 1 || it.dual || it.solo) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
             auto issue_pv = [&](int q, int j, int half) {  // half: of the tile's positions
                 const int load = 2 * (kv + j) + 1;
@@ -509,14 +509,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 (uint32_t)(!fresh || part || kk || half));
                 if (half == 0) return;
                 commit_one(one, &sh.pv_done[q]);
-                if (q == it.last_q || it.dual) commit_one(one, &sh.empty[load % Sh::kSlots]);
+                if (q == 1 || it.dual || it.solo) commit_one(one, &sh.empty[load % Sh::kSlots]);
             };
             TcPlace at;
             for (int n = 0; ok && take(n, at, ok); ++n) {
                 if (!it.get(c, a, p, at)) continue;
                 it.uniform();
                 const int J = it.tiles, step = it.dual ? 2 : 1;  // step: to the warpgroup's next tile
-                for (int q = 0; q < (it.dual ? 2 : it.last_q + 1) && ok; ++q) {
+                for (int q = 0; q < (it.solo ? 1 : 2) && ok; ++q) {
                     ok = wait(&sh.q_full[q], nitem[q]++ & 1);
                     tc_fence_after();
                     const int j = it.dual ? q : 0;
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         bool ok = true;
         TcPlace at;
             for (int n = 0; ok && take(n, at, ok); ++n) {
-            if (!it.get(c, a, p, at) || (!it.dual && q > it.last_q)) continue;
+            if (!it.get(c, a, p, at) || (it.solo && q == 1)) continue;
             const int tile0 = it.dual ? 0 : q * kTcRows, row = tile0 + r, J = it.J[q];  // tile0: the warpgroup's first row
             const bool real = row < it.rows;
             const int rr = it.r0 + (real ? row : 0), rt = row_token(p, rr), tok = it.first + rt, head = it.g * p.rep + rr - rt * p.rep;
