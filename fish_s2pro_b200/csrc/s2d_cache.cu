@@ -6,6 +6,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace s2d {
 
@@ -152,64 +153,65 @@ __global__ void __launch_bounds__(256, 4) append_kernel(const S2dCacheView c, co
     }
     __syncthreads();
 
-    const int d0 = tid % L * W, rows = a.heads + 2 * G;
+    const int d0 = tid % L * W;
     const uint32_t mates = (L == 32 ? 0xffffffffu : (1u << L) - 1u) << ((tid & 31) / L * L);  // the row's lanes
-    int tok = 0, row = tid / L;  // this lane group's next row: a query, a key or a value head of a token of the group
-    auto settle = [&]() {
-        while (row >= rows) row -= rows, ++tok;
-    };
-    settle();
-    while (tok < n) {
-        uint4 in[kAhead];
-        int its_tok[kAhead], its_row[kAhead];
+    // The head rows of one kind (0 queries, 1 keys, 2 values) of the group's
+    // tokens: lane group tid / L takes rows tid / L, + kRows, ... of them.
+    auto rows_of = [&](auto kind_of, const void *from, int64_t stride, int heads) {
+        constexpr int kind = decltype(kind_of)::value;
+        const bool normed = kind == 0 ? a.q_norm != nullptr : kind == 1 && a.k_norm != nullptr;
+        const Q *src = static_cast<const Q *>(from) + (int64_t)t0 * stride + d0;
+        const int next_tok = kRows / heads, next_head = kRows % heads;
+        int tok = tid / L / heads, head = tid / L % heads;
+        while (tok < n) {
+            uint4 in[kAhead];
+            int its_tok[kAhead], its_head[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            its_tok[k] = tok, its_row[k] = row;
-            if (tok < n) {
-                const bool is_q = row < a.heads, is_k = row < a.heads + G;
-                const Q *src = static_cast<const Q *>(is_q ? a.q : is_k ? a.k : a.v) + (int64_t)(t0 + tok) * (is_q ? a.q_stride : is_k ? a.k_stride : a.v_stride) +
-                               (row - (is_q ? 0 : is_k ? a.heads : a.heads + G)) * HD + d0;
-                in[k] = *reinterpret_cast<const uint4 *>(src);
+            for (int k = 0; k < kAhead; ++k) {
+                its_tok[k] = tok, its_head[k] = head;
+                if (tok < n) in[k] = *reinterpret_cast<const uint4 *>(src + tok * stride + head * HD);
+                tok += next_tok, head += next_head;
+                if (head >= heads) head -= heads, ++tok;
             }
-            row += kRows;
-            settle();
-        }
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            if (its_tok[k] >= n) break;  // whole rows: the row's lanes together
-            const bool is_q = its_row[k] < a.heads, is_k = !is_q && its_row[k] < a.heads + G;
-            float x[W];
-            unpack16<Q>(in[k], x);
-            if (is_q || is_k) {
-                if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
-                    float ss = 0.f;
+            for (int k = 0; k < kAhead; ++k) {
+                if (its_tok[k] >= n) break;  // whole rows: the row's lanes together
+                float x[W];
+                unpack16<Q>(in[k], x);
+                if (kind < 2) {
+                    if (normed) {
+                        float ss = 0.f;
 #pragma unroll
-                    for (int e = 0; e < W; ++e) ss = fmaf(x[e], x[e], ss);
+                        for (int e = 0; e < W; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-                    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mates, ss, o);
-                    const float norm = rsqrtf(ss * (1.f / HD) + a.eps);
+                        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mates, ss, o);
+                        const float norm = rsqrtf(ss * (1.f / HD) + a.eps);
 #pragma unroll
-                    for (int e = 0; e < W; e += 4) {
-                        const float4 gain = *reinterpret_cast<const float4 *>(&s_gain[is_k][d0 + e]);
-                        x[e] *= norm * gain.x, x[e + 1] *= norm * gain.y, x[e + 2] *= norm * gain.z, x[e + 3] *= norm * gain.w;
+                        for (int e = 0; e < W; e += 4) {
+                            const float4 gain = *reinterpret_cast<const float4 *>(&s_gain[kind][d0 + e]);
+                            x[e] *= norm * gain.x, x[e + 1] *= norm * gain.y, x[e + 2] *= norm * gain.z, x[e + 3] *= norm * gain.w;
+                        }
+                    }
+#pragma unroll
+                    for (int p = 0; p < W / 2; p += 2) {
+                        const float4 r = *reinterpret_cast<const float4 *>(&s_turn[its_tok[k]][d0 / 2 + p]);
+                        const float u0 = x[2 * p], w0 = x[2 * p + 1], u1 = x[2 * p + 2], w1 = x[2 * p + 3];
+                        x[2 * p] = u0 * r.x - w0 * r.y, x[2 * p + 1] = fmaf(u0, r.y, w0 * r.x);
+                        x[2 * p + 2] = u1 * r.z - w1 * r.w, x[2 * p + 3] = fmaf(u1, r.w, w1 * r.z);
                     }
                 }
-#pragma unroll
-                for (int p = 0; p < W / 2; p += 2) {
-                    const float4 r = *reinterpret_cast<const float4 *>(&s_turn[its_tok[k]][d0 / 2 + p]);
-                    const float u0 = x[2 * p], w0 = x[2 * p + 1], u1 = x[2 * p + 2], w1 = x[2 * p + 3];
-                    x[2 * p] = u0 * r.x - w0 * r.y, x[2 * p + 1] = fmaf(u0, r.y, w0 * r.x);
-                    x[2 * p + 2] = u1 * r.z - w1 * r.w, x[2 * p + 3] = fmaf(u1, r.w, w1 * r.z);
+                if constexpr (kind == 0) {
+                    store_pack(static_cast<Q *>(a.q_out) + (int64_t)(t0 + its_tok[k]) * a.q_out_stride + its_head[k] * HD + d0, x);
+                } else {
+                    const int64_t at = s_at[its_tok[k]];
+                    if (at >= 0) store_pack(static_cast<E *>(kind == 1 ? c.k : c.v) + at + (int64_t)its_head[k] * c.head_stride + d0, x);
                 }
             }
-            if (is_q) {
-                store_pack(static_cast<Q *>(a.q_out) + (int64_t)(t0 + its_tok[k]) * a.q_out_stride + its_row[k] * HD + d0, x);
-            } else if (s_at[its_tok[k]] >= 0) {
-                const int h = its_row[k] - (is_k ? a.heads : a.heads + G);
-                store_pack(static_cast<E *>(is_k ? c.k : c.v) + s_at[its_tok[k]] + (int64_t)h * c.head_stride + d0, x);
-            }
         }
-    }
+    };
+    rows_of(std::integral_constant<int, 0>{}, a.q, a.q_stride, a.heads);
+    rows_of(std::integral_constant<int, 1>{}, a.k, a.k_stride, G);
+    rows_of(std::integral_constant<int, 2>{}, a.v, a.v_stride, G);
 }
 
 template <typename Q, typename E>
