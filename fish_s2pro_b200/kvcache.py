@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional
 
 from .s2d import S2dError, lib
@@ -63,15 +64,35 @@ class _Evict(_c.Structure):
                 ("workspace_bytes", _c.c_size_t)]
 
 
+def _bad(message: str) -> S2dError:
+    return S2dError(-1, message)
+
+
+def _packer(cls):
+    """Packs a struct's fields, in their order and C's layout, into bytes: a tenth of the time of a ctypes.Structure."""
+    codes = {_c.c_void_p: "P", _c.c_int32: "i", _c.c_int64: "q", _c.c_float: "f", _c.c_double: "d", _c.c_size_t: "N"}
+    p = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0P")
+    assert p.size == _c.sizeof(cls)
+
+    def pack(*fields):
+        try:
+            return p.pack(*fields)
+        except (struct.error, OverflowError) as e:
+            raise _bad(f"an argument is out of range: {e}") from None
+    return pack
+
+
+_pack_append, _pack_attention, _pack_evict = _packer(_Append), _packer(_Attention), _packer(_Evict)
+
 _i32 = _c.c_int32
 _tail = [_c.c_char_p, _c.c_size_t]
-# symbol -> (restype, argtypes); every function declared in include/s2d_cache.h
+# symbol -> (restype, argtypes); every function declared in include/s2d_cache.h.  Argument structs go in as packed bytes.
 CACHE_SIGNATURES = {
-    "s2d_cache_append": (_i32, [_P(_View), _P(_Append), _c.c_void_p] + _tail),
-    "s2d_cache_attention_workspace": (_i32, [_P(_View), _P(_Attention), _P(_c.c_size_t)] + _tail),
-    "s2d_cache_attention": (_i32, [_P(_View), _P(_Attention), _c.c_void_p] + _tail),
-    "s2d_cache_evict_workspace": (_i32, [_P(_View), _P(_Evict), _P(_c.c_size_t)] + _tail),
-    "s2d_cache_evict": (_i32, [_P(_View), _P(_Evict), _c.c_void_p] + _tail),
+    "s2d_cache_append": (_i32, [_P(_View), _c.c_void_p, _c.c_void_p] + _tail),
+    "s2d_cache_attention_workspace": (_i32, [_P(_View), _c.c_void_p, _P(_c.c_size_t)] + _tail),
+    "s2d_cache_attention": (_i32, [_P(_View), _c.c_void_p, _c.c_void_p] + _tail),
+    "s2d_cache_evict_workspace": (_i32, [_P(_View), _c.c_void_p, _P(_c.c_size_t)] + _tail),
+    "s2d_cache_evict": (_i32, [_P(_View), _c.c_void_p, _c.c_void_p] + _tail),
     "s2d_cache_status": (_i32, [_P(_View), _P(_i32), _c.c_void_p] + _tail),
 }
 
@@ -89,10 +110,6 @@ def cache_lib() -> ctypes.CDLL:
             fn.argtypes = args
         _bound = l
     return _bound
-
-
-def _bad(message: str) -> S2dError:
-    return S2dError(-1, message)
 
 
 class PagedKvCache:
@@ -183,8 +200,9 @@ class PagedKvCache:
     def _like_q(self, q, out):
         """The output for q, new if none is given: (tensor, pointer, token stride)."""
         if out is None:
-            out = q.new_empty(q.shape)
-            return out, out.data_ptr(), q.shape[1] * q.shape[2]
+            tokens, heads, d = q.shape
+            out = q.new_empty_strided((tokens, heads, d), (heads * d, d, 1))
+            return out, out.data_ptr(), heads * d
         if out.shape != q.shape or out.dtype != q.dtype:
             raise _bad("out must be like q")
         return (out, *self._rows("out", out))
@@ -207,7 +225,7 @@ class PagedKvCache:
         if q_start is None:
             if tokens > self.n_seq:
                 raise _bad(f"{tokens} tokens for {self.n_seq} sequences: give q_start")
-            return None
+            return 0
         return self._ints("q_start", q_start, (self.n_seq + 1,))
 
     def append(self, q, k, v, pos, past, *, q_start=None, q_norm=None, k_norm=None, eps: float = 1e-6,
@@ -231,12 +249,12 @@ class PagedKvCache:
         if k.shape[0] != tokens or v.shape[0] != tokens:
             raise _bad("q, k and v must have the same tokens")
         out, op, os_ = self._like_q(q, out)
-        gains = [None if t is None else self._dense(n, t, self._torch.float32, (self.head_dim,))
+        gains = [0 if t is None else self._dense(n, t, self._torch.float32, (self.head_dim,))
                  for n, t in (("q_norm", q_norm), ("k_norm", k_norm))]
-        a = _Append(qp, kp, vp, qs, ks, vs, op, os_, gains[0], gains[1], self._ints("pos", pos, (tokens,)),
-                    self._ints("past", past, (self.n_seq,)), self._starts(q_start, tokens), tokens, q.shape[1], ty, eps,
-                    rope_base)
-        self._call(self._lib.s2d_cache_append(self._view_ref, _c.byref(a), self._stream(), self._err, 256))
+        a = _pack_append(qp, kp, vp, qs, ks, vs, op, os_, gains[0], gains[1], self._ints("pos", pos, (tokens,)),
+                         self._ints("past", past, (self.n_seq,)), self._starts(q_start, tokens), tokens, q.shape[1], ty, eps,
+                         rope_base)
+        self._call(self._lib.s2d_cache_append(self._view_ref, a, self._stream(), self._err, 256))
         return out
 
     def attention(self, q, *, q_start=None, prefix_pages=None, prefix_len: int = 0, scale: Optional[float] = None,
@@ -256,28 +274,26 @@ class PagedKvCache:
         tokens, heads = q.shape[0], q.shape[1]
         torch = self._torch
         out, op, os_ = self._like_q(q, out)
-        lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
-        prefix = None
+        lse = q.new_empty_strided((tokens, heads), (heads, 1), dtype=torch.float32) if return_lse else None
+        prefix = 0
         if prefix_len:
             if prefix_pages is None or prefix_pages.dim() != 1 or prefix_len < 0 or prefix_pages.shape[0] * PAGE < prefix_len:
                 raise _bad("prefix_pages must be int32 page ids that hold prefix_len positions")
-            prefix = self._ints("prefix_pages", prefix_pages, tuple(prefix_pages.shape))
-        a = _Attention(qp, qs, op, os_, lse.data_ptr() if return_lse else None, self._starts(q_start, tokens), prefix,
-                       prefix_len, tokens, heads, ty, 1 if weigh else 0,
-                       self._scale if scale is None else scale, None, 0)
+            prefix = self._ints("prefix_pages", prefix_pages, prefix_pages.shape)
+        fields = (qp, qs, op, os_, lse.data_ptr() if return_lse else 0, self._starts(q_start, tokens), prefix, prefix_len, tokens,
+                  heads, ty, 1 if weigh else 0, self._scale if scale is None else scale)
         key = (tokens, heads, prefix_len, ty, weigh, q_start is None)
         need = self._sizes.get(key)
         if need is None:
             n = _c.c_size_t()
-            self._call(self._lib.s2d_cache_attention_workspace(self._view_ref, _c.byref(a), _c.byref(n), self._err, 256))
+            self._call(self._lib.s2d_cache_attention_workspace(self._view_ref, _pack_attention(*fields, 0, 0), _c.byref(n), self._err, 256))
             if len(self._sizes) >= 256:
                 self._sizes.clear()
             need = self._sizes[key] = n.value
-        if need:
-            # from the caching allocator: stream-ordered, and a captured graph gets its own
-            work = q.new_empty(need, dtype=torch.uint8)
-            a.workspace, a.workspace_bytes = work.data_ptr(), need
-        self._call(self._lib.s2d_cache_attention(self._view_ref, _c.byref(a), self._stream(), self._err, 256))
+        # from the caching allocator: stream-ordered, and a captured graph gets its own
+        work = q.new_empty_strided((need,), (1,), dtype=torch.uint8) if need else None
+        self._call(self._lib.s2d_cache_attention(self._view_ref, _pack_attention(*fields, work.data_ptr() if need else 0, need),
+                                                 self._stream(), self._err, 256))
         return (out, lse) if return_lse else out
 
     def evict(self, budget: int, recent: int, past=None) -> None:
@@ -287,17 +303,18 @@ class PagedKvCache:
         into the freed ones before it, with their positions and mass.  past
         (int32 [n_seq], not the lengths tensor) receives min(length, budget),
         what the next append takes; lengths itself stays as it is."""
-        a = _Evict(budget, recent, None if past is None else self._ints("past", past, (self.n_seq,)), None, 0)
-        key = (budget,)
+        to = 0 if past is None else self._ints("past", past, (self.n_seq,))
+        key = budget
         need = self._sizes.get(key)
         if need is None:
             n = _c.c_size_t()
-            self._call(self._lib.s2d_cache_evict_workspace(self._view_ref, _c.byref(a), _c.byref(n), self._err, 256))
+            self._call(self._lib.s2d_cache_evict_workspace(self._view_ref, _pack_evict(budget, recent, to, 0, 0), _c.byref(n), self._err, 256))
+            if len(self._sizes) >= 256:
+                self._sizes.clear()
             need = self._sizes[key] = n.value
-        if need:
-            work = self.lengths.new_empty(need, dtype=self._torch.uint8)
-            a.workspace, a.workspace_bytes = work.data_ptr(), need
-        self._call(self._lib.s2d_cache_evict(self._view_ref, _c.byref(a), self._stream(), self._err, 256))
+        work = self.lengths.new_empty_strided((need,), (1,), dtype=self._torch.uint8) if need else None
+        self._call(self._lib.s2d_cache_evict(self._view_ref, _pack_evict(budget, recent, to, work.data_ptr() if need else 0, need),
+                                             self._stream(), self._err, 256))
 
     def check(self) -> None:
         """Wait for the current stream and raise S2dError if a call met a page

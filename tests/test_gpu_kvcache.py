@@ -677,6 +677,10 @@ def test_refusals(torch):
         lambda: c.attention(q, prefix_len=3),
         lambda: c.attention(q, prefix_pages=s.prefix_pages, prefix_len=-1),
         lambda: c.attention(q, scale=float("nan")),
+        lambda: c.attention(q, scale=1e300),
+        lambda: c.append(q, kn, kn, pos, past, eps=1e300),
+        lambda: c.evict(2 ** 31, 5),
+        lambda: c.evict(10.5, 5),
         lambda: c.attention(q, out=q[:, :4]),
         lambda: c.attention(q, out=q),
         lambda: c.attention(q.detach().clone().requires_grad_()),
