@@ -581,7 +581,7 @@ const char *append_fault(const S2dCacheView *c, const S2dCacheAppend *a) {
     if (a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0 || (a->tokens > 1 && a->q_out_stride < qrow))
         return "token strides must not be negative, and rows of q_out must not overlap";
     if (!(a->rope_base > 0.0) || !std::isfinite(a->rope_base)) return "rope_base must be positive and finite";
-    if (!(a->eps >= 0.f)) return "eps must not be negative";
+    if (!(a->eps >= 0.f) || !std::isfinite(a->eps)) return "eps must be finite and not negative";
     if (cache_overlap(a->past, sizeof(int32_t) * c->n_seq, c->lengths, sizeof(int32_t) * c->n_seq))
         return "past and lengths must not overlap";
     return nullptr;
