@@ -466,8 +466,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (ok) ok = put(n + 1, __shfl_sync(0xffffffffu, item, 0));
             }
             if (!ok) *abort_v = 1;
-            // no copy may still be landing when the CTA leaves
-            for (int i = max(0, issued - Sh::kSlots); i < issued; ++i) (void)mb_wait(&sh.full[i % Sh::kSlots], (i / Sh::kSlots) & 1, abort_v, false);
+            // neither a copy nor the arrival that frees its slot may still be landing when the CTA leaves
+            for (int i = max(0, issued - Sh::kSlots); i < issued; ++i) {
+                (void)mb_wait(&sh.full[i % Sh::kSlots], (i / Sh::kSlots) & 1, abort_v, false);
+                (void)mb_wait(&sh.empty[i % Sh::kSlots], (i / Sh::kSlots) & 1, abort_v);
+            }
         } else if (warp == 9) {
             // ---- MMA issuer ----
             constexpr uint32_t type = std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
@@ -898,11 +901,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // scores computed again with the slots as rows: S^T = K Q^T, so that a slot is
 // a TMEM lane and one thread adds its weights, in the order of the rows.
 //
-// A CTA keeps 256 slots' keys in shared memory (two tiles of 128, one for each
-// warpgroup) and takes the sequence's query rows 128 at a time.  Its phases
-// follow one another; with 16-bit queries two CTAs share an SM and fill each
-// other's waits.
-constexpr int kWeighSlots = 256;
+// A CTA takes up to kWeighTiles tiles of 128 slots of one (sequence, KV head)
+// and its query rows 128 at a time: the rows are loaded once, the keys stream
+// through a ring of two tiles, and two warpgroups take every other tile, each
+// with a TMEM buffer of its own.  Warps 0-7 load the rows and add the weights,
+// 8 loads keys, 9 issues the MMAs; with 16-bit queries two CTAs share an SM.
+// Every wait is bounded, as above.
+constexpr int kWeighTiles = 8, kWeighThreads = 320;
 
 template <typename Q, int HD>
 struct WeighShape {
@@ -914,18 +919,19 @@ struct WeighShape {
 };
 
 template <typename Q, typename E, int HD>
-__global__ void __launch_bounds__(256) weigh_tc_kernel(const __grid_constant__ CUtensorMap mk, const S2dCacheView c, const S2dCacheAttention a,
-                                                       const AttnPlan p) {
+__global__ void __launch_bounds__(kWeighThreads) weigh_tc_kernel(const __grid_constant__ CUtensorMap mk, const S2dCacheView c, const S2dCacheAttention a,
+                                                                 const AttnPlan p) {
     using Sh = WeighShape<Q, HD>;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t k_full, s_full;
+    __shared__ uint64_t k_full[2], k_empty[2], s_full[2], s_free[2], q_full, q_free;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ __align__(16) float2 s_row[kTcRows];  // a row's (multiplier of its scores, lse2); lse2 inf: no weight
     __shared__ int s_seen[kTcRows];                  // slots that a row sees
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = su32(smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y, g = blockIdx.z, p0 = (int)blockIdx.x * kWeighSlots;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, b = blockIdx.y, g = blockIdx.z;
+    const int p0 = (int)blockIdx.x * kWeighTiles * kTcRows;
     int first;
     const int n = cache_length(c, b), nt = cache_tokens(a.q_start, a.tokens, b, first, c.status);
     if (p0 >= n || nt == 0) {
@@ -936,7 +942,8 @@ __global__ void __launch_bounds__(256) weigh_tc_kernel(const __grid_constant__ C
     const int back = n - nt, rows = nt * p.rep;
     volatile int *abort_v = &s_abort;
     if (threadIdx.x == 0) {
-        mb_init(&k_full, 1), mb_init(&s_full, 1);
+        for (int i = 0; i < 2; ++i) mb_init(&k_full[i], 1), mb_init(&k_empty[i], 1), mb_init(&s_full[i], 1), mb_init(&s_free[i], 4);
+        mb_init(&q_full, 8), mb_init(&q_free, 8);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -948,121 +955,171 @@ __global__ void __launch_bounds__(256) weigh_tc_kernel(const __grid_constant__ C
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    const int n_pages = min(kWeighSlots / kCachePage, (n - p0 + kCachePage - 1) / kCachePage);
-    if (threadIdx.x == 0) {
-        mb_expect_tx(&k_full, (uint32_t)(n_pages * Sh::kHalves * kCachePage * 128));
+    // row tiles before this one see none of the CTA's slots
+    const int r_first = (int)min((int64_t)rows, (int64_t)max(0, p0 - back) * p.rep) / kTcRows * kTcRows;
+    // tiles of slots that the rows from r0 on see (the last of them the most)
+    auto tiles_of = [&](int r0) {
+        const int seen = min(n, back + row_token(p, min(rows, r0 + kTcRows) - 1) + 1);
+        return __shfl_sync(0xffffffffu, min(kWeighTiles, (seen - p0 + kTcRows - 1) / kTcRows), 0);
+    };
+    bool ok = true;
+    if (warp == 8) {
         const int32_t *table = c.page_table + (int64_t)b * c.table_stride + p0 / kCachePage;
-        for (int i = 0; i < n_pages; ++i) {
-            int page = __ldg(table + i);
-            if ((uint32_t)page >= (uint32_t)c.n_pages) {
-                cache_flag(c.status, S2D_CACHE_BAD_PAGE);
-                page = 0;
-            }
-            for (int h = 0; h < Sh::kHalves; ++h)
-                tma_page(smem + Sh::kQ + (i >> 1) * Sh::kK + h * Sh::kKHalf + (i & 1) * kCachePage * 128, &mk, 64 * h, g, page, &k_full);
-        }
-    }
-    const int tile = warp >> 2, slot = p0 + tile * kTcRows + 32 * (warp & 3) + lane;  // this thread's slot
-    const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(tile * kTcRows);
-    constexpr uint32_t id_s = idesc_f16_f32(kTcRows, kTcRows) | (std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
-    float sum = 0.f;
-    bool ok = true, waited = false;
-    uint32_t turn = 0;
-    // row tiles before this see none of the CTA's slots
-    for (int r0 = (int)min((int64_t)rows, (int64_t)max(0, p0 - back) * p.rep) / kTcRows * kTcRows; r0 < rows && ok; r0 += kTcRows, ++turn) {
-        // 128 query rows: 16 a warp, 16 bytes a lane
-        constexpr int kLanes = HD * (int)sizeof(Q) / 16, kTogether = 32 / kLanes, kLoads = 16 / kTogether;
-        const int c16 = lane % kLanes;
-        uint4 qv[kLoads];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int w = r0 + 16 * warp + i * kTogether + lane / kLanes, wt = row_token(p, w);
-            const Q *src = static_cast<const Q *>(a.q) + (int64_t)(first + wt) * a.q_stride + (int64_t)(g * p.rep + w - wt * p.rep) * HD;
-            qv[i] = w < rows ? reinterpret_cast<const uint4 *>(src)[c16] : make_uint4(0, 0, 0, 0);
-        }
-        if (!waited) grid_dep_wait(), waited = true;  // the rows' sums are there
-        if (threadIdx.x < kTcRows) {
-            const int w = r0 + (int)threadIdx.x, wt = row_token(p, w);
-            float l = INFINITY;
-            if (w < rows) l = __ldcg(&p.lse2[(int64_t)(first + wt) * a.heads + g * p.rep + w - wt * p.rep]);
-            s_row[threadIdx.x].y = l == -INFINITY ? INFINITY : l;
-            if (!Sh::kF32) s_row[threadIdx.x].x = a.scale * kLog2e;
-            s_seen[threadIdx.x] = w < rows ? back + wt + 1 : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int w = 16 * warp + i * kTogether + lane / kLanes;
-            if constexpr (Sh::kF32) {
-                const float x[4] = {__uint_as_float(qv[i].x), __uint_as_float(qv[i].y), __uint_as_float(qv[i].z), __uint_as_float(qv[i].w)};
-                float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-                for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);  // as in the kernel above
-                const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-                if (c16 == 0) s_row[w].x = a.scale * kLog2e * __uint_as_float((uint32_t)(127 + ex - 14) << 23);
-                uint32_t hi[2], lo[2];
-                split2<E>(x[0] * up, x[1] * up, hi[0], lo[0]);
-                split2<E>(x[2] * up, x[3] * up, hi[1], lo[1]);
-                const uint32_t at = sbase + (uint32_t)((c16 >> 4) * Sh::kQHalf) + swizzle(w, (c16 >> 1) & 7) + (c16 & 1) * 8;
-                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
-                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]) : "memory");
-            } else {
-                const uint32_t at = sbase + (uint32_t)((c16 >> 3) * Sh::kQHalf) + swizzle(w, c16 & 7);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(qv[i].x), "r"(qv[i].y), "r"(qv[i].z), "r"(qv[i].w) : "memory");
-            }
-        }
-        fence_proxy_async_smem();
-        tc_fence_before();
-        __syncthreads();
-        if (warp == 0) {
-            const uint32_t one = elect();
-            if (turn == 0 && !warp_wait(&k_full, 0, abort_v)) *abort_v = 1;
-            tc_fence_after();
-            if (!*abort_v) {
-                const int tiles = n - p0 > kTcRows ? 2 : 1;
-                for (int t = 0; t < tiles; ++t)
-#pragma unroll
-                    for (int part = Sh::kSplit - 1; part >= 0; --part)  // the remainders first: their sums are small
-#pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk) {
-                            const uint32_t half = (uint32_t)(kk >> 2), off = (uint32_t)((kk & 3) * 32);
-                            umma_ss(one, tmem + (uint32_t)(t * kTcRows), desc_k_sw128(sbase + Sh::kQ + (uint32_t)t * Sh::kK + half * Sh::kKHalf + off),
-                                    desc_k_sw128(sbase + (uint32_t)(part * Sh::kHalves * Sh::kQHalf) + half * Sh::kQHalf + off), id_s,
-                                    (uint32_t)(part != Sh::kSplit - 1 || kk > 0));
+        int loads = 0;
+        for (int r0 = r_first; r0 < rows && ok; r0 += kTcRows) {
+            const int tiles = tiles_of(r0);
+            for (int t = 0; t < tiles && ok; ++t, ++loads) {
+                const int s = loads & 1, use = loads >> 1;
+                if (use > 0 && !(ok = warp_wait(&k_empty[s], (use & 1) ^ 1, abort_v))) break;
+                const int n_pages = min(2, (n - p0 - t * kTcRows + kCachePage - 1) / kCachePage);
+                if (lane == 0) {
+                    mb_expect_tx(&k_full[s], (uint32_t)(n_pages * Sh::kHalves * kCachePage * 128));
+                    for (int i = 0; i < n_pages; ++i) {
+                        int page = __ldg(table + 2 * t + i);
+                        if ((uint32_t)page >= (uint32_t)c.n_pages) {
+                            cache_flag(c.status, S2D_CACHE_BAD_PAGE);
+                            page = 0;
                         }
-                commit_one(one, &s_full);
-            }
-        }
-        ok = warp_wait(&s_full, turn & 1, abort_v);
-        if (!ok) *abort_v = 1;
-        tc_fence_after();
-        if (ok && p0 + tile * kTcRows < n) {
-            // 128 rows that all see the tile's slots, or not
-            const bool whole = r0 + kTcRows <= rows && s_seen[0] >= min(n, p0 + (tile + 1) * kTcRows);
-#pragma unroll 1
-            for (int h = 0; h < kTcRows / 32; ++h) {
-                uint32_t x[32];
-                tmem_ld(st + 32 * h, x);
-                tmem_wait_ld();
-                float part[2] = {0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float4 r = *reinterpret_cast<const float4 *>(&s_row[32 * h + i]);
-                    const float w0 = ex2(fmaf(__uint_as_float(x[i]), r.x, -r.y)), w1 = ex2(fmaf(__uint_as_float(x[i + 1]), r.z, -r.w));
-                    part[0] += whole || slot < s_seen[32 * h + i] ? w0 : 0.f;
-                    part[1] += whole || slot < s_seen[32 * h + i + 1] ? w1 : 0.f;
+                        for (int h = 0; h < Sh::kHalves; ++h)
+                            tma_page(smem + Sh::kQ + s * Sh::kK + h * Sh::kKHalf + i * kCachePage * 128, &mk, 64 * h, g, page, &k_full[s]);
+                    }
                 }
-                sum += part[0] + part[1];
+                __syncwarp();
             }
         }
-        tc_fence_before();
-        __syncthreads();  // the rows and the scores are used up
+        if (!ok) *abort_v = 1;
+        // neither a copy nor the arrival that frees its slot may still be landing when the CTA leaves
+        for (int i = max(0, loads - 2); i < loads; ++i) {
+            (void)mb_wait(&k_full[i & 1], (i >> 1) & 1, abort_v, false);
+            (void)mb_wait(&k_empty[i & 1], (i >> 1) & 1, abort_v);
+        }
+    } else if (warp == 9) {
+        constexpr uint32_t id_s = idesc_f16_f32(kTcRows, kTcRows) | (std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
+        const uint32_t one = elect();
+        int loads = 0;
+        uint32_t turn = 0, used[2] = {0, 0};  // row tiles; tiles that a buffer has held
+        for (int r0 = r_first; r0 < rows && ok; r0 += kTcRows, ++turn) {
+            const int tiles = tiles_of(r0);
+            if (!(ok = warp_wait(&q_full, turn & 1, abort_v))) break;
+            for (int t = 0; t < tiles && ok; ++t, ++loads) {
+                const int s = loads & 1, w = t & 1;
+                if (!(ok = warp_wait(&k_full[s], (loads >> 1) & 1, abort_v))) break;
+                if (used[w] > 0 && !(ok = warp_wait(&s_free[w], (used[w] - 1) & 1, abort_v))) break;
+                ++used[w];
+                tc_fence_after();
+                const uint32_t k = sbase + Sh::kQ + (uint32_t)s * Sh::kK;
+#pragma unroll
+                for (int part = Sh::kSplit - 1; part >= 0; --part)  // the remainders first: their sums are small
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint32_t half = (uint32_t)(kk >> 2), off = (uint32_t)((kk & 3) * 32);
+                        umma_ss(one, tmem + (uint32_t)(w * kTcRows), desc_k_sw128(k + half * Sh::kKHalf + off),
+                                desc_k_sw128(sbase + (uint32_t)(part * Sh::kHalves * Sh::kQHalf) + half * Sh::kQHalf + off), id_s,
+                                (uint32_t)(part != Sh::kSplit - 1 || kk > 0));
+                    }
+                commit_one(one, &s_full[w]);
+                commit_one(one, &k_empty[s]);
+            }
+        }
+        if (!ok) *abort_v = 1;
+    } else {
+        const int wg = warp >> 2;
+        const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(wg * kTcRows);
+        float sum[kWeighTiles / 2] = {};
+        bool waited = false;
+        uint32_t turn = 0, taken = 0;  // row tiles; tiles of this warpgroup
+        for (int r0 = r_first; r0 < rows && ok; r0 += kTcRows, ++turn) {
+            // 128 query rows: 16 a warp, 16 bytes a lane
+            constexpr int kLanes = HD * (int)sizeof(Q) / 16, kTogether = 32 / kLanes, kLoads = 16 / kTogether;
+            const int c16 = lane % kLanes, tiles = tiles_of(r0);
+            uint4 qv[kLoads];
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int w = r0 + 16 * warp + i * kTogether + lane / kLanes, wt = row_token(p, w);
+                const Q *src = static_cast<const Q *>(a.q) + (int64_t)(first + wt) * a.q_stride + (int64_t)(g * p.rep + w - wt * p.rep) * HD;
+                qv[i] = w < rows ? reinterpret_cast<const uint4 *>(src)[c16] : make_uint4(0, 0, 0, 0);
+            }
+            if (!waited) grid_dep_wait(), waited = true;  // the rows' sums are there
+            // the last rows are used up: their MMAs are done and their weights added
+            if (turn > 0 && !(ok = warp_wait(&q_free, (turn - 1) & 1, abort_v))) break;
+            if (threadIdx.x < kTcRows) {
+                const int w = r0 + (int)threadIdx.x, wt = row_token(p, w);
+                float l = INFINITY;
+                if (w < rows) l = __ldcg(&p.lse2[(int64_t)(first + wt) * a.heads + g * p.rep + w - wt * p.rep]);
+                s_row[threadIdx.x].y = l == -INFINITY ? INFINITY : l;
+                if (!Sh::kF32) s_row[threadIdx.x].x = a.scale * kLog2e;
+                s_seen[threadIdx.x] = w < rows ? back + wt + 1 : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int w = 16 * warp + i * kTogether + lane / kLanes;
+                if constexpr (Sh::kF32) {
+                    const float x[4] = {__uint_as_float(qv[i].x), __uint_as_float(qv[i].y), __uint_as_float(qv[i].z), __uint_as_float(qv[i].w)};
+                    float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+                    for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                    const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);  // as in the kernel above
+                    const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+                    if (c16 == 0) s_row[w].x = a.scale * kLog2e * __uint_as_float((uint32_t)(127 + ex - 14) << 23);
+                    uint32_t hi[2], lo[2];
+                    split2<E>(x[0] * up, x[1] * up, hi[0], lo[0]);
+                    split2<E>(x[2] * up, x[3] * up, hi[1], lo[1]);
+                    const uint32_t at = sbase + (uint32_t)((c16 >> 4) * Sh::kQHalf) + swizzle(w, (c16 >> 1) & 7) + (c16 & 1) * 8;
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + (uint32_t)(Sh::kHalves * Sh::kQHalf)), "r"(lo[0]), "r"(lo[1]) : "memory");
+                } else {
+                    const uint32_t x[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
+                    sts16(sbase + (uint32_t)((c16 >> 3) * Sh::kQHalf) + swizzle(w, c16 & 7), x);
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mb_arrive(&q_full);
+            if (!(ok = warp_wait(&q_full, turn & 1, abort_v))) break;  // the other warps' entries of s_row
+#pragma unroll
+            for (int i = 0; i < kWeighTiles / 2; ++i) {
+                const int t = 2 * i + wg;
+                if (t >= tiles || !ok) continue;
+                if (!(ok = warp_wait(&s_full[wg], taken++ & 1, abort_v))) continue;
+                tc_fence_after();
+                const int slot = p0 + t * kTcRows + 32 * (warp & 3) + lane;  // this thread's slot
+                // 128 rows that all see the tile's slots, or not
+                const bool whole = r0 + kTcRows <= rows && s_seen[0] >= min(n, p0 + (t + 1) * kTcRows);
+#pragma unroll 1
+                for (int h = 0; h < kTcRows / 32; ++h) {
+                    uint32_t x[32];
+                    tmem_ld(st + 32 * h, x);
+                    tmem_wait_ld();
+                    float part[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float4 r = *reinterpret_cast<const float4 *>(&s_row[32 * h + e]);
+                        const float w0 = ex2(fmaf(__uint_as_float(x[e]), r.x, -r.y)), w1 = ex2(fmaf(__uint_as_float(x[e + 1]), r.z, -r.w));
+                        part[0] += whole || slot < s_seen[32 * h + e] ? w0 : 0.f;
+                        part[1] += whole || slot < s_seen[32 * h + e + 1] ? w1 : 0.f;
+                    }
+                    sum[i] += part[0] + part[1];
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&s_free[wg]);
+            }
+            __syncwarp();
+            if (lane == 0) mb_arrive(&q_free);
+        }
+        if (!waited) grid_dep_wait();
+        if (!ok) *abort_v = 1;
+        float *mass = c.mass + ((int64_t)b * c.kv_heads + g) * c.max_pages * kCachePage;
+#pragma unroll
+        for (int i = 0; i < kWeighTiles / 2; ++i) {
+            const int slot = p0 + (2 * i + wg) * kTcRows + 32 * (warp & 3) + lane;
+            if (ok && slot < n) mass[slot] += sum[i];
+        }
     }
-    if (!waited) grid_dep_wait();
-    if (turn == 0) (void)warp_wait(&k_full, 0, abort_v);  // no copy may still be landing when the CTA leaves
-    if (ok && slot < n) c.mass[((int64_t)b * c.kv_heads + g) * c.max_pages * kCachePage + slot] += sum;
-    if (threadIdx.x == 0 && *abort_v) cache_flag(c.status, S2D_CACHE_ABORTED);
+    __syncwarp();
+    tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *abort_v) cache_flag(c.status, S2D_CACHE_ABORTED);
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kTcRows));
@@ -1110,9 +1167,10 @@ cudaError_t weigh(const S2dCacheView &c, const S2dCacheAttention &a, const AttnP
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = smem_limit(done, weigh_tc_kernel<Q, E, HD>, c.device, smem);
     if (e) return e;
-    const dim3 grid((unsigned)((c.max_pages * kCachePage + kWeighSlots - 1) / kWeighSlots), (unsigned)c.n_seq, (unsigned)c.kv_heads);
+    const int slots = kWeighTiles * kTcRows;
+    const dim3 grid((unsigned)((c.max_pages * kCachePage + slots - 1) / slots), (unsigned)c.n_seq, (unsigned)c.kv_heads);
     // its first keys and queries are loaded while the rows' sums are still computed
-    return s2d_launch(weigh_tc_kernel<Q, E, HD>, grid, dim3(256), smem, s, true, mk, c, a, p);
+    return s2d_launch(weigh_tc_kernel<Q, E, HD>, grid, dim3(kWeighThreads), smem, s, true, mk, c, a, p);
 }
 
 }  // namespace
