@@ -159,7 +159,7 @@ constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots
 // call needs no kernel to join them.  When weighing, the scores stay in shared memory until the row's sum over
 // prefix and own slots is known, and each CTA adds its slots' weights to the
 // mass: the keys are read once and no score leaves the SM.
-template <typename Q, typename E, int HD>
+template <typename Q, typename E, int HD, bool KEEP>
 __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const S2dCacheAttention a, const AttnPlan p, int score_pitch) {
     constexpr int KC = 16, NO = HD / 8, UNITS = HD / 8, PITCH = HD * 2 + 16, STAGE = 2 * KC * PITCH, NW = 4, R = 8;
     extern __shared__ __align__(16) uint8_t sm[];
@@ -177,7 +177,6 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
     const int g = item % G, b = item / G;
     const int head0 = g * p.rep + grp * R, n_rows = min(R, p.rep - grp * R);
     const int32_t *table = c.page_table + (int64_t)b * c.table_stride;
-    const bool keep = score_pitch > 0;
     // what the first copies and scores wait for, all under way together: the
     // length, 32 page ids (id `lane` of a window, read again as the window
     // moves on), the query rows
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
                 x[q][e] = q * 8 + 2 * t + e < have ? (s[q][e] + s[q][2 + e]) * qmul : -INFINITY;
                 mx = fmaxf(mx, x[q][e]);
             }
-            if (keep && gl < n_rows)
+            if (KEEP && gl < n_rows)
                 *reinterpret_cast<float2 *>(s_score + gl * score_pitch + (ch - ch0) * KC + q * 8 + 2 * t) = make_float2(x[q][0], x[q][1]);
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -308,9 +307,27 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
     // prefix's parts.  With a prefix alone the own part goes to the workspace
     // like the others, for the join kernel: no block holds its SM until the
     // prefix is done, but the last one, so that the grid ends after it.
-    const bool late = p.parts && !keep;
-    const int parts = late ? 0 : p.parts;  // prefix parts that are joined here
-    if (p.parts && (keep || blockIdx.x == gridDim.x - 1)) grid_dep_wait();
+    const bool late = !KEEP && p.parts;
+    const int parts = KEEP ? p.parts : 0;  // prefix parts that are joined here
+    if (p.parts && (KEEP || blockIdx.x == gridDim.x - 1)) grid_dep_wait();
+    // the mass so far of kMass slots a thread, under way while the parts meet
+    constexpr int kMass = 16;
+    const int slot0 = ch0 * KC + (int)threadIdx.x, slot1 = min(n, ch1 * KC);
+    float *mass = c.mass + ((int64_t)b * G + g) * c.max_pages * kCachePage, before[kMass];
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < kMass; ++i) before[i] = slot0 + 128 * i < slot1 ? mass[slot0 + 128 * i] : 0.f;
+    }
+    // and the first prefix parts of its outputs
+    constexpr int kPre = 8;
+    const int out0 = rank * 128 + (int)threadIdx.x;
+    float4 pv[kPre];
+    if (parts && out0 < n_rows * (HD / 4)) {
+        const float4 *part = reinterpret_cast<const float4 *>(p.part + ((int64_t)b * a.heads + head0 + out0 / (HD / 4)) * p.parts * HD + out0 % (HD / 4) * 4);
+#pragma unroll
+        for (int k = 0; k < kPre; ++k)
+            if (k < parts) pv[k] = __ldcg(part + k * (HD / 4));
+    }
     cluster_sync(S);
 
     // what every part counts in the row's softmax: ranks, then prefix parts
@@ -347,7 +364,7 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
     }
     __syncthreads();
     // the outputs, four elements a thread, shared by the ranks
-    for (int i = rank * 128 + (int)threadIdx.x; i < n_rows * (HD / 4); i += S * 128) {
+    for (int i = out0; i < n_rows * (HD / 4); i += S * 128) {
         const int row = i / (HD / 4), d = i % (HD / 4) * 4;
         const int64_t id = (int64_t)b * a.heads + head0 + row;
         float sum[4] = {};
@@ -356,24 +373,33 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
         };
         for (int k = 0; k < S; ++k) add(cluster_get(reinterpret_cast<const float4 *>(&s_o[row * HD + d]), k, S), s_rank[row][k]);
         const float4 *part = reinterpret_cast<const float4 *>(p.part + id * p.parts * HD + d);
-        for (int k0 = 0; k0 < parts; k0 += 8) {  // eight parts in flight
-            float4 v[8];
+        for (int k0 = 0; k0 < parts; k0 += kPre) {
+            if (k0 || i != out0) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k0 + k < parts) v[k] = __ldcg(part + (k0 + k) * (HD / 4));
+                for (int k = 0; k < kPre; ++k)
+                    if (k0 + k < parts) pv[k] = __ldcg(part + (k0 + k) * (HD / 4));
+            }
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k0 + k < parts) add(v[k], s_pre[row * p.parts + k0 + k]);
+            for (int k = 0; k < kPre; ++k)
+                if (k0 + k < parts) add(pv[k], s_pre[row * p.parts + k0 + k]);
         }
         if (late) store_out4(p.part + (id * p.parts + p.parts - 1) * HD + d, sum);
         else store_out4(static_cast<Q *>(a.out) + (int64_t)b * a.out_stride + (int64_t)(head0 + row) * HD + d, sum);
     }
-    if (keep) {
-        float *mass = c.mass + ((int64_t)b * G + g) * c.max_pages * kCachePage;
-        for (int j = ch0 * KC + (int)threadIdx.x; j < min(n, ch1 * KC); j += 128) {
-            float sum = 0.f;
-            for (int row = 0; row < n_rows; ++row) sum += exp2f(s_score[row * score_pitch + j - ch0 * KC] - s_lse[row]);
-            mass[j] += sum;
+    if constexpr (KEEP) {
+        for (int j0 = slot0; j0 < slot1; j0 += 128 * kMass) {
+            if (j0 != slot0) {
+#pragma unroll
+                for (int i = 0; i < kMass; ++i) before[i] = j0 + 128 * i < slot1 ? mass[j0 + 128 * i] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kMass; ++i) {
+                const int j = j0 + 128 * i;
+                if (j >= slot1) break;
+                float sum = 0.f;
+                for (int row = 0; row < n_rows; ++row) sum += exp2f(s_score[row * score_pitch + j - ch0 * KC] - s_lse[row]);
+                mass[j] = before[i] + sum;
+            }
         }
     }
     cluster_sync(S);  // no CTA leaves while another may read its part
@@ -536,12 +562,11 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
     bytes = at;
 }
 
-template <typename Q, typename E, int HD>
-cudaError_t token_launch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
-    const int pitch = score_pitch(c, a, p);
+template <typename Q, typename E, int HD, bool KEEP>
+cudaError_t token_launch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, int pitch, cudaStream_t s) {
     const size_t smem = token_smem(c, p, pitch);
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = smem_limit(done, token_kernel<Q, E, HD>, c.device, kTokenSmemMost);
+    const cudaError_t e = smem_limit(done, token_kernel<Q, E, HD, KEEP>, c.device, kTokenSmemMost);
     if (e) return e;
     const int64_t blocks = (int64_t)a.tokens * c.kv_heads * ((p.rep + 7) / 8) * p.own_splits;
     if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
@@ -554,15 +579,16 @@ cudaError_t token_launch(const S2dCacheView &c, const S2dCacheAttention &a, cons
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = p.parts ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, token_kernel<Q, E, HD>, c, a, p, pitch);
+    return cudaLaunchKernelEx(&cfg, token_kernel<Q, E, HD, KEEP>, c, a, p, pitch);
 }
 
 template <typename Q, typename E, int HD>
 cudaError_t attention_launch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, cudaStream_t s) {
     cudaError_t e = cudaSuccess;
     if (p.prefix_tiles || p.own_tiles) e = launch_rows_tc(c, a, p, s);
-    if (!e && !a.q_start) e = token_launch<Q, E, HD>(c, a, p, s);
-    if (!e && p.parts && (a.q_start || !score_pitch(c, a, p)))
+    const int pitch = a.q_start ? 0 : score_pitch(c, a, p);
+    if (!e && !a.q_start) e = pitch ? token_launch<Q, E, HD, true>(c, a, p, pitch, s) : token_launch<Q, E, HD, false>(c, a, p, 0, s);
+    if (!e && p.parts && !pitch)
         e = s2d_launch(join_kernel<Q, HD>, dim3((unsigned)(((int64_t)a.tokens * a.heads + 3) / 4)), dim3(128), 0, s, true, c, a, p);
     if (e || !p.lse2) return e;
     return launch_weigh_tc(c, a, p, s);
