@@ -235,7 +235,7 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// The block's maximum or sum of a value, in every thread.
+// A reduction over the block, in every thread.
 template <int WARPS, typename F>
 __device__ __forceinline__ int block_reduce(int v, int *sh, F warp_op, int none) {
     v = warp_op(v);
@@ -333,15 +333,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const S2
     auto used = [&](int r) { return min(KPT, (n - r * ROUND + THREADS - 1) / THREADS); };
 
     uint32_t key[KPT];
+    float weight[KPT];
     int newest = INT32_MIN;
-    for (int r = 0; r < rounds; ++r)
+    for (int r = 0; r < rounds; ++r) {
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
             if (i >= used(r)) break;
-            const int j = slot(r, i), x = j < n ? pos[j] : INT32_MIN;
-            key[i] = (uint32_t)x;  // the position, for now
-            newest = max(newest, x);
+            const int j = slot(r, i);
+            key[i] = (uint32_t)(j < n ? pos[j] : INT32_MIN);  // the position, for now
+            weight[i] = rounds == 1 && j < n ? mass[j] : 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            if (i >= used(r)) break;
+            newest = max(newest, (int)key[i]);
+        }
+    }
     newest = block_reduce<WARPS>(newest, sh, [](int v) { return __reduce_max_sync(0xffffffffu, v); }, INT32_MIN);
     const int64_t edge = (int64_t)newest - a.recent;
     int recents = 0;
@@ -356,15 +363,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const S2
     // More recent slots than the budget (positions that repeat): only they can
     // stay, by their mass.  Otherwise all of them stay.
     const bool crowded = recents > budget;
-    auto key_of = [&](int j, int position) {
+    auto key_of = [&](int position, float w) {
         const bool late = (int64_t)position > edge;
-        return late == crowded ? ordered(mass[j]) : late ? 0xffffffffu : 0u;
+        return late == crowded ? ordered(w) : late ? 0xffffffffu : 0u;
     };
     if (rounds == 1) {
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
             if (i >= used(0)) break;
-            key[i] = slot(0, i) < n ? key_of(slot(0, i), (int)key[i]) : 0u;
+            key[i] = slot(0, i) < n ? key_of((int)key[i], weight[i]) : 0u;
         }
     }
     auto load = [&](int r) {
@@ -373,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const S2
         for (int i = 0; i < KPT; ++i) {
             if (i >= used(r)) break;
             const int j = slot(r, i);
-            key[i] = j < n ? key_of(j, pos[j]) : 0u;
+            key[i] = j < n ? key_of(pos[j], mass[j]) : 0u;
         }
     };
 
@@ -382,8 +389,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const S2
     uint32_t least = crowded ? 0u : 0xffffffffu;
     int need = crowded ? budget : budget - recents;
     if (need > 0) {
-        uint32_t prefix = 0;
-        for (int shift = 32; shift > 0;) {
+        // the bits that all of them share are settled; weights are close to
+        // one another, and keys that all fall into a few bins wait in line
+        uint32_t any = 0, all = 0xffffffffu;
+        for (int r = 0; r < rounds; ++r) {
+            load(r);
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) {
+                if (i >= used(r)) break;
+                if (slot(r, i) < n && key[i] != 0xffffffffu) any |= key[i], all &= key[i];
+            }
+        }
+        any = block_reduce<WARPS>(any, sh, [](uint32_t v) { return __reduce_or_sync(0xffffffffu, v); }, 0u);
+        all = block_reduce<WARPS>(all, sh, [](uint32_t v) { return __reduce_and_sync(0xffffffffu, v); }, 0xffffffffu);
+        const int open = 32 - __clz(any ^ all);
+        uint32_t prefix = open < 32 ? all >> open << open : 0u;
+        least = prefix;
+        for (int shift = open; shift > 0;) {
             const int from = shift, width = min(kDigit, shift);
             shift -= width;
             for (int i = tid; i < BINS; i += THREADS) hist[i] = 0;
