@@ -156,9 +156,17 @@ constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots
 // of every type), so the sums have f32's precision at no extra MMA.
 //
 // The CTAs' parts meet through distributed shared memory; without a prefix the
-// call needs no kernel to join them.  When weighing, the scores stay in shared memory until the row's sum over
-// prefix and own slots is known, and each CTA adds its slots' weights to the
-// mass: the keys are read once and no score leaves the SM.
+// call needs no kernel to join them.  KEEP (weighing): the scores stay in
+// shared memory until the row's sum over prefix and own slots is known, and
+// each CTA adds its slots' weights to the mass: the keys are read once and no
+// score leaves the SM.  What a CTA reads at its end (the mass, the prefix's
+// parts) is under way before the parts meet: 1 us a read, 140 us a call
+// instead of 146.
+//
+// HBM bound: f16, 64 sequences of 1,025 to 4,096 slots, 32 and 8 heads of 128,
+// weighing: 140 us, 4.9 TB/s with the prefix's launch.  Two CTAs share an SM;
+// the rest is their beginnings and ends, which more and smaller CTAs do not
+// hide (2 warps: 139 us, 1: 147).
 template <typename Q, typename E, int HD, bool KEEP>
 __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const S2dCacheAttention a, const AttnPlan p, int score_pitch) {
     constexpr int KC = 16, NO = HD / 8, UNITS = HD / 8, PITCH = HD * 2 + 16, STAGE = 2 * KC * PITCH, NW = 4, R = 8;
@@ -406,6 +414,8 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
 }
 
 // One warp per (token, head): joins its parts, eight in flight, in their order.
+// A call of a few us (128 tokens of 32 heads with 10 parts: 8), bound by its
+// launch and two dependent reads.
 template <typename Q, int HD>
 __global__ void __launch_bounds__(128) join_kernel(const S2dCacheView c, const S2dCacheAttention a, const AttnPlan p) {
     constexpr int V = HD / 32;  // elements of a lane
@@ -529,12 +539,20 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
             p.prefix_splits = cut(pooled * c.kv_heads, a.prefix_len, 128, tiles < 8 * kSms ? 88 : kSms);
         }
         const int64_t items = (int64_t)a.tokens * c.kv_heads;
+        // A cluster per item until four CTAs an SM run, of at least 8 pages
+        // each: 512 items of 1,025 to 4,096 slots take 191 us on one CTA each,
+        // 148 on two, 163 on four.
         p.own_splits = 1;
         while (p.own_splits < kMaxCluster && items * p.own_splits < 4 * kSms && c.max_pages > 8 * p.own_splits) p.own_splits *= 2;
         p.parts = p.prefix_splits;
         if (p.parts && !score_pitch(c, a, p)) ++p.parts;  // the own part goes with them
     } else {
         const int64_t own = rows / kTcTile + std::min<int64_t>(c.n_seq, rows);  // sum of ceil(rows of b / 256) is no more
+        // Row tiles that fill the SMs take all their positions and, with half
+        // a tile of rows a sequence or more, the prefix as well (`fused`);
+        // fewer are split by positions and joined: 8 sequences of 32 tokens
+        // and 1,968 to 8,160 slots take 111 us with 2 items an SM, 102 with
+        // 3, 109 with 4, 127 with 8.
         const bool fill = own * c.kv_heads >= kSms;
         p.own_tiles = (int)own;
         p.own_splits = fill ? 1 : cut(own * c.kv_heads, (int64_t)c.max_pages * kCachePage, 512, 3 * kSms);

@@ -8,17 +8,27 @@
 //   P = 2^(s - m)    one thread per row, S read from TMEM, P written over it
 //   O += P V         P from TMEM, V from shared memory (MN-major), O in TMEM
 // The two row tiles alternate: while one is in its softmax, the tensor core
-// runs the products of the other; an item of one row tile is walked by both
-// warpgroups in the same way, tile by tile in turn.  One CTA per SM draws items from a counter,
-// the longest first; one item's first loads run under the last one's epilogue.
+// runs the products of the other.  An item of one row tile is walked by both
+// warpgroups in the same way, tile by tile in turn, or by one of them where
+// the ring holds no more than three tiles (f32 heads of 128).  One CTA per SM
+// draws items from a counter, the longest first; one item's first loads run
+// under the last one's epilogue.
+//
+// What bounds it: the softmax's turn of 128 scores a thread (exponentials, TMEM
+// reads and P's writes) is about as long as a tile's two products, so the two
+// row tiles keep both busy.  bf16 prompts of 500 to 2,048 tokens behind 2,000
+// positions (32 and 8 heads of 128): 254 us, 864 TFLOP/s; f32 prompts of 33 to
+// 400 tokens behind 727: 167 us, 290 TFLOP/s of the formula's and 580 of f16
+// products.  Short items pay 7 us to start and end.
 //
 // 16-bit queries: Q as it is, P rounded once to the cache's type (its relative
 // error, half a step of that type, is that of the output's own rounding).
 //
 // f32 queries: Q and P enter as f16 pairs hi + lo (two MMAs into one
-// accumulator, about 22 bits).  Every MMA step of 16 positions truncates its sum to f32 (measured: 1.6e-8 of the
-// result a step, all toward zero: 3.4e-5 after 16,000 positions), so O is
-// moved every kFlush tiles into registers, where it is added with rounding.
+// accumulator, about 22 bits).  Every MMA step of 16 positions truncates its
+// sum to f32 (measured: 1.6e-8 of the result a step, all toward zero: 3.4e-5
+// after 16,000 positions), so O is moved every kFlush tiles into registers,
+// where it is added with rounding (1.2e-6 at any length).
 //
 // m is not the running maximum itself but a reference that follows it: it is
 // set 6 below the first tile's maximum and moves (and what is summed so far is
@@ -28,8 +38,9 @@
 // Warps: 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (warp w owns
 // TMEM lanes 32 (w % 4) ..), 8 loads K and V pages by TMA (one page of 64
 // positions x 64 columns a box, 128-byte swizzle) into a ring of tiles,
-// 9 issues the MMAs (10 and 11 only give up registers).  Every wait is bounded; one that gives up sets the
-// status word's S2D_CACHE_ABORTED, and the CTA leaves with its TMEM freed.
+// 9 issues the MMAs (10 and 11 only give up registers).  Every wait is bounded;
+// one that gives up sets the status word's S2D_CACHE_ABORTED, and the CTA
+// leaves with its TMEM freed.
 #include <cuda.h>
 
 #include "s2d_cache_attn.cuh"
@@ -43,6 +54,7 @@ namespace s2d {
 namespace {
 
 constexpr int kTcThreads = 384;
+constexpr int kTcSorted = 64;  // sequences whose row tiles are ordered
 constexpr int kTcRows = 128;
 constexpr int kTcItemRows = 2 * kTcRows;
 constexpr int kTcColumns = 512;
@@ -221,8 +233,13 @@ struct TcShared {
 // nearly together.
 // A tile's slots follow from its sequence's length, so the step of the k-th is
 // found by bisection over the count of tiles that see as much.  By one warp.
+// Without an order the k-th is the k-th by sequence, looked for from b0 on,
+// before which there are `past` of them; a later call has a larger k.
 // k < 0: the number of own row tiles.
-__device__ __noinline__ int find_own_tile(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, int k, int &b) {
+struct TcCursor {
+    int b0, past;
+};
+__device__ __noinline__ int find_own_tile(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, int k, int &b, TcCursor &from) {
     const int lane = threadIdx.x & 31;
     // tiles of sequence i that see at least x steps; they are its last ones
     auto count = [&](int i, int x, int &tiles) {
@@ -239,8 +256,9 @@ __device__ __noinline__ int find_own_tile(const S2dCacheView &c, const S2dCacheA
     };
     if (k < 0) return total(0);
     // Items of split positions are short: any order will do, and the bisection
-    // costs more than it saves (weigh window 122.4 us with it, 120.5 without).
-    const bool sorted = p.own_splits == 1;
+    // costs more than it saves (8 sequences, 122.4 us with it, 120.5 without).
+    // So it does with many sequences, whose items are short too: XXX
+    const bool sorted = p.own_splits == 1 && c.n_seq <= kTcSorted;
     int lo = 0, hi = sorted ? c.max_pages * kCachePage / 128 + 1 : 0;  // total(lo) > k (it is for 0); total(hi + 1) = 0
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -248,8 +266,9 @@ __device__ __noinline__ int find_own_tile(const S2dCacheView &c, const S2dCacheA
         else hi = mid - 1;
     }
     const int above = sorted ? lo + 1 : INT32_MAX;  // among those that see exactly lo steps (unsorted: all), by sequence
-    if (sorted) k -= total(above);
-    for (int b0 = 0; b0 < c.n_seq; b0 += 32) {
+    if (sorted) k -= total(above), from = {};
+    else k -= from.past;
+    for (int b0 = from.b0; b0 < c.n_seq; b0 += 32) {
         int tiles = 0, more = 0, n = 0;
         if (b0 + lane < c.n_seq) more = count(b0 + lane, above, tiles), n = count(b0 + lane, lo, tiles) - more;
         int sum = n;
@@ -262,9 +281,11 @@ __device__ __noinline__ int find_own_tile(const S2dCacheView &c, const S2dCacheA
         if (past) {
             const int l = __ffs(past) - 1;
             b = b0 + l;
+            from.b0 = b0;
             return __shfl_sync(0xffffffffu, tiles - more - 1, l) - (k - __shfl_sync(0xffffffffu, sum - n, l));
         }
-        k -= __shfl_sync(0xffffffffu, sum, 31);
+        const int tiles32 = __shfl_sync(0xffffffffu, sum, 31);
+        k -= tiles32, from.past += tiles32;
     }
     return 0;
 }
@@ -383,11 +404,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             bool ok = true;
             const int G = c.kv_heads, prefix_items = p.prefix_tiles * p.prefix_splits * G;
             TcPlace next = {};
+            TcCursor cursor = {};
             // Own items of whole row tiles, and behind them the last few, where
             // they are at most half a round of the CTAs, as halves: 616 items on
             // 148 SMs would else end with 24 SMs at work on a fifth.  Not more
             // of them: a half reads as many keys and values.
-            const int tiles = p.own_tiles ? find_own_tile(c, a, p, -1, next.b) * p.own_splits * G : 0;
+            const int tiles = p.own_tiles ? find_own_tile(c, a, p, -1, next.b, cursor) * p.own_splits * G : 0;
             const int odd = tiles % (int)gridDim.x, whole = Sh::kSlots >= 5 && odd <= (int)gridDim.x / 2 ? tiles - odd : tiles;
             const int items = prefix_items + whole + 2 * (tiles - whole);
             // places item `item` in `next` and hands it to the others as the n-th
@@ -401,7 +423,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     next.g = item % G, item /= G;
                     const int splits = next.pooled ? p.prefix_splits : p.own_splits;
                     next.split = item % splits, next.tile = item / splits;
-                    if (!next.pooled) next.tile = find_own_tile(c, a, p, next.tile, next.b);
+                    if (!next.pooled) next.tile = find_own_tile(c, a, p, next.tile, next.b, cursor);
                 }
                 const int s = n & 1, use = n >> 1;
                 if (use > 0 && !warp_wait(&sh.item_empty[s], (use - 1) & 1, abort_v)) return false;
@@ -907,6 +929,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // with a TMEM buffer of its own.  Warps 0-7 load the rows and add the weights,
 // 8 loads keys, 9 issues the MMAs; with 16-bit queries two CTAs share an SM.
 // Every wait is bounded, as above.
+//
+// Bound by latency: 8 sequences of 1,968 to 8,160 slots, 32 tokens each, 8 KV
+// heads of 128 take 36 us, of which reading the keys is 13.  The whole call: 106
+// us with 2 tiles a CTA, 99 to 103 with 4 to 16.
 constexpr int kWeighTiles = 8, kWeighThreads = 320;
 
 template <typename Q, int HD>

@@ -15,8 +15,10 @@ A decode loop keeps two int32 tensors, `past` and the cache's `lengths`:
     cache.evict(budget, recent, past)      # past = min(lengths, budget)
 
 Calls are enqueued on torch's current stream of the cache's device and return
-without waiting; they can be captured into CUDA graphs.  Lengths, past and
-q_start are read on the device.  Errors in the arguments raise S2dError; what
+without waiting; they can be captured into CUDA graphs.  One thread at a time
+uses a PagedKvCache; workspaces come from torch's allocator, so calls on
+several streams do not share one.  Lengths, past and q_start are read on the
+device.  Errors in the arguments raise S2dError; what
 only the device can see is kept in a status word that `check` reads.  The
 operators have no backward pass.
 """
@@ -268,7 +270,7 @@ class PagedKvCache:
         mass.  A token that sees nothing gives zeros.  Returns out, or (out,
         lse) with lse f32 [tokens, heads] the natural log of the sum of
         exponentials (-inf where a token sees nothing); rows past
-        q_start[n_seq] are not written."""
+        q_start[n_seq] are not written.  out, if given, must not overlap q."""
         ty = self._type("q", q)
         qp, qs = self._rows("q", q)
         tokens, heads = q.shape[0], q.shape[1]

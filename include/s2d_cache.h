@@ -35,6 +35,17 @@
  * view's status word; what the sequences concerned get is then unspecified,
  * but nothing outside the buffers is touched.  s2d_cache_status reads the
  * word.
+ *
+ * Limits (S2D_EINVAL beyond): head_dim 64 or 128, heads / kv_heads <= 16,
+ * kv_heads <= 1024, n_seq <= 65,535, max_pages <= 2^18, prefix_len <= 2^24,
+ * tokens * heads <= 2^26.
+ *
+ * Pages may be shared by sequences that only read them.  Append and evict
+ * write their sequence's pages, so a page that they reach belongs to one
+ * sequence.  Key rows and value rows that no token may see yet enter with
+ * weight 0, so an infinity or a NaN in the value row of a slot can reach the
+ * sequence's earlier tokens of the same call; slots at and past the length
+ * never count, whatever they hold.
  */
 #ifndef S2D_CACHE_H
 #define S2D_CACHE_H
@@ -111,7 +122,7 @@ int32_t s2d_cache_append(const S2dCacheView *view, const S2dCacheAppend *args, v
 typedef struct S2dCacheAttention {
     const void *q;             /* [tokens][heads][head_dim]                        */
     int64_t q_stride;
-    void *out;                 /* [tokens][heads][head_dim]; not q itself          */
+    void *out;                 /* [tokens][heads][head_dim]; must not overlap q      */
     int64_t out_stride;
     float *lse;                /* [tokens][heads] natural log of the softmax's sum, or NULL */
     const int32_t *q_start;    /* [n_seq + 1] or NULL                               */
