@@ -548,15 +548,21 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
         if (p.parts && !score_pitch(c, a, p)) ++p.parts;  // the own part goes with them
     } else {
         const int64_t own = rows / kTcTile + std::min<int64_t>(c.n_seq, rows);  // sum of ceil(rows of b / 256) is no more
-        // Row tiles that fill the SMs take all their positions and, with half
-        // a tile of rows a sequence or more, the prefix as well (`fused`);
-        // fewer are split by positions and joined: 8 sequences of 32 tokens
-        // and 1,968 to 8,160 slots take 111 us with 2 items an SM, 102 with
-        // 3, 109 with 4, 127 with 8.
+        // Row tiles that fill the SMs take all their positions; fewer are
+        // split by positions and joined: 8 sequences of 32 tokens and 1,968 to
+        // 8,160 slots take 111 us with 2 items an SM, 102 with 3, 109 with 4,
+        // 127 with 8.
         const bool fill = own * c.kv_heads >= kSms;
         p.own_tiles = (int)own;
         p.own_splits = fill ? 1 : cut(own * c.kv_heads, (int64_t)c.max_pages * kCachePage, 512, 3 * kSms);
-        p.fused = a.prefix_len && fill && rows >= (int64_t)c.n_seq * kTcTile / 2;
+        // They take the prefix as well (`fused`) unless its tiles in the rows
+        // that each sequence leaves empty, about n_seq / 2 row tiles, cost more
+        // than items and parts of their own.  64 sequences of 48 tokens of 32
+        // bf16 heads, fused and not: behind 727 positions (8 of these units)
+        // 102 and 161 us, 2,000 (23) 170 and 202, 8,000 (78) 564 and 471; f32,
+        // with twice the products: 193 and 239, 343 and 325, 861 and 746.
+        const int64_t waste = (int64_t)c.n_seq * ((a.prefix_len + 127) / 128);
+        p.fused = a.prefix_len && fill && waste <= pooled * (a.type == S2D_TYPE_F32 ? 12 : 32);
         if (a.prefix_len && !p.fused) {
             p.prefix_tiles = (int)pooled;
             p.prefix_splits = cut(pooled * c.kv_heads, a.prefix_len, 128, kSms);
