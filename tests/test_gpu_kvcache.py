@@ -544,6 +544,18 @@ def test_many_sequences(torch):
     s.compare(out, lse, weigh=True)
 
 
+@pytest.mark.parametrize("ty,n_seq,longest,prefix", [("bf16", 40, 5, 700), ("f32", 40, 70, 100), ("f32", 70, 40, 700), ("f16", 70, 100, 130), ("bf16", 64, 2, 9000)])
+def test_ragged_batches_behind_a_prefix(torch, ty, n_seq, longest, prefix):
+    """More row tiles than SMs, few rows or many behind short and long prefixes, up to 64 sequences and more."""
+    rng = np.random.default_rng(36)
+    tokens = rng.integers(0, longest + 1, n_seq)
+    tokens[3] = 0
+    lengths = tokens + rng.integers(0, 200, n_seq) * rng.integers(0, 2, n_seq)
+    s = Case(torch, ty, 16, 8, 64, lengths.tolist(), tokens.tolist(), prefix, seed=36, pad=1)
+    out, lse = s.attend(weigh=True)
+    s.compare(out, lse, weigh=True)
+
+
 def test_results_do_not_change_from_call_to_call(torch):
     """Weights and outputs are summed in a fixed order: repeated calls give the same bits."""
     for tokens in (None, [300, 20, 77]):
