@@ -14,12 +14,14 @@
 // draws items from a counter, the longest first; one item's first loads run
 // under the last one's epilogue.
 //
-// What bounds it: the softmax's turn of 128 scores a thread (exponentials, TMEM
-// reads and P's writes) is about as long as a tile's two products, so the two
-// row tiles keep both busy.  bf16 prompts of 500 to 2,048 tokens behind 2,000
-// positions (32 and 8 heads of 128): 254 us, 864 TFLOP/s; f32 prompts of 33 to
-// 400 tokens behind 727: 167 us, 290 TFLOP/s of the formula's and 580 of f16
-// products.  Short items pay 7 us to start and end.
+// What bounds it: bf16 prompts of 500 to 2,048 tokens behind 2,000 positions (32
+// and 8 heads of 128) take 254 us, 864 TFLOP/s; the products alone take 200,
+// the softmax alone 219 (without its exponentials 177: TMEM reads, the
+// hand-overs, the items' starts and ends), so the two row tiles overlap most
+// of the smaller one.  S in halves of 64 positions, one under the other's
+// softmax, is slower (259): the products alone then take 227.  f32 prompts of
+// 33 to 400 tokens behind 727: 167 us, 290 TFLOP/s of the formula's and 580 of
+// f16 products.  Short items pay 7 us to start and end.
 //
 // 16-bit queries: Q as it is, P rounded once to the cache's type (its relative
 // error, half a step of that type, is that of the output's own rounding).
@@ -257,7 +259,9 @@ __device__ __noinline__ int find_own_tile(const S2dCacheView &c, const S2dCacheA
     if (k < 0) return total(0);
     // Items of split positions are short: any order will do, and the bisection
     // costs more than it saves (8 sequences, 122.4 us with it, 120.5 without).
-    // So it does with many sequences, whose items are short too: XXX
+    // So it does with many sequences, which need no order for an even end: 32 of
+    // 400 tokens 171 us with it, 178 without; 128 of 16 142 and 121; 1,024 of 2
+    // 2,860 and 648.
     const bool sorted = p.own_splits == 1 && c.n_seq <= kTcSorted;
     int lo = 0, hi = sorted ? c.max_pages * kCachePage / 128 + 1 : 0;  // total(lo) > k (it is for 0); total(hi + 1) = 0
     while (lo < hi) {
@@ -380,6 +384,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr uint32_t tmem = 0;
     if (sh.tmem != 0) {
         if (threadIdx.x == 0) cache_flag(c.status, S2D_CACHE_ABORTED);
+        if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem), "r"(kTcColumns));
         return;
     }
     TcItem<BN, (Sh::kSlots >= 5)> it;
