@@ -139,6 +139,9 @@ ATTENTION = [  # type, H, G, D, own lengths, tokens per sequence (None: one each
     ("f16", 6, 2, 128, [140, 33], [140, 33], 64, 0),       # three heads per group: tiles that cut tokens
     ("f32", 10, 2, 128, [140, 33], [40, 33], 10, 2),
     ("bf16", 32, 8, 128, [1000], [1000], 300, 0),
+    ("f32", 8, 2, 64, [2500, 1100], [1500, 40], 50, 0),    # row tiles that see none of the last slots
+    ("bf16", 12, 2, 128, [3100, 7], [1300, 7], 0, 1),
+    ("f16", 8, 8, 128, [1025, 1024, 2049], [1, 300, 260], 0, 0),
 ]
 
 
@@ -261,6 +264,43 @@ def test_append(torch, ty, H, G, D, tokens, norm):
         assert torch.all(positions[b][:, dev(free)] == -7) and torch.all(mass[b][:, dev(free)] == 5.0)
     assert np.all(k_all.transpose(0, 2, 1, 3)[~touched] == 9.0) and np.all(v_all.transpose(0, 2, 1, 3)[~touched] == 9.0)
     assert lengths.tolist() == [int(p) + n for p, n in zip(past, counts)]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("counts", [[593], [700, 0, 1, 1200, 0, 333], [0, 9000, 1, 0, 31, 10100, 7]])
+def test_append_of_many_tokens(torch, counts, D):
+    """More tokens than blocks that run at once: groups of tokens that cross sequences, pages and empty sequences."""
+    from fish_s2pro_b200 import PagedKvCache
+    rng = np.random.default_rng(sum(counts))
+    B, H, G, T = len(counts), 2, 1, sum(counts)
+    past = rng.integers(0, 70, B).astype(np.int32)
+    per = -(-int((past + counts).max()) // PAGE)
+    starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    table = rng.permutation(B * per).reshape(B, per).astype(np.int32)
+    pos = rng.integers(0, 100000, T).astype(np.int32)
+    (q64, q), (k64, k), (v64, v) = (rounded(torch, rng.standard_normal((T, n, D)), torch.float32) for n in (H, G, G))
+    gain = (1 + 0.2 * rng.standard_normal(D)).astype(np.float32)
+    dev = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    kp, vp = (torch.full((B * per, G, PAGE, D), 9.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    positions = torch.full((B, G, per * PAGE), -7, dtype=torch.int32, device="cuda")
+    c = PagedKvCache(kp, vp, dev(table), dev(np.zeros(B, np.int32)), positions=positions)
+    got = c.append(q, k, v, dev(pos), dev(past), q_start=dev(starts), q_norm=dev(gain), eps=1e-6, rope_base=1e6)
+    c.check()
+    seq = np.repeat(np.arange(B), counts)
+    slot = past[seq] + np.arange(T) - starts[seq]
+    page, r = table[seq, slot // PAGE], slot % PAGE
+    for have, want, u in ((got, ref.rotate(q64, gain, pos, 1e-6, 1e6), HALF_STEP["f32"]),
+                          (kp[dev(page).long(), :, dev(r).long()], ref.rotate(k64, None, pos, 1e-6, 1e6), HALF_STEP["f16"] + 2.0 ** -24)):
+        pair = np.repeat(np.sqrt(want[..., 0::2] ** 2 + want[..., 1::2] ** 2), 2, -1)
+        assert np.all(np.abs(have.double().cpu().numpy() - want) <= 2.0 ** -20 * pair + u * np.abs(want) + 2.0 ** -25)  # f16's smallest half step
+    assert torch.equal(vp[dev(page).long(), :, dev(r).long()], v.half())
+    want = np.full((B, per * PAGE), -7, np.int32)
+    want[seq, slot] = pos
+    assert np.array_equal(positions[:, 0].cpu().numpy(), want)
+    free = np.ones((B * per, PAGE), bool)
+    free[page, r] = False
+    assert torch.all(kp[:, 0][dev(free)] == 9.0) and torch.all(vp[:, 0][dev(free)] == 9.0)
+    assert c.lengths.tolist() == (past + counts).tolist()
 
 
 def test_append_in_place_from_packed_rows(torch):
