@@ -547,10 +547,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 it.uniform();
                 const int J = it.tiles, step = it.dual ? 2 : 1;  // step: to the warpgroup's next tile
                 for (int q = 0; q < (it.solo ? 1 : 2) && ok; ++q) {
+                    if (it.J[q] == 0) continue;  // a range of positions that the rows do not reach
                     ok = wait(&sh.q_full[q], nitem[q]++ & 1);
                     tc_fence_after();
                     const int j = it.dual ? q : 0;
-                    if (ok && it.J[q] > 0 && (ok = slot_wait(2 * (kv + j)))) issue_s(q, j);
+                    if (ok && (ok = slot_wait(2 * (kv + j)))) issue_s(q, j);
                 }
                 for (int j = 0; j < J && ok; ++j) {
                     const int load = 2 * (kv + j) + 1;
@@ -610,63 +611,67 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // instruction.
             constexpr int kLanes = HD * (int)sizeof(Q) / 16, kTogether = 32 / kLanes;  // lanes of a row, rows of a load
             auto q_slot = [&](int w, int slot) { return qdst + (uint32_t)((slot >> 3) * Sh::kQHalf) + swizzle(32 * (warp & 3) + w, slot & 7); };
-            const int c16 = lane % kLanes;  // 16-byte chunk of the row
-            // 16-bit: chunk c to its place.  f32: chunks 2k and 2k + 1 to where their elements' hi and lo will be.
-            const int to_slot = Sh::kF32 ? (c16 & 1) * (kLanes / 2) + (c16 >> 1) : c16;
-#pragma unroll 4
-            for (int i = 0; i < kLanes; ++i) {
-                const int w = i * kTogether + lane / kLanes, wr = it.r0 + tile0 + 32 * (warp & 3) + w, wt = row_token(p, wr);
-                const bool is = tile0 + 32 * (warp & 3) + w < it.rows;
-                const Q *src = static_cast<const Q *>(a.q);
-                if (is) src += (int64_t)(it.first + wt) * a.q_stride + (int64_t)(it.g * p.rep + wr - wt * p.rep) * HD + c16 * (16 / (int)sizeof(Q));
-                cp_async16(q_slot(w, to_slot), src, is);
-            }
-            cp_commit();
-            cp_wait<0>();
-            __syncwarp();
             // Scores are taken with |scale|: the rows' sign takes the scale's, so
             // that their maximum is that of q . k.
             float qmul = fabsf(a.scale) * kLog2e;
-            if constexpr (Sh::kF32) {
-                // a thread splits its row into hi + lo, scaled by the power of two that puts its largest element near 2^14: the
-                // remainders stay normal f16 (at most by 2^114, which keeps rows of subnormal numbers finite)
-                float amax = 0.f;
+            // Without tiles there is nothing to load or to hand over, and the issuer
+            // does not wait: the warpgroup could be two items ahead of it.
+            if (J > 0) {
+                const int c16 = lane % kLanes;  // 16-byte chunk of the row
+                // 16-bit: chunk c to its place.  f32: chunks 2k and 2k + 1 to where their elements' hi and lo will be.
+                const int to_slot = Sh::kF32 ? (c16 & 1) * (kLanes / 2) + (c16 >> 1) : c16;
 #pragma unroll 4
-                for (int k = 0; k < kLanes; ++k) {
-                    float x[4];
-                    lds16(q_slot(lane, k), x);
-                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
+                for (int i = 0; i < kLanes; ++i) {
+                    const int w = i * kTogether + lane / kLanes, wr = it.r0 + tile0 + 32 * (warp & 3) + w, wt = row_token(p, wr);
+                    const bool is = tile0 + 32 * (warp & 3) + w < it.rows;
+                    const Q *src = static_cast<const Q *>(a.q);
+                    if (is) src += (int64_t)(it.first + wt) * a.q_stride + (int64_t)(it.g * p.rep + wr - wt * p.rep) * HD + c16 * (16 / (int)sizeof(Q));
+                    cp_async16(q_slot(w, to_slot), src, is);
                 }
-                const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);
-                const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - ex) << 23), a.scale);
-                qmul *= __uint_as_float((uint32_t)(127 + ex - 14) << 23);
+                cp_commit();
+                cp_wait<0>();
+                __syncwarp();
+                if constexpr (Sh::kF32) {
+                    // a thread splits its row into hi + lo, scaled by the power of two that puts its largest element near 2^14: the
+                    // remainders stay normal f16 (at most by 2^114, which keeps rows of subnormal numbers finite)
+                    float amax = 0.f;
+#pragma unroll 4
+                    for (int k = 0; k < kLanes; ++k) {
+                        float x[4];
+                        lds16(q_slot(lane, k), x);
+                        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
+                    }
+                    const int ex = max((int)(__float_as_uint(amax) >> 23) - 126, -100);
+                    const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - ex) << 23), a.scale);
+                    qmul *= __uint_as_float((uint32_t)(127 + ex - 14) << 23);
 #pragma unroll 2
-                for (int k = 0; k < kLanes / 2; ++k) {
-                    float x[4], y[4];
-                    uint32_t hi[4], lo[4];
-                    lds16(q_slot(lane, k), x);
-                    lds16(q_slot(lane, kLanes / 2 + k), y);
-                    split2<E>(x[0] * up, x[1] * up, hi[0], lo[0]);
-                    split2<E>(x[2] * up, x[3] * up, hi[1], lo[1]);
-                    split2<E>(y[0] * up, y[1] * up, hi[2], lo[2]);
-                    split2<E>(y[2] * up, y[3] * up, hi[3], lo[3]);
-                    sts16(q_slot(lane, k), hi);
-                    sts16(q_slot(lane, kLanes / 2 + k), lo);
-                }
-            } else if (a.scale < 0.f) {
+                    for (int k = 0; k < kLanes / 2; ++k) {
+                        float x[4], y[4];
+                        uint32_t hi[4], lo[4];
+                        lds16(q_slot(lane, k), x);
+                        lds16(q_slot(lane, kLanes / 2 + k), y);
+                        split2<E>(x[0] * up, x[1] * up, hi[0], lo[0]);
+                        split2<E>(x[2] * up, x[3] * up, hi[1], lo[1]);
+                        split2<E>(y[0] * up, y[1] * up, hi[2], lo[2]);
+                        split2<E>(y[2] * up, y[3] * up, hi[3], lo[3]);
+                        sts16(q_slot(lane, k), hi);
+                        sts16(q_slot(lane, kLanes / 2 + k), lo);
+                    }
+                } else if (a.scale < 0.f) {
 #pragma unroll 1
-                for (int k = 0; k < kLanes; ++k) {
-                    float x[4];
-                    lds16(q_slot(lane, k), x);
-                    const uint32_t y[4] = {__float_as_uint(x[0]) ^ 0x80008000u, __float_as_uint(x[1]) ^ 0x80008000u, __float_as_uint(x[2]) ^ 0x80008000u,
-                                           __float_as_uint(x[3]) ^ 0x80008000u};
-                    sts16(q_slot(lane, k), y);
+                    for (int k = 0; k < kLanes; ++k) {
+                        float x[4];
+                        lds16(q_slot(lane, k), x);
+                        const uint32_t y[4] = {__float_as_uint(x[0]) ^ 0x80008000u, __float_as_uint(x[1]) ^ 0x80008000u, __float_as_uint(x[2]) ^ 0x80008000u,
+                                               __float_as_uint(x[3]) ^ 0x80008000u};
+                        sts16(q_slot(lane, k), y);
+                    }
                 }
+                qmul = fmaxf(qmul, 1e-38f);  // a masked score stays -inf when the scale is 0
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&sh.q_full[q]);
             }
-            qmul = fmaxf(qmul, 1e-38f);  // a masked score stays -inf when the scale is 0
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mb_arrive(&sh.q_full[q]);
 
             const int own_limit = min(it.pooled ? 0 : max(0, it.back + rt + 1), it.own1) - it.own0;  // own slots of the item that this row sees
             float mref = -INFINITY, l = 0.f;

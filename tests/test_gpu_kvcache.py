@@ -596,6 +596,18 @@ def test_ragged_batches_behind_a_prefix(torch, ty, n_seq, longest, prefix):
     s.compare(out, lse, weigh=True)
 
 
+@pytest.mark.parametrize("ty,D", [("bf16", 128), ("f32", 128), ("f16", 64)])
+def test_short_sequences_beside_long_ones(torch, ty, D):
+    """Positions are split by the longest sequence's slots, so most of the short ones' ranges are empty: many calls, as these
+    items need no products and their threads run ahead."""
+    s = Case(torch, ty, 12, 2, D, [3100, 7, 1, 0, 130, 64], [300, 7, 1, 0, 30, 2], 0, seed=37)
+    first = [x.clone() for x in s.attend()]
+    s.compare(*first)
+    for _ in range(100):
+        assert all(torch.equal(x, y) for x, y in zip(first, s.attend()))
+    s.c.check()
+
+
 def test_results_do_not_change_from_call_to_call(torch):
     """Weights and outputs are summed in a fixed order: repeated calls give the same bits."""
     for tokens in (None, [300, 20, 77]):
