@@ -9,10 +9,10 @@
 //   O += P V         P from TMEM, V from shared memory (MN-major), O in TMEM
 // The two row tiles alternate: while one is in its softmax, the tensor core
 // runs the products of the other.  An item of one row tile is walked by both
-// warpgroups in the same way, tile by tile in turn, or by one of them where
-// the ring holds no more than three tiles (f32 heads of 128).  One CTA per SM
-// draws items from a counter, the longest first; one item's first loads run
-// under the last one's epilogue.
+// warpgroups in the same way, tile by tile in turn; or by one of them, the next
+// such item by the other, where it is short or the ring holds no more than
+// three tiles (f32 heads of 128).  One CTA per SM draws items from a counter,
+// the longest first; one item's first loads run under the last one's epilogue.
 //
 // What bounds it: bf16 prompts of 500 to 2,048 tokens behind 2,000 positions (32
 // and 8 heads of 128) take 254 us, 864 TFLOP/s; the products alone take 200,
@@ -56,6 +56,10 @@ namespace s2d {
 namespace {
 
 constexpr int kTcThreads = 384;
+// Tiles of positions up to which one warpgroup takes an item of one row tile
+// alone.  128 sequences of 16 bf16 tokens, 32 and 8 heads: over 16 positions 67
+// us, shared by both 82; over 350 97 and 101; over 850 140 (8) and 137.
+constexpr int kTcAlone = 5;
 constexpr int kTcSorted = 64;  // sequences whose row tiles are ordered
 constexpr int kTcRows = 128;
 constexpr int kTcItemRows = 2 * kTcRows;
@@ -300,9 +304,10 @@ struct TcItem {
     int g, split, b, first, rows, r0, back;  // back: own slots before the sequence's first token
     int pre0, pre1, own0, own1;              // prefix positions and own slots of the item
     int jp, tiles, J[2];                     // prefix tiles; all tiles; those of each warpgroup
-    // one row tile only: both warpgroups take it, with the even and the odd tiles (if the ring holds two tiles' loads), or
-    // the first alone
+    // one row tile only: both warpgroups take it, with the even and the odd
+    // tiles, or one alone (`by`), in turn, under the end of the other's item
     bool pooled, dual, solo;
+    int by;
 
     // own slots that rows [0, n) of the item see together
     __device__ __forceinline__ int seen(int n, int rep) const { return pooled ? 0 : max(0, back + (r0 + n - 1) / rep + 1); }
@@ -312,11 +317,11 @@ struct TcItem {
     // The fields of the MMA warp's loops, known to be alike in all lanes.
     __device__ __forceinline__ void uniform() {
         auto u = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
-        pre0 = u(pre0), pre1 = u(pre1), own0 = u(own0), own1 = u(own1), jp = u(jp), tiles = u(tiles), dual = DUAL && u(dual), solo = !DUAL && u(solo), J[0] = u(J[0]), J[1] = u(J[1]);
+        pre0 = u(pre0), pre1 = u(pre1), own0 = u(own0), own1 = u(own1), jp = u(jp), tiles = u(tiles), dual = DUAL && u(dual), solo = u(solo), by = u(by), J[0] = u(J[0]), J[1] = u(J[1]);
     }
 
-    // false: nothing to do.
-    __device__ bool get(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, const TcPlace &at) {
+    // The CTA's n-th item.  false: nothing to do.
+    __device__ bool get(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p, const TcPlace &at, int n) {
         pooled = at.pooled, g = at.g, split = at.split, b = at.b;
         const int tile = at.tile, splits = pooled ? p.prefix_splits : p.own_splits;
         first = back = pre0 = pre1 = own0 = own1 = 0;
@@ -333,15 +338,16 @@ struct TcItem {
         r0 = tile * kTcItemRows + max(0, at.half) * kTcRows, rows -= max(0, at.half) * kTcRows;
         if (rows <= 0) return false;
         rows = min(rows, at.half >= 0 ? kTcRows : kTcItemRows);
-        dual = DUAL && rows <= kTcRows, solo = !DUAL && rows <= kTcRows;
         if (!pooled) {
             const int span = seen(rows, p.rep), tiles = (span + BN - 1) / BN, per = (tiles + splits - 1) / splits;
             own0 = min(span, split * per * BN), own1 = min(span, own0 + per * BN);
         }
         jp = (pre1 - pre0 + BN - 1) / BN;
         tiles = jp + (own1 - own0 + BN - 1) / BN;
-        J[0] = dual ? (tiles + 1) / 2 : solo ? tiles : jp + max(0, (min(seen(kTcRows, p.rep), own1) - own0 + BN - 1) / BN);
-        J[1] = dual ? tiles / 2 : solo ? 0 : tiles;
+        const bool one = rows <= kTcRows;
+        dual = DUAL && one && tiles > kTcAlone, solo = one && !dual, by = n & 1;
+        J[0] = dual ? (tiles + 1) / 2 : solo ? (by == 0 ? tiles : 0) : jp + max(0, (min(seen(kTcRows, p.rep), own1) - own0 + BN - 1) / BN);
+        J[1] = dual ? tiles / 2 : solo ? (by == 1 ? tiles : 0) : tiles;
         return true;
     }
 };
@@ -445,7 +451,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // the next item is drawn here, and placed once this one's loads are issued
                 int item = items;
                 if (p.next_item && lane == 0) item = (int)gridDim.x + atomicAdd(p.next_item, 1);
-                const bool real = it.get(c, a, p, at);
+                const bool real = it.get(c, a, p, at, n);
                 const int32_t *own_table = c.page_table + (int64_t)it.b * c.table_stride;  // pooled: unused
                 int ids = 0, have = -1;  // page ids 32 * have + lane of the current segment
                 for (int j = 0; real && j < it.tiles && ok; ++j) {
@@ -543,11 +549,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             };
             TcPlace at;
             for (int n = 0; ok && take(n, at, ok); ++n) {
-                if (!it.get(c, a, p, at)) continue;
+                if (!it.get(c, a, p, at, n)) continue;
                 it.uniform();
                 const int J = it.tiles, step = it.dual ? 2 : 1;  // step: to the warpgroup's next tile
-                for (int q = 0; q < (it.solo ? 1 : 2) && ok; ++q) {
-                    if (it.J[q] == 0) continue;  // a range of positions that the rows do not reach
+                for (int q = 0; q < 2 && ok; ++q) {
+                    if (it.J[q] == 0) continue;  // solo: the other warpgroup; or a range of positions that the rows do not reach
                     ok = wait(&sh.q_full[q], nitem[q]++ & 1);
                     tc_fence_after();
                     const int j = it.dual ? q : 0;
@@ -601,8 +607,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         bool ok = true;
         TcPlace at;
             for (int n = 0; ok && take(n, at, ok); ++n) {
-            if (!it.get(c, a, p, at) || (it.solo && q == 1)) continue;
-            const int tile0 = it.dual ? 0 : q * kTcRows, row = tile0 + r, J = it.J[q];  // tile0: the warpgroup's first row
+            if (!it.get(c, a, p, at, n) || (it.solo && q != it.by)) continue;
+            const int tile0 = it.dual || it.solo ? 0 : q * kTcRows, row = tile0 + r, J = it.J[q];  // tile0: the warpgroup's first row
             const bool real = row < it.rows;
             const int rr = it.r0 + (real ? row : 0), rt = row_token(p, rr), tok = it.first + rt, head = it.g * p.rep + rr - rt * p.rep;
             // The warp's 32 query rows, 16 bytes a lane with a row's lanes side by
