@@ -502,6 +502,7 @@ constexpr int kTcTile = 256;      // query rows of a tcgen05 item
 constexpr int kMaxCluster = 8;    // CTAs that share one (sequence, KV head) of single tokens
 constexpr int kSms = 148;
 constexpr int kTokenSmemMost = 224 * 1024;
+constexpr int kTokenSmemTwo = 111 * 1024;  // of each of two CTAs on an SM
 
 // Shared memory of the token kernel: rings (16 slots x 2 stages x 4 warps of
 // K and V), the CTA's part, the factors of the prefix parts, the scores.
@@ -510,7 +511,9 @@ size_t token_smem(const S2dCacheView &c, const AttnPlan &p, int pitch) {
            sizeof(float) * (size_t)std::min(p.rep, 8) * pitch;
 }
 // Floats between the rows of kept scores, 0 if none are kept; + 8 spreads the
-// rows over the banks.
+// rows over the banks.  Kept wherever they fit: 64 sequences of up to 4,096
+// slots 128 us, computed again from the keys 212; of up to 12,288, which leaves
+// one CTA an SM, 431 and 579.
 int score_pitch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p) {
     if (!a.weigh || p.rep > 8) return 0;
     const int chunks = c.max_pages * (kCachePage / 16), pitch = (chunks + p.own_splits - 1) / p.own_splits * 16 + 8;
@@ -545,6 +548,16 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
         p.own_splits = 1;
         while (p.own_splits < kMaxCluster && items * p.own_splits < 4 * kSms && c.max_pages > 8 * p.own_splits) p.own_splits *= 2;
         p.parts = p.prefix_splits;
+        // Kept scores: twice the CTAs where two of them then fit an SM and one
+        // does not leave room (64 sequences in tables of 8,192 slots, filled to
+        // 2,048 and more 300 us and 235, to 100 and more 56 and 59).
+        auto two_fit = [&](int splits) {
+            AttnPlan t = p;
+            t.own_splits = splits;
+            const int pitch = score_pitch(c, a, t);
+            return pitch && token_smem(c, t, pitch) <= (size_t)kTokenSmemTwo;
+        };
+        if (p.own_splits < kMaxCluster && !two_fit(p.own_splits) && two_fit(2 * p.own_splits)) p.own_splits *= 2;
         if (p.parts && !score_pitch(c, a, p)) ++p.parts;  // the own part goes with them
     } else {
         const int64_t own = rows / kTcTile + std::min<int64_t>(c.n_seq, rows);  // sum of ceil(rows of b / 256) is no more
