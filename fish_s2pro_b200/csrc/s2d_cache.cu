@@ -612,8 +612,11 @@ const char *append_fault(const S2dCacheView *c, const S2dCacheAppend *a) {
         return "token strides must not be negative, and rows of q_out must not overlap";
     if (!(a->rope_base > 0.0) || !std::isfinite(a->rope_base)) return "rope_base must be positive and finite";
     if (!(a->eps >= 0.f) || !std::isfinite(a->eps)) return "eps must be finite and not negative";
-    if (cache_overlap(a->past, sizeof(int32_t) * c->n_seq, c->lengths, sizeof(int32_t) * c->n_seq))
-        return "past and lengths must not overlap";
+    // a block writes lengths while others still read these
+    const size_t lengths = sizeof(int32_t) * c->n_seq;
+    if (cache_overlap(a->past, lengths, c->lengths, lengths) || cache_overlap(a->q_start, lengths + sizeof(int32_t), c->lengths, lengths) ||
+        (a->tokens && cache_overlap(a->pos, sizeof(int32_t) * (size_t)a->tokens, c->lengths, lengths)))
+        return "lengths must not overlap past, pos or q_start";
     return nullptr;
 }
 

@@ -236,10 +236,11 @@ class PagedKvCache:
         kv_heads, head_dim], of the cache's type or f32 with an f16 cache.
         Queries and keys are normed per head (q_norm, k_norm: f32 [head_dim]
         gains; None leaves them as they are) and rotated by pos (int32
-        [tokens]); keys and values go to the slots after past (int32 [n_seq],
-        not the lengths tensor), with their positions and no mass, and lengths
-        becomes past + tokens.  q_start: int32 [n_seq + 1], the sequences'
-        first tokens in a packed batch; None: token i is sequence i's.
+        [tokens]); keys and values go to the slots after past (int32 [n_seq]),
+        with their positions and no mass, and lengths becomes past + tokens:
+        neither past nor pos nor q_start may be the lengths tensor.  q_start:
+        int32 [n_seq + 1], the sequences' first tokens in a packed batch; None:
+        token i is sequence i's.
         Returns the queries, in `out` (may be q) if given."""
         tokens = q.shape[0] if q.dim() == 3 else 0
         ty = self._type("q", q)

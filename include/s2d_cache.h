@@ -113,8 +113,9 @@ typedef struct S2dCacheAppend {
  * by pos / rope_base^(2i / head_dim), the queries written to q_out, the key
  * and the value (as they are) to slot past[b] + t of their sequence;
  * positions[slot] = pos, mass[slot] = 0 where the view has them.  Then
- * lengths[b] = past[b] + tokens of b, for every sequence: past and lengths
- * must not overlap (S2D_EINVAL), and the layers of a model may share both.
+ * lengths[b] = past[b] + tokens of b, for every sequence: lengths must not
+ * overlap past, pos or q_start (S2D_EINVAL), and the layers of a model may
+ * share them.
  * A token beyond the last slot is left out (S2D_CACHE_FULL). */
 int32_t s2d_cache_append(const S2dCacheView *view, const S2dCacheAppend *args, void *stream, char *err,
                          size_t err_cap);

@@ -768,3 +768,22 @@ def test_refusals(torch):
             call()
         assert e.value.code == -1, i
     c.check()
+
+
+def test_append_refuses_lengths_among_its_inputs(torch):
+    """After past.copy_(lengths) the lengths have the values of pos, but the call writes them."""
+    from fish_s2pro_b200 import S2dError
+    s = Case(torch, "f16", 8, 2, 64, [30, 40], None, 0, seed=42, spare=1)
+    kn = torch.zeros(2, 2, 64, dtype=torch.float16, device="cuda")
+    past = s.c.lengths.clone()
+    ends = torch.zeros(3, dtype=torch.int32, device="cuda")
+    ends[1:] = s.c.lengths
+    from fish_s2pro_b200 import PagedKvCache
+    other = PagedKvCache(s.c.k, s.c.v, s.c.page_table, ends[1:])
+    for call in (lambda: s.c.append(s.q, kn, kn, s.c.lengths, past), lambda: other.append(s.q, kn, kn, s.ints([1, 2]), past, q_start=ends)):
+        with pytest.raises(S2dError, match="lengths") as e:
+            call()
+        assert e.value.code == -1
+    s.c.append(s.q, kn, kn, past, past)  # pos and past may be one tensor
+    s.c.check()
+    assert s.c.lengths.tolist() == [31, 41]

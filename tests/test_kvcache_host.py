@@ -161,3 +161,10 @@ def test_status_needs_a_word(kv):
     assert L.s2d_cache_status(ctypes.byref(view(kv, status=0)), ctypes.byref(bits), None, err, 256) == -1
     assert L.s2d_cache_status(ctypes.byref(view(kv)), None, None, err, 256) == -1
     assert L.s2d_cache_status(None, ctypes.byref(bits), None, err, 256) == -1
+
+
+@pytest.mark.parametrize("bad", [dict(pos=A), dict(pos=A + 4), dict(pos=A - 4), dict(q_start=A), dict(q_start=A + 4), dict(q_start=A - 8)])
+def test_append_writes_lengths_over_nothing_that_it_reads(kv, bad):
+    """lengths is written while other blocks still read the positions and the starts: the two entries at A here."""
+    fine = dict(pos=A + 8192, q=A + 16384, k=A + 32768, v=A + 65536, q_out=A + 16384)
+    assert "lengths" in refused(kv, "s2d_cache_append", view(kv), append(kv, **{**fine, **bad}))
