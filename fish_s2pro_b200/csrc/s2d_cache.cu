@@ -599,17 +599,19 @@ const char *append_fault(const S2dCacheView *c, const S2dCacheAppend *a) {
         return "q, k and v must have the cache's type, or F32 with an F16 cache";
     const int w = a->type == S2D_TYPE_F32 ? 4 : 8;
     const int64_t qrow = (int64_t)a->heads * c->head_dim;
-    if (a->tokens > 0 && (a->q != a->q_out || a->q_stride != a->q_out_stride)) {
-        const size_t es = a->type == S2D_TYPE_F32 ? 4 : 2;
-        if (cache_overlap(a->q, es * ((size_t)std::max<int64_t>(a->q_stride, 0) * (a->tokens - 1) + qrow), a->q_out,
-                    es * ((size_t)std::max<int64_t>(a->q_out_stride, 0) * (a->tokens - 1) + qrow)))
-            return "q_out must be q itself or not overlap it";
-    }
     if (a->q_stride % w || a->k_stride % w || a->v_stride % w || a->q_out_stride % w || !cache_aligned16(a->q) ||
         !cache_aligned16(a->k) || !cache_aligned16(a->v) || !cache_aligned16(a->q_out))
         return "misaligned buffer: rows of q, k, v and q_out must be 16-byte aligned";
     if (a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0 || (a->tokens > 1 && a->q_out_stride < qrow))
         return "token strides must not be negative, and rows of q_out must not overlap";
+    if (a->tokens > 0) {
+        // blocks write q_out while others still read q, k and v
+        const int64_t es = a->type == S2D_TYPE_F32 ? 4 : 2, kvrow = (int64_t)c->kv_heads * c->head_dim;
+        const CacheRows out{a->q_out, a->q_out_stride * es, qrow * es};
+        auto shares = [&](const void *p, int64_t stride, int64_t row) { return cache_rows_overlap(out, {p, stride * es, row * es}, a->tokens); };
+        if (!(a->q == a->q_out && a->q_stride == a->q_out_stride) && shares(a->q, a->q_stride, qrow)) return "q_out must be q itself or not overlap it";
+        if (shares(a->k, a->k_stride, kvrow) || shares(a->v, a->v_stride, kvrow)) return "q_out must not overlap k or v";
+    }
     if (!(a->rope_base > 0.0) || !std::isfinite(a->rope_base)) return "rope_base must be positive and finite";
     if (!(a->eps >= 0.f) || !std::isfinite(a->eps)) return "eps must be finite and not negative";
     // a block writes lengths while others still read these

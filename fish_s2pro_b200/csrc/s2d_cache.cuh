@@ -129,6 +129,36 @@ inline bool cache_overlap(const void *a, size_t na, const void *b, size_t nb) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return a && b && x < y + nb && y < x + na;
 }
+// n rows of `row` bytes from p, `stride` >= 0 bytes apart
+struct CacheRows {
+    const void *p;
+    int64_t stride, row;
+};
+// Some row of a shares a byte with some row of b, both of n > 0 rows.  Slices of
+// one packed buffer lie between each other's rows and share none.  Row i of a
+// can only meet the last row of b that starts before its end, as that one ends
+// last too.
+inline bool cache_rows_overlap(const CacheRows &a, const CacheRows &b, int64_t n) {
+    if (!cache_overlap(a.p, (size_t)(a.stride * (n - 1) + a.row), b.p, (size_t)(b.stride * (n - 1) + b.row))) return false;
+    const int64_t off = (int64_t)((uintptr_t)b.p - (uintptr_t)a.p);  // row j of b starts here + j * b.stride from a's first
+    auto meets = [&](int64_t i) {
+        const int64_t at = i * a.stride, reach = at + a.row - 1 - off;
+        if (reach < 0) return false;
+        const int64_t j = b.stride && reach / b.stride < n ? reach / b.stride : n - 1;
+        return off + j * b.stride + b.row > at;
+    };
+    if (a.stride == b.stride && a.stride) {
+        // j - i is the same for all i that meet a row at all, up to b's last row:
+        // the first of them, and the first that only b's last row can meet
+        int64_t d = (a.row - 1 - off) / a.stride;
+        if (d * a.stride > a.row - 1 - off) --d;
+        const int64_t first = d < 0 ? -d : 0, last = n - d > 0 ? n - d : 0;
+        return (first < n && meets(first)) || (last < n && meets(last));
+    }
+    for (int64_t i = 0; i < n; ++i)
+        if (meets(i)) return true;
+    return false;
+}
 inline bool cache_aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
 }  // namespace s2d

@@ -241,7 +241,8 @@ class PagedKvCache:
         neither past nor pos nor q_start may be the lengths tensor.  q_start:
         int32 [n_seq + 1], the sequences' first tokens in a packed batch; None:
         token i is sequence i's.
-        Returns the queries, in `out` (may be q) if given."""
+        Returns the queries, in `out` if given: q itself, or rows apart from
+        those of q, k and v (slices of one packed tensor will do)."""
         tokens = q.shape[0] if q.dim() == 3 else 0
         ty = self._type("q", q)
         if k.dtype != q.dtype or v.dtype != q.dtype:

@@ -96,7 +96,8 @@ typedef struct S2dCacheView {
 typedef struct S2dCacheAppend {
     const void *q, *k, *v;     /* [tokens][heads | kv_heads | kv_heads][head_dim] */
     int64_t q_stride, k_stride, v_stride;
-    void *q_out;               /* [tokens][heads][head_dim]; may be q itself        */
+    void *q_out;               /* [tokens][heads][head_dim]; may be q itself, else its
+                                  rows share no byte with those of q, k and v      */
     int64_t q_out_stride;
     const float *q_norm, *k_norm; /* [head_dim] gains, or NULL: no norm             */
     const int32_t *pos;        /* [tokens]: rotary position of each token           */

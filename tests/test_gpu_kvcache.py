@@ -787,3 +787,22 @@ def test_append_refuses_lengths_among_its_inputs(torch):
     s.c.append(s.q, kn, kn, past, past)  # pos and past may be one tensor
     s.c.check()
     assert s.c.lengths.tolist() == [31, 41]
+
+
+def test_append_refuses_an_output_over_keys_or_values(torch):
+    """As many query heads as KV heads: out = k has the right shape, and queries would be written over keys still to be read.
+    Slices of one packed tensor lie between each other's rows and are taken."""
+    from fish_s2pro_b200 import PagedKvCache, S2dError
+    s = Case(torch, "f16", 2, 2, 64, [30, 40], None, 0, seed=43)
+    packed = torch.randn(2, 8, 64, dtype=torch.float16, device="cuda")
+    q, k, v, spare = (packed[:, i:i + 2] for i in (0, 2, 4, 6))
+    past = s.ints([3, 4])
+    for out in (k, v, packed[:, 1:3], packed[:, 5:7]):
+        with pytest.raises(S2dError, match="q_out") as e:
+            s.c.append(q, k, v, s.ints([1, 2]), past, out=out)
+        assert e.value.code == -1
+    before = packed.clone()
+    want = s.c.append(q, k, v, s.ints([1, 2]), past)
+    assert s.c.append(q, k, v, s.ints([1, 2]), past, out=spare).data_ptr() == spare.data_ptr()
+    s.c.check()
+    assert torch.equal(spare, want) and torch.equal(packed[:, :6], before[:, :6])

@@ -168,3 +168,39 @@ def test_append_writes_lengths_over_nothing_that_it_reads(kv, bad):
     """lengths is written while other blocks still read the positions and the starts: the two entries at A here."""
     fine = dict(pos=A + 8192, q=A + 16384, k=A + 32768, v=A + 65536, q_out=A + 16384)
     assert "lengths" in refused(kv, "s2d_cache_append", view(kv), append(kv, **{**fine, **bad}))
+
+
+def _rows(at, stride, row, n):
+    return set().union(*(range(at + i * stride, at + i * stride + row) for i in range(n)))
+
+
+def test_append_output_over_its_inputs(kv):
+    """q_out's rows against those of k and v, byte by byte: every distance and pair of strides that alignment allows, rows that
+    lie between each other's and rows that meet.  2 query heads and 1 KV head of 64 f16 elements: rows of 256 and 128 bytes.
+    There is no device -1, so what is not refused for its rows fails before any launch."""
+    L, err = kv.cache_lib(), ctypes.create_string_buffer(256)
+    one = view(kv, kv_heads=1, page_stride=64 * 64, n_seq=8, lengths=A + 2 ** 20, device=-1)
+    far, met, apart = A + 2 ** 22, 0, 0
+    for n in (1, 2, 5):
+        for out_stride in (256, 384, 512):
+            for k_stride in (0, 64, 128, 256, 384, 512):
+                for off in range(-1024, 1025, 64):
+                    shared = bool(_rows(0, out_stride, 256, n) & _rows(off, k_stride, 128, n))
+                    for name in ("k", "v"):
+                        a = append(kv, tokens=n, heads=2, q=far, q_out=A + 8192, q_stride=128, q_out_stride=out_stride // 2, pos=far, past=far,
+                                   **{"k": far, "v": far, name: A + 8192 + off, "k_stride": 64, "v_stride": 64, name + "_stride": k_stride // 2})
+                        rc = L.s2d_cache_append(ctypes.byref(one), ctypes.byref(a), None, err, 256)
+                        assert rc != 0 and (b"k or v" in err.value) == shared, (n, out_stride, k_stride, off, err.value)
+                    met, apart = met + shared, apart + (not shared)
+    assert met > 500 and apart > 500
+
+
+def test_append_output_over_the_queries(kv):
+    """The queries themselves with another stride, or rows that meet theirs, are refused; rows between theirs are not."""
+    L, err = kv.cache_lib(), ctypes.create_string_buffer(256)
+    v = view(kv, lengths=A + 2 ** 20, device=-1)
+    for off, refuse in ((0, False), (512, False), (16, True), (496, True), (-16, True), (1024, True), (1536, False)):
+        a = append(kv, q=A + 8192, q_out=A + 8192 + off, q_stride=512, q_out_stride=512, k=A + 2 ** 21, v=A + 2 ** 21, pos=A + 2 ** 21)
+        L.s2d_cache_append(ctypes.byref(v), ctypes.byref(a), None, err, 256)
+        assert (b"q_out" in err.value) == refuse, (off, err.value)
+    assert "q_out" in refused(kv, "s2d_cache_append", v, append(kv, q_stride=512, q_out_stride=256, k=A + 2 ** 21, v=A + 2 ** 21, pos=A + 2 ** 21))
