@@ -492,8 +492,8 @@ const char *attention_fault(const S2dCacheView *c, const S2dCacheAttention *a) {
     if (a->q_stride % w || a->out_stride % w || !cache_aligned16(a->q) || !cache_aligned16(a->out))
         return "misaligned buffer: rows of q and out must be 16-byte aligned";
     if (a->q_stride < 0 || (a->tokens > 1 && a->out_stride < row)) return "q_stride must not be negative, and rows of out must not overlap";
-    const size_t es = a->type == S2D_TYPE_F32 ? 4 : 2, last = a->tokens > 0 ? (size_t)a->tokens - 1 : 0;
-    if (a->tokens && cache_overlap(a->q, es * ((size_t)a->q_stride * last + row), a->out, es * ((size_t)a->out_stride * last + row)))
+    const int64_t es = a->type == S2D_TYPE_F32 ? 4 : 2;
+    if (a->tokens && cache_rows_overlap({a->q, a->q_stride * es, row * es}, {a->out, a->out_stride * es, row * es}, a->tokens))
         return "out must not overlap q";
     return nullptr;
 }

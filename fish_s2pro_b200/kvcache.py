@@ -272,7 +272,8 @@ class PagedKvCache:
         mass.  A token that sees nothing gives zeros.  Returns out, or (out,
         lse) with lse f32 [tokens, heads] the natural log of the sum of
         exponentials (-inf where a token sees nothing); rows past
-        q_start[n_seq] are not written.  out, if given, must not overlap q."""
+        q_start[n_seq] are not written.  The rows of out, if given, lie apart
+        from q's (slices of one packed tensor will do)."""
         ty = self._type("q", q)
         qp, qs = self._rows("q", q)
         tokens, heads = q.shape[0], q.shape[1]

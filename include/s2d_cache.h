@@ -124,7 +124,7 @@ int32_t s2d_cache_append(const S2dCacheView *view, const S2dCacheAppend *args, v
 typedef struct S2dCacheAttention {
     const void *q;             /* [tokens][heads][head_dim]                        */
     int64_t q_stride;
-    void *out;                 /* [tokens][heads][head_dim]; must not overlap q      */
+    void *out;                 /* [tokens][heads][head_dim]; rows share no byte with q's */
     int64_t out_stride;
     float *lse;                /* [tokens][heads] natural log of the softmax's sum, or NULL */
     const int32_t *q_start;    /* [n_seq + 1] or NULL                               */

@@ -806,3 +806,15 @@ def test_append_refuses_an_output_over_keys_or_values(torch):
     assert s.c.append(q, k, v, s.ints([1, 2]), past, out=spare).data_ptr() == spare.data_ptr()
     s.c.check()
     assert torch.equal(spare, want) and torch.equal(packed[:, :6], before[:, :6])
+
+
+@pytest.mark.parametrize("tokens", [None, [30, 4]])
+def test_attention_output_beside_the_queries(torch, tokens):
+    """q and out as slices of one packed tensor, each token's output behind its queries."""
+    s = Case(torch, "bf16", 8, 2, 64, [50, 60], tokens, 70, seed=44)
+    packed = torch.zeros(s.q.shape[0], 17, 64, dtype=torch.bfloat16, device="cuda")
+    packed[:, :8] = s.q
+    s.q = packed[:, :8]
+    out, lse = s.attend(out=packed[:, 9:])
+    s.compare(out, lse)
+    assert torch.all(packed[:, 8] == 0) and np.array_equal(packed[:, :8].double().cpu().numpy(), s.q64)

@@ -204,3 +204,12 @@ def test_append_output_over_the_queries(kv):
         L.s2d_cache_append(ctypes.byref(v), ctypes.byref(a), None, err, 256)
         assert (b"q_out" in err.value) == refuse, (off, err.value)
     assert "q_out" in refused(kv, "s2d_cache_append", v, append(kv, q_stride=512, q_out_stride=256, k=A + 2 ** 21, v=A + 2 ** 21, pos=A + 2 ** 21))
+
+
+def test_attention_output_between_the_queries_rows(kv):
+    """Rows of 512 bytes, 1,024 apart: out between q's rows is taken (and there is no device -1 to run it), over them refused."""
+    L, err = kv.cache_lib(), ctypes.create_string_buffer(256)
+    for off, refuse in ((512, False), (528, True), (496, True), (-512, False), (-496, True), (1024, True), (0, True)):
+        a = attention(kv, q=A + 8192, out=A + 8192 + off, q_stride=512, out_stride=512)
+        assert L.s2d_cache_attention(ctypes.byref(view(kv, device=-1)), ctypes.byref(a), None, err, 256) == (-1 if refuse else -3)
+        assert (b"overlap" in err.value) == refuse, (off, err.value)
