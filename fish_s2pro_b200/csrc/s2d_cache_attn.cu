@@ -153,7 +153,11 @@ constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots
 // slots, contiguous ranges) and in each by four warps in turn, every warp with
 // its own two-stage copy ring.  MMA rows 0-7 hold the heads' values, rows 8-15
 // the remainders of what the cache's type rounds (f32 queries, and the weights
-// of every type), so the sums have f32's precision at no extra MMA.
+// of every type), so the sums have f32's precision at no extra MMA.  f16 has no
+// exponents below 2^-24: weights are taken from a reference 2^14 below the
+// maximum, which leaves every one of them right to 2^-39 of the largest (from
+// the maximum itself it was 2^-25: 32,768 slots 25 binades below one of them
+// lost a quarter of what they add, 2.4e-4).
 //
 // The CTAs' parts meet through distributed shared memory; without a prefix the
 // call needs no kernel to join them.  KEEP (weighing): the scores stay in
@@ -170,6 +174,7 @@ constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots
 template <typename Q, typename E, int HD, bool KEEP>
 __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const S2dCacheAttention a, const AttnPlan p, int score_pitch) {
     constexpr int KC = 16, NO = HD / 8, UNITS = HD / 8, PITCH = HD * 2 + 16, STAGE = 2 * KC * PITCH, NW = 4, R = 8;
+    constexpr float kBelow = std::is_same<E, __half>::value ? 14.f : 0.f;  // the reference of the weights below their maximum
     extern __shared__ __align__(16) uint8_t sm[];
     __shared__ float2 s_ml[R];        // this CTA's (m, l) of each row
     __shared__ float s_lse[R];        // lse2 of each row
@@ -257,7 +262,7 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mnew = fmaxf(mrun, mx), base = mnew == -INFINITY ? 0.f : mnew;  // nothing seen yet: all weights 0
+        const float mnew = fmaxf(mrun, mx - kBelow), base = mnew == -INFINITY ? 0.f : mnew;  // nothing seen yet: all weights 0
         const float corr = exp2f(mrun - base);
         mrun = mnew;
         uint32_t pa[4];

@@ -818,3 +818,38 @@ def test_attention_output_beside_the_queries(torch, tokens):
     out, lse = s.attend(out=packed[:, 9:])
     s.compare(out, lse)
     assert torch.all(packed[:, 8] == 0) and np.array_equal(packed[:, :8].double().cpu().numpy(), s.q64)
+
+
+def one_above_many(torch, ty, n, gap, n_seq, G=8, tokens=None):
+    """One slot (key 1, value 0) and n - 1 slots (key 0, value 1), which get 2^-gap of its weight each.  n_seq sequences over the
+    same pages, or a prompt of `tokens` behind them as its prefix: (results, what all of them should be)."""
+    from fish_s2pro_b200 import PagedKvCache
+    D, dtype = 64, act_dtype(torch, ty)
+    kv = torch.bfloat16 if ty == "bf16" else torch.float16
+    k, v = torch.zeros(9, G, PAGE, D, dtype=kv, device="cuda"), torch.ones(9, G, PAGE, D, dtype=kv, device="cuda")
+    k[0, :, 0, 0], v[0, :, 0] = 1.0, 0.0
+    ids = torch.arange(n // PAGE, device="cuda") % 8 + 1  # the eight other pages again and again
+    ids[0] = 0
+    ids = ids.to(torch.int32)
+    q = torch.zeros(tokens or n_seq, G, D, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    if tokens:
+        c = PagedKvCache(k, v, ints([[1]]), ints([0]))
+        got = c.attention(q, q_start=ints([0, tokens]), prefix_pages=ids, prefix_len=n, scale=gap * math.log(2))
+    else:
+        c = PagedKvCache(k, v, ids.expand(n_seq, -1).contiguous(), ints([n] * n_seq))
+        got = c.attention(q, scale=gap * math.log(2))
+    c.check()
+    w = (n - 1) * 2.0 ** -gap
+    return got.double().cpu().numpy(), w / (1 + w)
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [8192, 32768])
+@pytest.mark.parametrize("gap", [15.5, 25.05, 31.1])
+def test_single_tokens_count_small_weights(torch, ty, n, gap):
+    """Weights far below the largest count in the sum and in the values alike, down to where all of them together are below the
+    tolerance (values are at most 1).  Enough sequences that one CTA takes each one's slots."""
+    got, want = one_above_many(torch, ty, n, gap, 80)
+    assert np.max(np.abs(got - want)) <= F32_TOL + (HALF_STEP[ty] * want if ty != "f32" else 0)
