@@ -157,7 +157,10 @@ constexpr int kMaxParts = 64;  // position splits of the prefix, or of own slots
 // exponents below 2^-24: weights are taken from a reference 2^14 below the
 // maximum, which leaves every one of them right to 2^-39 of the largest (from
 // the maximum itself it was 2^-25: 32,768 slots 25 binades below one of them
-// lost a quarter of what they add, 2.4e-4).
+// lost a quarter of what they add, 2.4e-4).  An MMA truncates what it adds to, so
+// each chunk starts from 0 and is added to O with rounding, in the instruction
+// that rescales O anyway (summed in the MMAs, equal weights over 32,768 slots
+// came out 5.1e-5 too small, over 131,072 2.1e-4).
 //
 // The CTAs' parts meet through distributed shared memory; without a prefix the
 // call needs no kernel to join them.  KEEP (weighing): the scores stay in
@@ -275,15 +278,14 @@ __global__ void __launch_bounds__(128) token_kernel(const S2dCacheView c, const 
         }
         lrun = fmaf(lrun, corr, sum);
 #pragma unroll
-        for (int j = 0; j < NO; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] *= corr;
-#pragma unroll
         for (int nd = 0; nd < HD / 16; ++nd) {
             uint32_t vf[4];
             ldsm4_trans(vf, vt + ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (nd * 16 + (lane >> 4) * 8) * 2);
-            mma<E>(o[2 * nd], pa, vf[0], vf[1]);
-            mma<E>(o[2 * nd + 1], pa, vf[2], vf[3]);
+            float d[2][4] = {};
+            mma<E>(d[0], pa, vf[0], vf[1]);
+            mma<E>(d[1], pa, vf[2], vf[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[2 * nd][e] = fmaf(o[2 * nd][e], corr, d[0][e]), o[2 * nd + 1][e] = fmaf(o[2 * nd + 1][e], corr, d[1][e]);
         }
         __syncwarp();  // the stage is read before it is filled again
     }

@@ -853,3 +853,42 @@ def test_single_tokens_count_small_weights(torch, ty, n, gap):
     tolerance (values are at most 1).  Enough sequences that one CTA takes each one's slots."""
     got, want = one_above_many(torch, ty, n, gap, 80)
     assert np.max(np.abs(got - want)) <= F32_TOL + (HALF_STEP[ty] * want if ty != "f32" else 0)
+
+
+def periodic(torch, ty, H, G, D, n, n_seq=None, tokens=None):
+    """n positions (a multiple of 4,096) over the same 64 pages again and again, values in [1/2, 3/2]: as the prefix of `tokens`
+    packed tokens, or as the slots of n_seq single ones.  (out, lse, what they should be): softmax over the period, its sum times
+    the periods."""
+    from fish_s2pro_b200 import PagedKvCache
+    gen = torch.Generator(device="cuda").manual_seed(n + D)
+    kv = torch.bfloat16 if ty == "bf16" else torch.float16
+    k = torch.randn(64, G, PAGE, D, generator=gen, device="cuda").to(kv)
+    v = (torch.rand(64, G, PAGE, D, generator=gen, device="cuda") + 0.5).to(kv)
+    ids = (torch.arange(n // PAGE, device="cuda") % 64).to(torch.int32)
+    q = torch.randn(tokens or n_seq, H, D, generator=gen, device="cuda").to(act_dtype(torch, ty))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    if tokens:
+        c = PagedKvCache(k, v, ints([[0]]), ints([0]))
+        out, lse = c.attention(q, q_start=ints([0, tokens]), prefix_pages=ids, prefix_len=n, return_lse=True)
+    else:
+        c = PagedKvCache(k, v, ids.expand(n_seq, -1).contiguous(), ints([n] * n_seq))
+        out, lse = c.attention(q, return_lse=True)
+    c.check()
+    rows = lambda x: x.permute(1, 0, 2, 3).reshape(G, -1, D).double()
+    s = torch.einsum("tgrd,gnd->tgrn", q.double().view(-1, G, H // G, D), rows(k)) / math.sqrt(D)
+    want = torch.einsum("tgrn,gnd->tgrd", s.softmax(-1), rows(v)).reshape(out.shape)
+    return out.double(), lse.double(), want, torch.logsumexp(s, -1).reshape(lse.shape) + math.log(n // 4096)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ty,n", [("f32", 8192), ("f32", 65536), ("f16", 131072), ("bf16", 524288)])
+def test_single_tokens_over_long_caches(torch, ty, n, D):
+    """Sums over many slots of like values, one CTA a (sequence, KV head): each element to the bounds of the short cases, and
+    their mean to f32's and what roundings of 16-bit results leave of it.  All sequences see nearly the same means of the values,
+    so 8 D roundings are independent, each of them even over [-u, u], of deviation u / sqrt(3); four deviations of their mean are
+    4 u / sqrt(3 * 8 D)."""
+    out, lse, want, want_lse = periodic(torch, ty, 8, 8, D, n, n_seq=80)
+    u = HALF_STEP[ty] if ty != "f32" else 0.0
+    assert torch.all((out - want).abs() <= u * want + 1.5 * F32_TOL)
+    assert abs(float((out - want).mean())) <= 1.5 * F32_TOL + 4 * u / math.sqrt(24 * D) * float(want.mean())
+    assert torch.all((lse - want_lse).abs() <= F32_TOL * want_lse)
