@@ -33,9 +33,13 @@
 // where it is added with rounding (1.2e-6 at any length).
 //
 // m is not the running maximum itself but a reference that follows it: it is
-// set 6 below the first tile's maximum and moves (and what is summed so far is
-// rescaled) only when a tile's maximum is more than 14 above it.  P stays
-// below 2^14, an f16, and its small entries keep their bits.
+// set kBelow below the first tile's maximum and moves (and what is summed so far
+// is rescaled) only when a tile's maximum is more than kAbove above it.  For f16
+// these are 9 and 15: P stays below 2^15, and half of f16's smallest step is
+// 2^-34 of the largest weight, so that what is rounded away stays below 2e-5
+// over 2^18 positions (set 6 below, 2^-31: as many positions 31 binades below one
+// of them were lost, 1.1e-4 of the result).  bf16 has f32's exponents, and 6 and
+// 14 move the reference less often.
 //
 // Warps: 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (warp w owns
 // TMEM lanes 32 (w % 4) ..), 8 loads K and V pages by TMA (one page of 64
@@ -603,6 +607,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t st = lane_t + (uint32_t)(q * BN), ot = lane_t + Sh::kO + (uint32_t)(q * HD);
         const uint32_t qdst = sbase + (uint32_t)q * Sh::kQTile;
+        constexpr float kBelow = std::is_same<E, __half>::value ? 9.f : 6.f, kAbove = std::is_same<E, __half>::value ? 15.f : 14.f;
         uint32_t ns = 0, nd = 0;  // S tiles taken so far (P V tiles done are as many); items shared by both warpgroups
         bool ok = true;
         TcPlace at;
@@ -727,8 +732,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     mx = max_of(s);
                 }
                 mx *= qmul;
-                const bool up = mx > mref + 14.f;
-                const float mnew = up ? mx - 6.f : mref;
+                const bool up = mx > mref + kAbove;
+                const float mnew = up ? mx - kBelow : mref;
                 const float corr = up && mref > -INFINITY ? ex2(mref - mnew) : 1.f;
                 const bool rescale = jj > 0 && __any_sync(0xffffffffu, corr != 1.f);
                 const bool flushes = Sh::kF32 && jj > 0 && (rescale || jj % Sh::kFlush == 0);

@@ -892,3 +892,15 @@ def test_single_tokens_over_long_caches(torch, ty, n, D):
     assert torch.all((out - want).abs() <= u * want + 1.5 * F32_TOL)
     assert abs(float((out - want).mean())) <= 1.5 * F32_TOL + 4 * u / math.sqrt(24 * D) * float(want.mean())
     assert torch.all((lse - want_lse).abs() <= F32_TOL * want_lse)
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [32768, 262144])
+@pytest.mark.parametrize("gap", [15.5, 25.05, 31.1])
+def test_prompts_count_small_weights(torch, ty, n, gap):
+    """The same for packed tokens behind a prefix, enough of them that one CTA takes all positions of its rows.  16-bit queries
+    round each weight to half a step, here all of them alike.  O and l are f32 sums over n / 128 tiles, whose addends are all the
+    same here: each sum rounds by up to 2^-24 of itself, and always to the same side, so O / l is off by up to 2 n / 128 of that."""
+    got, want = one_above_many(torch, ty, n, gap, 1, tokens=2400)
+    u = HALF_STEP[ty] if ty != "f32" else 0.0
+    assert np.max(np.abs(got - want)) <= F32_TOL + 2 * (u + n / 128 * 2.0 ** -24) * want
