@@ -220,7 +220,7 @@ template <typename Q, typename E>
 cudaError_t append_launch(const S2dCacheView &c, const S2dCacheAppend &a, const RopeTurns &r, cudaStream_t s) {
     // as few waves of blocks as groups of kGroup tokens take, all of them full:
     // of 36,900 tokens, groups of 32 (1.95 waves) take 168 us, of 28 (2.2) 188
-    constexpr int kRun = 148 * 4;
+    constexpr int kRun = kCacheSms * 4;
     const int waves = std::max(1, (int)(((int64_t)a.tokens + kRun * kGroup - 1) / (kRun * kGroup)));
     const int tokens = std::max(1, (int)(((int64_t)a.tokens + kRun * waves - 1) / (kRun * waves)));
     const unsigned blocks = (unsigned)std::max<int64_t>(1, ((int64_t)a.tokens + tokens - 1) / tokens);
@@ -570,7 +570,7 @@ int evict_threads(const S2dCacheView &c) {
 // Blocks that share the moves of one (sequence, KV head): as many (up to 8) as
 // run at once, as each chooses for itself.
 int evict_share(const S2dCacheView &c) {
-    const int64_t pairs = (int64_t)c.n_seq * c.kv_heads, most = 148 * (1024 / evict_threads(c));
+    const int64_t pairs = (int64_t)c.n_seq * c.kv_heads, most = kCacheSms * (1024 / evict_threads(c));
     int share = 1;
     while (share < 8 && pairs * share * 2 <= most) share *= 2;
     return share;

@@ -17,6 +17,7 @@ namespace s2d {
 
 constexpr int kCachePage = S2D_CACHE_PAGE;
 constexpr int kCacheMaxRep = 16;
+constexpr int kCacheSms = 148;  // SMs of a B200, which grids and plans are made for
 
 // Two f32 as a pair of 16-bit elements, and back.
 template <typename E>

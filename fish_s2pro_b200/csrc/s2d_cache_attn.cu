@@ -507,7 +507,7 @@ const char *attention_fault(const S2dCacheView *c, const S2dCacheAttention *a) {
 
 constexpr int kTcTile = 256;      // query rows of a tcgen05 item
 constexpr int kMaxCluster = 8;    // CTAs that share one (sequence, KV head) of single tokens
-constexpr int kSms = 148;
+constexpr int kSms = kCacheSms;
 constexpr int kTokenSmemMost = 224 * 1024;
 constexpr int kTokenSmemTwo = 111 * 1024;  // of each of two CTAs on an SM
 
@@ -603,6 +603,12 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
     p.next_item = reinterpret_cast<int *>(take(p.prefix_tiles || p.own_tiles ? sizeof(int) : 0));
     const bool again = a.weigh && (a.q_start || !score_pitch(c, a, p));  // weights by computing the scores again
     p.lse2 = reinterpret_cast<float *>(take(again ? sizeof(float) * ids : 0));
+    // the most tiles that an item may take
+    auto tiles_of = [](int64_t positions, int splits) { return ((positions + kTcTilePositions - 1) / kTcTilePositions + splits - 1) / splits; };
+    const int64_t pooled_tiles = p.prefix_tiles ? tiles_of(a.prefix_len, p.prefix_splits) : 0;
+    const int64_t own_tiles = p.own_tiles ? (p.fused ? tiles_of(a.prefix_len, 1) : 0) + tiles_of((int64_t)c.max_pages * kCachePage, p.own_splits) : 0;
+    const bool hold = a.type != S2D_TYPE_F32 && std::max(pooled_tiles, own_tiles) > kTcHold;
+    p.held = reinterpret_cast<float *>(take(hold ? sizeof(float) * kSms * kTcTile * c.head_dim : 0));
     bytes = at;
 }
 

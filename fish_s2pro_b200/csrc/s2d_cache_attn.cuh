@@ -39,7 +39,12 @@ struct AttnPlan {
     float2 *ml;                       // [tokens][heads][parts]
     int *next_item;                   // what the tcgen05 CTAs draw further items from
     float *lse2;                      // [tokens][heads] in base 2, for the weigh kernel, or NULL
+    float *held;                      // [CTAs][2][head_dim / 4][128][4]: O of earlier tiles, where an item of 16-bit rows may take over kTcHold; or NULL
 };
+
+// Tiles of positions, and the tiles that O of 16-bit rows takes in the tensor
+// core's accumulator before it is added up in f32 with rounding.
+constexpr int kTcTilePositions = 128, kTcHold = 64;
 
 // row / rep without a division, for rows below 2^28 (rep <= 16).
 __device__ __forceinline__ int row_token(const AttnPlan &p, int row) { return p.rep_inv ? (int)__umulhi((uint32_t)row, p.rep_inv) : row; }

@@ -27,10 +27,16 @@
 // error, half a step of that type, is that of the output's own rounding).
 //
 // f32 queries: Q and P enter as f16 pairs hi + lo (two MMAs into one
-// accumulator, about 22 bits).  Every MMA step of 16 positions truncates its
-// sum to f32 (measured: 1.6e-8 of the result a step, all toward zero: 3.4e-5
-// after 16,000 positions), so O is moved every kFlush tiles into registers,
-// where it is added with rounding (1.2e-6 at any length).
+// accumulator, about 22 bits).
+//
+// Every MMA step of 16 positions truncates its sum to f32, always toward zero:
+// up to 1.0e-7 of the result a step (equal weights, values of one sign).  So O
+// is moved and added up with rounding every kFlush tiles: of f32 rows every two
+// tiles, into registers (1.5e-6 at any length); of 16-bit rows, which have no
+// registers left, every kTcHold = 64 into device memory that the CTA keeps to
+// itself (p.held, which stays in L2): 5e-5 at any length, a ninth of half an f16
+// step, where 131,072 positions without it came out 8.4e-4 too small and 2^20
+// 6.7e-3.
 //
 // m is not the running maximum itself but a reference that follows it: it is
 // set kBelow below the first tile's maximum and moves (and what is summed so far
@@ -206,7 +212,7 @@ __device__ __forceinline__ void mask(uint32_t (&s)[N], int vis) {
 template <typename Q, int HD>
 struct TcShape {
     static constexpr bool kF32 = sizeof(Q) == 4;
-    static constexpr int BN = 128;                         // positions per tile
+    static constexpr int BN = kTcTilePositions;            // positions per tile
     static constexpr int kPages = BN / kCachePage;         // pages per tile
     static constexpr int kHalves = HD / 64;                // 128-byte column blocks of a row
     static constexpr int kSplit = kF32 ? 2 : 1;            // hi and lo
@@ -217,11 +223,53 @@ struct TcShape {
     static constexpr int kFit = (224 * 1024 - 2 * kQTile) / kSlot;
     static constexpr int kSlots = kFit < 8 ? kFit : 8;     // K and V tiles in flight
     static constexpr int kSmem = 2 * kQTile + kSlots * kSlot + 1024;
-    static constexpr int kFlush = 2;                       // f32: tiles that O takes before it moves to registers
+    static constexpr int kFlush = kF32 ? 2 : kTcHold;      // tiles that O takes before it moves, f32: to registers, else to p.held
     static constexpr uint32_t kO = 2 * BN;                 // TMEM: S0, S1 (BN columns each), O0, O1 (HD each)
     static_assert(kO + 2 * HD <= kTcColumns, "TMEM columns");
     static_assert(kSlots >= 3, "K and V of a tile and the next K");
 };
+
+// What is put aside of O of a 16-bit row (see the top): by the row's thread, 16
+// columns at a time, in functions of their own between two tiles, where no score
+// is held in registers: inline, or in the midst of a tile, long prompts take 1 %
+// more.
+//
+// held = by * held + O, or O alone
+template <int HD>
+__device__ __noinline__ void hold(uint32_t ot, float4 *held, bool more, float by) {
+#pragma unroll 1
+    for (int i = 0; i < HD; i += 16) {
+        uint32_t o[16];
+        tmem_ld16(ot + i, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const float4 x = more ? held[(i + e) / 4 * kTcRows] : make_float4(0.f, 0.f, 0.f, 0.f);
+            held[(i + e) / 4 * kTcRows] = make_float4(fmaf(x.x, by, __uint_as_float(o[e])), fmaf(x.y, by, __uint_as_float(o[e + 1])),
+                                                      fmaf(x.z, by, __uint_as_float(o[e + 2])), fmaf(x.w, by, __uint_as_float(o[e + 3])));
+        }
+    }
+}
+// O += by * held
+template <int HD>
+__device__ __noinline__ void hold_back(uint32_t ot, const float4 *held, float by) {
+#pragma unroll 1
+    for (int i = 0; i < HD; i += 16) {
+        uint32_t o[16];
+        tmem_ld16(ot + i, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; e += 8) {
+            const float4 x = held[(i + e) / 4 * kTcRows], y = held[((i + e) / 4 + 1) * kTcRows];
+            const float add[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            uint32_t w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(fmaf(add[k], by, __uint_as_float(o[e + k])));
+            tmem_st8(ot + i + e, w);
+        }
+    }
+    tmem_wait_st();
+}
 
 // Where an item lies.
 struct TcPlace {
@@ -539,7 +587,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint32_t v = slot_base(load) + (uint32_t)(half * (BN / 32) * 2048), d = tmem + Sh::kO + (uint32_t)(q * HD);
                 const uint32_t pt = tmem + (uint32_t)(q * BN + half * (Sh::kF32 ? BN / 2 : BN / 4));
                 const int jj = it.dual ? j >> 1 : j;  // the warpgroup's own count
-                const bool fresh = Sh::kF32 ? jj % Sh::kFlush == 0 : jj == 0;
+                const bool fresh = jj % Sh::kFlush == 0;
 #pragma unroll
                 for (int part = 0; part < Sh::kSplit; ++part)
 #pragma unroll
@@ -685,10 +733,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
 
             const int own_limit = min(it.pooled ? 0 : max(0, it.back + rt + 1), it.own1) - it.own0;  // own slots of the item that this row sees
-            float mref = -INFINITY, l = 0.f;
+            float mref = -INFINITY, l = 0.f, fade = 1.f;  // fade: what `held` is to be rescaled by
             float acc[Sh::kF32 ? HD : 1];
 #pragma unroll
             for (int i = 0; i < (Sh::kF32 ? HD : 1); ++i) acc[i] = 0.f;
+            // 16-bit: where O goes after kFlush tiles, elements 4 i .. 4 i + 3 of the row at [128 i]
+            float4 *const held = reinterpret_cast<float4 *>(p.held) + ((int64_t)blockIdx.x * 2 + q) * (HD / 4) * kTcRows + r;
             // acc += O (f32), once P V of the last tile is done
             auto flush = [&](bool clear) {
                 if constexpr (Sh::kF32) {
@@ -709,6 +759,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             };
             for (int jj = 0; jj < J; ++jj, ++ns) {
                 const int j = it.dual ? 2 * jj + q : jj;
+                if (!Sh::kF32 && jj > 0 && jj % Sh::kFlush == 0) {
+                    // the next P V starts O anew
+                    if (!(ok = warp_wait(&sh.pv_done[q], (ns - 1) & 1, abort_v))) break;
+                    tc_fence_after();
+                    hold<HD>(ot, held, jj > Sh::kFlush, fade);
+                    fade = 1.f;
+                }
                 if (!(ok = warp_wait(&sh.s_full[q], ns & 1, abort_v))) break;
                 tc_fence_after();
                 const int vis = !real ? BN : j < it.jp ? it.pre1 - it.pre0 - j * BN : own_limit - (j - it.jp) * BN;
@@ -759,7 +816,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tmem_st32(ot + i, o);
                     }
                 }
-                l *= corr;
+                l *= corr, fade *= corr;
                 mref = mnew;
                 const float base = mref == -INFINITY ? 0.f : mref;  // nothing seen yet: every score is -inf
                 const uint64_t qm2 = two(qmul, qmul), nb2 = two(-base, -base);
@@ -811,6 +868,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!ok) break;
             tc_fence_after();
             if (J > 0) flush(false);
+            if (!Sh::kF32 && J > Sh::kFlush) hold_back<HD>(ot, held, fade);
             float mine = 1.f, other = 0.f;  // what this warpgroup's and the other's O count
             if (it.dual) {
                 // the second warpgroup's part goes to the first, which shares its TMEM lanes: O is there (f32: put there), (m, l)
@@ -1200,6 +1258,7 @@ cudaError_t launch(const S2dCacheView &c, const S2dCacheAttention &a, const Attn
     int sms = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device))) return e;
     AttnPlan q = p;
+    sms = std::min(sms, kCacheSms);  // p.held has room for as many CTAs
     if (items <= sms) q.next_item = nullptr;  // one item each
     if (q.next_item && (e = cudaMemsetAsync(q.next_item, 0, sizeof(int), s))) return e;
     rows_tc_kernel<Q, E, HD><<<(unsigned)std::min<int64_t>(items, sms), kTcThreads, smem, s>>>(mk, mv, c, a, q);

@@ -855,10 +855,10 @@ def test_single_tokens_count_small_weights(torch, ty, n, gap):
     assert np.max(np.abs(got - want)) <= F32_TOL + (HALF_STEP[ty] * want if ty != "f32" else 0)
 
 
-def periodic(torch, ty, H, G, D, n, n_seq=None, tokens=None):
+def periodic(torch, ty, H, G, D, n, n_seq=None, tokens=None, packed=False):
     """n positions (a multiple of 4,096) over the same 64 pages again and again, values in [1/2, 3/2]: as the prefix of `tokens`
-    packed tokens, or as the slots of n_seq single ones.  (out, lse, what they should be): softmax over the period, its sum times
-    the periods."""
+    packed tokens, or as the slots of n_seq single ones (packed: the same by q_start).  (out, lse, what they should be): softmax
+    over the period, its sum times the periods."""
     from fish_s2pro_b200 import PagedKvCache
     gen = torch.Generator(device="cuda").manual_seed(n + D)
     kv = torch.bfloat16 if ty == "bf16" else torch.float16
@@ -872,7 +872,7 @@ def periodic(torch, ty, H, G, D, n, n_seq=None, tokens=None):
         out, lse = c.attention(q, q_start=ints([0, tokens]), prefix_pages=ids, prefix_len=n, return_lse=True)
     else:
         c = PagedKvCache(k, v, ids.expand(n_seq, -1).contiguous(), ints([n] * n_seq))
-        out, lse = c.attention(q, return_lse=True)
+        out, lse = c.attention(q, q_start=ints(list(range(n_seq + 1))) if packed else None, return_lse=True)
     c.check()
     rows = lambda x: x.permute(1, 0, 2, 3).reshape(G, -1, D).double()
     s = torch.einsum("tgrd,gnd->tgrn", q.double().view(-1, G, H // G, D), rows(k)) / math.sqrt(D)
@@ -904,3 +904,58 @@ def test_prompts_count_small_weights(torch, ty, n, gap):
     got, want = one_above_many(torch, ty, n, gap, 1, tokens=2400)
     u = HALF_STEP[ty] if ty != "f32" else 0.0
     assert np.max(np.abs(got - want)) <= F32_TOL + 2 * (u + n / 128 * 2.0 ** -24) * want
+
+
+@pytest.mark.parametrize("ty,n,kw", [
+    ("f16", 131072, dict(tokens=2400, D=128)),              # row tiles of 256 behind a prefix
+    ("bf16", 1048576, dict(tokens=2400, D=64)),
+    ("f16", 131072, dict(n_seq=40, packed=True, D=128)),    # few rows: the positions of one row tile by both warpgroups
+    ("bf16", 1048576, dict(n_seq=40, packed=True, D=64)),
+    ("f16", 131072, dict(tokens=9000, D=64)),               # prefix and own slots by one item
+    ("f32", 65536, dict(tokens=2400, D=128)),
+    ("f32", 65536, dict(n_seq=40, packed=True, D=64)),
+    ("f16", 8192, dict(tokens=2400, D=64)),                 # as many tiles as O takes at a time, and one more
+    ("f16", 12288, dict(tokens=2400, D=128)),
+])
+def test_rows_over_long_ranges(torch, ty, n, kw):
+    """Sums over many positions of like values on the tensor core: elements and their mean to the bounds of the single tokens'
+    test, with half a step more for 16-bit weights."""
+    out, lse, want, want_lse = periodic(torch, ty, 8, 8, n=n, **kw)
+    u = HALF_STEP[ty] if ty != "f32" else 0.0
+    assert torch.all((out - want).abs() <= 2 * u * want + 1.5 * F32_TOL)
+    assert abs(float((out - want).mean())) <= 1.5 * F32_TOL + (u / 8 + 4 * u / math.sqrt(24 * kw["D"])) * float(want.mean())
+    assert torch.all((lse - want_lse).abs() <= F32_TOL * want_lse)
+
+
+@pytest.mark.parametrize("ty,D", [("f16", 128), ("bf16", 64), ("f32", 64)])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_rows_whose_scores_climb_over_long_ranges(torch, ty, D, prefix):
+    """25,600 positions whose keys grow by a factor of eight on the way: the running reference of the softmax moves after tiles of
+    O have been put aside, too, and then they are rescaled with it."""
+    from fish_s2pro_b200 import PagedKvCache
+    G, n = 8, 25600
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    kv = torch.bfloat16 if ty == "bf16" else torch.float16
+    grow = 1.0 + 7.0 * torch.arange(n // PAGE, device="cuda") / (n // PAGE)
+    k = (torch.randn(n // PAGE, G, PAGE, D, generator=gen, device="cuda") * grow[:, None, None, None]).to(kv)
+    v = torch.randn(n // PAGE, G, PAGE, D, generator=gen, device="cuda").to(kv)
+    ids = torch.arange(n // PAGE, device="cuda", dtype=torch.int32)
+    T = 4800 if prefix else 40
+    q = torch.randn(T, G, D, generator=gen, device="cuda").to(act_dtype(torch, ty))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    if prefix:
+        c = PagedKvCache(k, v, ints([[0]]), ints([0]))
+        out = c.attention(q, q_start=ints([0, T]), prefix_pages=ids, prefix_len=n)
+    else:
+        c = PagedKvCache(k, v, ids.expand(T, -1).contiguous(), ints([n] * T))
+        out = c.attention(q, q_start=ints(list(range(T + 1))))
+    c.check()
+    some = torch.arange(0, T, 97 if prefix else 1, device="cuda")
+    rows = lambda x: x.permute(1, 0, 2, 3).reshape(G, -1, D).double()
+    s = torch.einsum("tgd,gnd->tgn", q[some].double(), rows(k)) / math.sqrt(D)
+    w = s.softmax(-1)
+    want, spread = torch.einsum("tgn,gnd->tgd", w, rows(v)), torch.einsum("tgn,gnd->tgd", w, rows(v).abs())
+    u = HALF_STEP[ty]
+    # scores reach some tens: 2^-24 of them in an exponent, and the products' truncation (8 steps of 16 elements), 2^-20 of a weight
+    bound = u * want.abs() + (u if ty != "f32" else 0) * spread + (2.0 ** -20 * float(s.abs().max()) * spread) + F32_TOL * float(v.abs().max())
+    assert torch.all((out[some].double() - want).abs() <= bound)
