@@ -959,3 +959,24 @@ def test_rows_whose_scores_climb_over_long_ranges(torch, ty, D, prefix):
     # scores reach some tens: 2^-24 of them in an exponent, and the products' truncation (8 steps of 16 elements), 2^-20 of a weight
     bound = u * want.abs() + (u if ty != "f32" else 0) * spread + (2.0 ** -20 * float(s.abs().max()) * spread) + F32_TOL * float(v.abs().max())
     assert torch.all((out[some].double() - want).abs() <= bound)
+
+
+def test_gains_that_require_a_gradient_are_refused(torch):
+    """The gains are a model's parameters: with gradients on, the queries would be cut off from them.  Without, they are taken.
+    The same for a cache of such tensors."""
+    from fish_s2pro_b200 import PagedKvCache, S2dError
+    s = Case(torch, "f16", 8, 2, 64, [30, 40], None, 0, seed=45)
+    kn, gain = torch.ones(2, 2, 64, dtype=torch.float16, device="cuda"), torch.nn.Parameter(torch.full((64,), 2.0, device="cuda"))
+    pos, past = s.ints([1, 2]), s.ints([3, 4])
+    for kw in (dict(q_norm=gain), dict(k_norm=gain), dict(q_norm=gain, k_norm=gain.detach())):
+        with pytest.raises(S2dError, match="gradient") as e:
+            s.c.append(s.q, kn, kn, pos, past, **kw)
+        assert e.value.code == -1
+    want = s.c.append(s.q, kn, kn, pos, past, q_norm=gain.detach(), k_norm=gain.detach())
+    with torch.no_grad():
+        assert torch.equal(s.c.append(s.q, kn, kn, pos, past, q_norm=gain, k_norm=gain), want)
+    s.c.check()
+    k = s.c.k.clone().requires_grad_()
+    for buffers in ((k, s.c.v), (s.c.k, k)):
+        with pytest.raises(S2dError, match="gradient"):
+            PagedKvCache(*buffers, s.c.page_table, s.c.lengths)
