@@ -980,3 +980,19 @@ def test_gains_that_require_a_gradient_are_refused(torch):
     for buffers in ((k, s.c.v), (s.c.k, k)):
         with pytest.raises(S2dError, match="gradient"):
             PagedKvCache(*buffers, s.c.page_table, s.c.lengths)
+
+
+@pytest.mark.parametrize("end", [-1, -2 ** 31, -2 ** 31 + 40])
+def test_append_of_starts_that_end_below_zero(torch, end):
+    """A last entry so far below zero that its distance to a block's first token is no int: no row is read or written, whichever
+    block it is (650 tokens: groups of two, the last of them past the tokens if it counted)."""
+    from fish_s2pro_b200 import S2dError
+    T = 651
+    s = Case(torch, "f16", 8, 2, 64, [192, 192], [T - 200, 200], 0, seed=47)
+    wide = torch.full((T + 40, 8, 64), 5.0, dtype=torch.float16, device="cuda")
+    kn = torch.ones(T + 40, 2, 64, dtype=torch.float16, device="cuda")
+    before = s.c.v.clone()
+    s.c.append(s.q, kn[:T], kn[:T], s.ints([0] * T), s.ints([0, 0]), q_start=s.ints([0, 100, end]), out=wide[:T])
+    with pytest.raises(S2dError, match="out of range"):
+        s.c.check()
+    assert torch.all(wide == 5.0) and torch.equal(s.c.v.view(torch.int16), before.view(torch.int16))
