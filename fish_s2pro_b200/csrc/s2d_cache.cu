@@ -107,8 +107,9 @@ __global__ void __launch_bounds__(256, 4) append_kernel(const S2dCacheView c, co
     __shared__ int64_t s_at[kGroup], s_side[kGroup];         // a token's cache rows and its positions / mass, of head 0; -1: none
     __shared__ int s_pos[kGroup];
     const int G = c.kv_heads, cap = c.max_pages * kCachePage, tid = threadIdx.x;
-    const int last = a.q_start ? max(0, min(a.tokens, __ldg(a.q_start + c.n_seq))) : min(a.tokens, c.n_seq);  // not negative: last - t0 is an int
-    const int t0 = (int)blockIdx.x * tokens, n = min(tokens, last - t0);
+    // the rows of sequences: [first_row, last), none of them negative, so that their differences are ints; those before and behind stay as they are
+    const int first_row = a.q_start ? max(0, __ldg(a.q_start)) : 0, last = a.q_start ? max(0, min(a.tokens, __ldg(a.q_start + c.n_seq))) : min(a.tokens, c.n_seq);
+    const int t0 = max((int)blockIdx.x * tokens, first_row), n = (int)min((int64_t)(blockIdx.x + 1) * tokens, (int64_t)last) - t0;
     // lengths of every sequence, tokens or none
     for (int b = (int)blockIdx.x * 256 + tid; b < c.n_seq; b += (int)gridDim.x * 256) {
         int first;

@@ -72,7 +72,8 @@ __device__ __forceinline__ int cache_length(const S2dCacheView &c, int b) {
 }
 
 // Rows [first, first + count) of a packed batch that belong to sequence b,
-// held inside [0, tokens].
+// held inside [0, tokens].  Rows before the first sequence's belong to none, and
+// are reported as an entry out of range.
 __device__ __forceinline__ int cache_tokens(const int32_t *q_start, int tokens, int b, int &first, int32_t *status) {
     if (!q_start) {
         first = b;
@@ -84,6 +85,7 @@ __device__ __forceinline__ int cache_tokens(const int32_t *q_start, int tokens, 
         first = 0;
         return 0;
     }
+    if (b == 0 && t0 > 0) cache_flag(status, S2D_CACHE_BAD_LENGTH);
     first = t0;
     return t1 - t0;
 }

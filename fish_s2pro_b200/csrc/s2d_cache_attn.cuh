@@ -49,11 +49,13 @@ constexpr int kTcTilePositions = 128, kTcHold = 64;
 // row / rep without a division, for rows below 2^28 (rep <= 16).
 __device__ __forceinline__ int row_token(const AttnPlan &p, int row) { return p.rep_inv ? (int)__umulhi((uint32_t)row, p.rep_inv) : row; }
 
-// Tokens that belong to some sequence: [0, this).
+// No token at or past this belongs to a sequence, nor one before first_token.
 __device__ __forceinline__ int real_tokens(const S2dCacheAttention &a, int n_seq) {
     const int n = a.q_start ? __ldg(a.q_start + n_seq) : n_seq;
     return max(0, min(n, a.tokens));
 }
+
+__device__ __forceinline__ int first_token(const S2dCacheAttention &a) { return a.q_start ? max(0, __ldg(a.q_start)) : 0; }
 
 // s2d_cache_tc.cu: the items of `p` on tcgen05, and the weights of its rows by
 // computing their scores again (from p.lse2).

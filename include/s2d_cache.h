@@ -90,7 +90,9 @@ typedef struct S2dCacheView {
 
 /* New tokens, packed: token t of sequence b is row q_start[b] + t, for
  * q_start[b + 1] - q_start[b] tokens; rows at and past q_start[n_seq] are
- * padding and left as they are.  q_start NULL: one token per sequence.
+ * padding and left as they are.  q_start[0] is 0: if it is more, the rows before
+ * it are left as they are too, and S2D_CACHE_BAD_LENGTH is set.  q_start NULL:
+ * one token per sequence.
  * With heads rows per token of head_dim elements each: consecutive heads are
  * head_dim apart, tokens *_stride elements apart; all rows 16-byte aligned. */
 typedef struct S2dCacheAppend {

@@ -996,3 +996,35 @@ def test_append_of_starts_that_end_below_zero(torch, end):
     with pytest.raises(S2dError, match="out of range"):
         s.c.check()
     assert torch.all(wide == 5.0) and torch.equal(s.c.v.view(torch.int16), before.view(torch.int16))
+
+
+@pytest.mark.parametrize("prefix,n_seq", [(0, 3), (100, 3), (100, 300)])
+def test_rows_before_the_first_sequence_stay(torch, prefix, n_seq):
+    """q_start[0] above 0: reported by every call, and the rows below it, which are no sequence's, are left as they are, whether
+    parts are joined or not; the sequences' rows come out as they should."""
+    from fish_s2pro_b200 import S2dError
+    s = Case(torch, "bf16", 8, 2, 64, [130, 150, 70] * (n_seq // 3), [20] * n_seq, prefix, seed=46)
+    s.starts[0], s.tokens = 7, [13] + [20] * (n_seq - 1)
+    s.q_start = s.ints(s.starts)
+    out, lse = torch.full_like(s.q, 5.0), None
+    got, lse = s.attend(out=out)
+    assert torch.all(out[:7] == 5.0)
+    with pytest.raises(S2dError, match="out of range"):
+        s.c.check()
+    want, want_lse, _, spread = s.expected()
+    u = HALF_STEP["bf16"]
+    assert np.all(np.abs(out.double().cpu().numpy() - want)[7:] <= (u * (np.abs(want) + spread) + F32_TOL * 8)[7:])
+    assert np.all(np.abs(lse.double().cpu().numpy() - want_lse)[7:] <= F32_TOL * np.maximum(1, np.abs(want_lse[7:])))
+    T = s.q.shape[0]
+    kn = torch.randn(T, 2, 64, dtype=torch.bfloat16, device="cuda")
+    q = torch.full_like(s.q, 5.0)
+    past = torch.clamp(s.c.lengths - 40, min=0)
+    s.c.append(s.q, kn, kn, s.ints([0] * T), past, q_start=s.q_start, out=q)  # position 0: the queries as they are
+    with pytest.raises(S2dError, match="out of range"):
+        s.c.check()
+    assert torch.all(q[:7] == 5.0) and torch.equal(q[7:], s.q[7:])
+    for b in (0, 1, n_seq - 1):
+        at = [int(past[b]) + i for i in range(s.tokens[b])]
+        rows = torch.stack([s.c.v[int(s.table[b, j // PAGE]), :, j % PAGE] for j in at])
+        assert torch.equal(rows, kn[int(s.starts[b]): int(s.starts[b + 1])])
+    assert s.c.lengths.tolist() == [int(p) + n for p, n in zip(past, s.tokens)]
