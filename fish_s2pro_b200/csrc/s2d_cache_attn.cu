@@ -431,7 +431,8 @@ __global__ void __launch_bounds__(128) join_kernel(const S2dCacheView c, const S
     const int lane = threadIdx.x & 31;
     grid_dep_wait();
     grid_dep_launch();
-    if (id < (int64_t)first_token(a) * a.heads || id >= (int64_t)real_tokens(a, c.n_seq) * a.heads) return;
+    const int64_t from = first_token(a), to = real_tokens(a, c.n_seq);  // both loads under way together
+    if (id < from * a.heads || id >= to * a.heads) return;
     const int64_t tok = id / a.heads;
     const int head = (int)(id % a.heads);
     const Vec *part = reinterpret_cast<const Vec *>(p.part + id * p.parts * HD) + lane;

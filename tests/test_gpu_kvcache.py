@@ -1028,3 +1028,94 @@ def test_rows_before_the_first_sequence_stay(torch, prefix, n_seq):
         rows = torch.stack([s.c.v[int(s.table[b, j // PAGE]), :, j % PAGE] for j in at])
         assert torch.equal(rows, kn[int(s.starts[b]): int(s.starts[b + 1])])
     assert s.c.lengths.tolist() == [int(p) + n for p, n in zip(past, s.tokens)]
+
+
+class SharedPages:
+    """Long tables at little memory: every sequence's row draws its pages from one small pool, which attention only reads.  The
+    reference is the formula in float64 on the GPU, a sequence at a time."""
+
+    def __init__(self, torch, ty, H, G, D, lengths, max_pages, tokens=None, prefix_len=0, pool=70, seed=0):
+        from fish_s2pro_b200 import PagedKvCache
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        kv, B = torch.bfloat16 if ty == "bf16" else torch.float16, len(lengths)
+        counts = [1] * B if tokens is None else tokens
+        self.torch, self.ty, self.H, self.G, self.D, self.lengths, self.prefix_len = torch, ty, H, G, D, lengths, prefix_len
+        self.starts = np.concatenate([[0], np.cumsum(counts)]).tolist()
+        self.k, self.v = (torch.randn(pool, G, PAGE, D, generator=gen, device="cuda").to(kv) for _ in range(2))
+        self.table = torch.randint(0, pool, (B, max_pages), generator=gen, device="cuda", dtype=torch.int32)
+        self.prefix = torch.randint(0, pool, (-(-prefix_len // PAGE),), generator=gen, device="cuda", dtype=torch.int32)
+        self.q = (torch.randn(self.starts[-1], H, D, generator=gen, device="cuda") * 2).to(act_dtype(torch, ty))
+        self.mass0 = torch.rand(B, G, max_pages * PAGE, generator=gen, device="cuda")
+        self.mass, self.scale = self.mass0.clone(), 1 / math.sqrt(D)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        self.c = PagedKvCache(self.k, self.v, self.table, ints(lengths), mass=self.mass)
+        self.q_start = None if tokens is None else ints(self.starts)
+
+    def check(self, weigh=True):
+        torch, G, D, rep = self.torch, self.G, self.D, self.H // self.G
+        out, lse = self.c.attention(self.q, q_start=self.q_start, prefix_pages=self.prefix if self.prefix_len else None,
+                                    prefix_len=self.prefix_len, weigh=weigh, scale=self.scale, return_lse=True)
+        self.c.check()
+        u, want_mass, P = HALF_STEP[self.ty], self.mass0.double(), self.prefix_len
+        rows = lambda x, pages, n: x[pages.long()].permute(1, 0, 2, 3).reshape(G, -1, D)[:, :n].double()
+        most = float(self.v.abs().max())
+        for b, n in enumerate(self.lengths):
+            t0, t1 = self.starts[b], self.starts[b + 1]
+            if t1 == t0:
+                continue
+            k, v = (torch.cat([rows(x, self.prefix, P), rows(x, self.table[b], n)], 1) for x in (self.k, self.v))
+            s = torch.einsum("tgrd,gnd->tgrn", self.q[t0:t1].double().view(-1, G, rep, D), k) * self.scale
+            last = P + n - (t1 - t0) + torch.arange(t1 - t0, device="cuda")
+            s.masked_fill_((torch.arange(P + n, device="cuda") > last[:, None])[:, None, None], -math.inf)
+            w = torch.softmax(s, -1).nan_to_num(0.0)
+            want, spread = torch.einsum("tgrn,gnd->tgrd", w, v), torch.einsum("tgrn,gnd->tgrd", w, v.abs())
+            bound = u * want.abs() + (u if self.ty != "f32" else 0) * spread + F32_TOL * most
+            assert torch.all((out[t0:t1].double().view(want.shape) - want).abs() <= bound), b
+            want_lse, got = torch.logsumexp(s, -1), lse[t0:t1].double().view(s.shape[:-1])
+            seen = want_lse > -math.inf
+            assert torch.all((got - want_lse)[seen].abs() <= F32_TOL * want_lse[seen].abs().clamp(min=1)), b
+            assert torch.all(got[~seen] == -math.inf)
+            if weigh:
+                want_mass[b, :, :n] += w[..., P:].sum((0, 2))
+        assert torch.all((self.mass.double() - want_mass).abs() <= F32_TOL * want_mass.clamp(min=1))
+        beyond = torch.arange(self.mass.shape[2], device="cuda") >= torch.tensor(self.lengths, device="cuda")[:, None, None]
+        assert torch.all((self.mass == self.mass0) | ~beyond)
+
+
+def ragged_lengths(n_seq, most, seed):
+    rng = np.random.default_rng(seed)
+    x = rng.integers(0, most + 1, n_seq)
+    x[:4] = [most, 0, 1, most - 1]
+    return x.tolist()
+
+
+@pytest.mark.parametrize("ty,H,G,D,n_seq,max_pages,prefix", [
+    ("f16", 32, 8, 128, 64, 128, 0),      # tables of 8,192 slots: more CTAs a sequence, so that two of them fit an SM
+    ("f32", 32, 8, 128, 64, 128, 300),
+    ("bf16", 32, 8, 128, 64, 100, 65),
+    ("f16", 32, 8, 128, 80, 128, 0),      # one CTA a (sequence, KV head), which keeps up to 8,192 scores
+    ("f32", 32, 8, 128, 80, 128, 200),
+    ("bf16", 64, 8, 128, 80, 64, 300),    # eight heads a group: more outputs than threads, behind prefix parts
+    ("f16", 64, 8, 64, 80, 64, 1000),
+    ("f16", 8, 1, 128, 2, 606, 300),      # eight CTAs a sequence: the longest table whose scores fit, and a longer one
+    ("f16", 8, 1, 128, 2, 608, 300),
+    ("f32", 8, 1, 128, 1, 608, 0),
+    ("bf16", 8, 1, 64, 2, 740, 0),
+    ("f32", 8, 2, 64, 3, 1600, 130),      # weights from scores computed again
+    ("f16", 32, 8, 128, 80, 170, 64),
+    ("bf16", 32, 2, 128, 9, 40, 500),     # sixteen heads a group
+])
+def test_single_tokens_that_weigh_in_long_tables(torch, ty, H, G, D, n_seq, max_pages, prefix):
+    lengths = ragged_lengths(n_seq, max_pages * PAGE, n_seq + max_pages) if n_seq > 3 else [max_pages * PAGE - 5, 700, 0][:n_seq]
+    SharedPages(torch, ty, H, G, D, lengths, max_pages, prefix_len=prefix, seed=max_pages).check()
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [-0.125, 0.0, -0.0, 1e-30])
+@pytest.mark.parametrize("tokens", [None, [3, 0, 150, 40]])
+def test_negative_and_zero_scales(torch, ty, scale, tokens):
+    """The maximum of scale * q . k where the scale is negative is the minimum of q . k; scale 0 weighs every position alike."""
+    for H, G, D, prefix in ((8, 2, 64, 200), (32, 8, 128, 0), (16, 1, 128, 70)):
+        s = SharedPages(torch, ty, H, G, D, [130, 700, 150, 64], 12, tokens, prefix, seed=D)
+        s.scale = scale
+        s.check()
