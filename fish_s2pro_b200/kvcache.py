@@ -114,6 +114,24 @@ def cache_lib() -> ctypes.CDLL:
     return _bound
 
 
+_status_streams = {}  # device index -> the stream that status words are made on
+
+
+def _status_word(torch, device):
+    """A clear status word, at once and whatever the current stream is at: the cache may next be used on another one.  Its memory
+    is the status stream's, so that a word freed while a call still runs elsewhere can only become another word."""
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(1, dtype=torch.int32, device=device)  # cleared by each replay
+        stream = _status_streams.get(device.index)
+        if stream is None:
+            stream = _status_streams[device.index] = torch.cuda.Stream(device)
+        with torch.cuda.stream(stream):
+            word = torch.zeros(1, dtype=torch.int32, device=device)
+        stream.synchronize()
+        return word
+
+
 class PagedKvCache:
     """One layer's paged cache over the caller's tensors, which it keeps and
     writes in place.
@@ -165,7 +183,7 @@ class PagedKvCache:
         self._types = {k.dtype: 1 if k.dtype == torch.float16 else 30}
         if k.dtype == torch.float16:
             self._types[torch.float32] = 0
-        self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._status = _status_word(torch, self.device)
         self._view = _View(
             k.data_ptr(), v.data_ptr(), k.stride(0) if self.n_pages > 1 else max(k.stride(0), self.kv_heads * PAGE * self.head_dim),
             k.stride(1) if self.kv_heads > 1 else PAGE * self.head_dim, page_table.data_ptr(),

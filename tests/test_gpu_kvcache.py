@@ -1119,3 +1119,43 @@ def test_negative_and_zero_scales(torch, ty, scale, tokens):
         s = SharedPages(torch, ty, H, G, D, [130, 700, 150, 64], 12, tokens, prefix, seed=D)
         s.scale = scale
         s.check()
+
+
+def test_a_new_cache_on_another_stream(torch):
+    """A cache made on a busy stream and used on another: its status word is clear there too, and what it reports is not cleared
+    when the first stream gets that far."""
+    from fish_s2pro_b200 import PagedKvCache, S2dError
+    s = Case(torch, "f16", 8, 2, 64, [30, 40], None, 0, seed=48)
+    bad = s.ints([30, -1])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for lengths, fails in ((s.c.lengths, False), (bad, True)):
+        trash = [torch.full((1,), -1, dtype=torch.int32, device="cuda") for _ in range(64)]  # what a new word may hold
+        torch.cuda.synchronize()
+        del trash
+        torch.cuda._sleep(400_000_000)
+        c = PagedKvCache(s.c.k, s.c.v, s.c.page_table, lengths)
+        with torch.cuda.stream(side):
+            c.attention(s.q)
+            side.synchronize()
+            torch.cuda.synchronize()
+            if fails:
+                with pytest.raises(S2dError, match="out of range"):
+                    c.check()
+            else:
+                c.check()
+    torch.cuda.synchronize()
+
+
+def test_a_cache_made_while_capturing(torch):
+    """A function that makes its cache can be captured: the word is cleared at each replay, and the results are the eager ones."""
+    from fish_s2pro_b200 import PagedKvCache
+    s = Case(torch, "f16", 8, 2, 64, [30, 40], None, 0, seed=49)
+    want = PagedKvCache(s.c.k, s.c.v, s.c.page_table, s.c.lengths).attention(s.q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c = PagedKvCache(s.c.k, s.c.v, s.c.page_table, s.c.lengths)
+        out = c.attention(s.q)
+    g.replay()
+    c.check()
+    assert torch.equal(out, want)
