@@ -676,6 +676,9 @@ extern "C" int32_t s2d_cache_status(const S2dCacheView *view, int32_t *bits, voi
     DeviceGuard guard(view->device);
     cudaError_t e = guard.error;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (!e) e = cudaStreamIsCapturing(s, &capture);
+    if (!e && capture != cudaStreamCaptureStatusNone) return cache_fail(err, err_cap, S2D_EINVAL, "the status cannot be read while the stream is captured");
     if (!e) e = cudaMemcpyAsync(bits, view->status, sizeof(int32_t), cudaMemcpyDeviceToHost, s);
     if (!e) e = cudaMemsetAsync(view->status, 0, sizeof(int32_t), s);
     if (!e) e = cudaStreamSynchronize(s);

@@ -352,7 +352,7 @@ class PagedKvCache:
     def check(self) -> None:
         """Wait for the current stream and raise S2dError if a call met a page
         id outside the pool, a length, past or q_start out of range, or a full
-        sequence since the last check."""
+        sequence since the last check.  Not inside a capture."""
         bits = _c.c_int32()
         self._call(self._lib.s2d_cache_status(self._view_ref, _c.byref(bits), self._stream(), self._err, 256))
         if bits.value:

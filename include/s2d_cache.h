@@ -172,7 +172,9 @@ int32_t s2d_cache_evict_workspace(const S2dCacheView *view, const S2dCacheEvict 
  * Needs the view's positions and mass. */
 int32_t s2d_cache_evict(const S2dCacheView *view, const S2dCacheEvict *args, void *stream, char *err, size_t err_cap);
 
-/* Waits for `stream`, returns the status word in *bits and clears it. */
+/* Waits for `stream`, returns the status word in *bits and clears it: not
+ * while `stream` is captured (S2D_EINVAL), and a bit that a call on another
+ * stream sets meanwhile may be cleared unread. */
 int32_t s2d_cache_status(const S2dCacheView *view, int32_t *bits, void *stream, char *err, size_t err_cap);
 
 #ifdef __cplusplus

@@ -1159,3 +1159,19 @@ def test_a_cache_made_while_capturing(torch):
     g.replay()
     c.check()
     assert torch.equal(out, want)
+
+
+def test_check_while_capturing_is_refused(torch):
+    """The check waits, which a capture cannot: it says so and leaves the capture as it is."""
+    from fish_s2pro_b200 import S2dError
+    s = Case(torch, "f16", 8, 2, 64, [30, 40], None, 70, seed=50)
+    want, _ = s.attend()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = s.attend()
+        with pytest.raises(S2dError, match="captur") as e:
+            s.c.check()
+        assert e.value.code == -1
+    g.replay()
+    s.c.check()
+    assert torch.equal(out, want)
