@@ -175,8 +175,8 @@ class PagedKvCache:
         if v.device != self.device:
             raise _bad("every buffer must be on the cache's device")
         for name, t in (("k", k), ("v", v), ("mass", mass)):
-            if t is not None:
-                self._no_grad(name, t)
+            if t is not None and t.requires_grad:
+                self._no_grad(name)
         self.k, self.v, self.page_table, self.lengths, self.positions, self.mass = k, v, page_table, lengths, positions, mass
         self.dtype = k.dtype
         self._scale = 1.0 / math.sqrt(self.head_dim)
@@ -216,17 +216,17 @@ class PagedKvCache:
             raise _bad(f"the heads of a token of {name} must be contiguous")
         if t.get_device() != self._index:
             raise _bad(f"{name} must be on {self.device}")
-        self._no_grad(name, t)
+        if t.requires_grad:
+            self._no_grad(name)
         return t.data_ptr(), step if s[0] > 1 else s[1] * s[2]
 
-    def _no_grad(self, name, t):
-        if t.requires_grad and self._torch.is_grad_enabled():
+    def _no_grad(self, name):
+        if self._torch.is_grad_enabled():
             raise _bad(f"{name} requires a gradient: the cache operators have no backward pass")
 
     def _gain(self, name, t):
-        if t is None:
-            return 0
-        self._no_grad(name, t)
+        if t.requires_grad:
+            self._no_grad(name)
         return self._dense(name, t, self._torch.float32, (self.head_dim,))
 
     def _like_q(self, q, out):
@@ -283,9 +283,10 @@ class PagedKvCache:
         if k.shape[0] != tokens or v.shape[0] != tokens:
             raise _bad("q, k and v must have the same tokens")
         out, op, os_ = self._like_q(q, out)
-        a = _pack_append(qp, kp, vp, qs, ks, vs, op, os_, self._gain("q_norm", q_norm), self._gain("k_norm", k_norm),
-                         self._ints("pos", pos, (tokens,)), self._ints("past", past, (self.n_seq,)), self._starts(q_start, tokens),
-                         tokens, q.shape[1], ty, eps, rope_base)
+        a = _pack_append(qp, kp, vp, qs, ks, vs, op, os_, 0 if q_norm is None else self._gain("q_norm", q_norm),
+                         0 if k_norm is None else self._gain("k_norm", k_norm), self._ints("pos", pos, (tokens,)),
+                         self._ints("past", past, (self.n_seq,)), self._starts(q_start, tokens), tokens, q.shape[1], ty, eps,
+                         rope_base)
         self._call(self._lib.s2d_cache_append(self._view_ref, a, self._stream(), self._err, 256))
         return out
 
