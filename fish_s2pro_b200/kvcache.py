@@ -27,6 +27,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+import threading
 from typing import Optional
 
 from .s2d import S2dError, lib
@@ -114,22 +115,25 @@ def cache_lib() -> ctypes.CDLL:
     return _bound
 
 
-_status_streams = {}  # device index -> the stream that status words are made on
+_words, _words_lock = {}, threading.Lock()  # device index -> (clear status words, how many of them are taken)
 
 
 def _status_word(torch, device):
-    """A clear status word, at once and whatever the current stream is at: the cache may next be used on another one.  Its memory
-    is the status stream's, so that a word freed while a call still runs elsewhere can only become another word."""
-    with torch.cuda.device(device):
-        if torch.cuda.is_current_stream_capturing():
-            return torch.zeros(1, dtype=torch.int32, device=device)  # cleared by each replay
-        stream = _status_streams.get(device.index)
-        if stream is None:
-            stream = _status_streams[device.index] = torch.cuda.Stream(device)
-        with torch.cuda.stream(stream):
-            word = torch.zeros(1, dtype=torch.int32, device=device)
-        stream.synchronize()
-        return word
+    """A status word that is clear whatever the current stream is at, as the cache may next be used on another one, and that no
+    other cache has had, as a call of one that is gone may still be running.  Words are cleared in blocks, so that few caches
+    wait for it."""
+    with _words_lock:
+        block, taken = _words.get(device.index, (None, 0))
+        if block is None or taken == block.shape[0]:
+            with torch.cuda.device(device):
+                if torch.cuda.is_current_stream_capturing():
+                    return torch.zeros(1, dtype=torch.int32, device=device)  # cleared by each replay
+                stream = torch.cuda.Stream(device)
+                with torch.cuda.stream(stream):
+                    block, taken = torch.zeros(1024, dtype=torch.int32, device=device), 0
+                stream.synchronize()
+        _words[device.index] = block, taken + 1
+        return block[taken:taken + 1]
 
 
 class PagedKvCache:

@@ -1161,6 +1161,21 @@ def test_a_cache_made_while_capturing(torch):
     assert torch.equal(out, want)
 
 
+def test_status_words_of_many_caches(torch):
+    """Words come in blocks: what one cache reports no other does, past the end of a block too."""
+    from fish_s2pro_b200 import PagedKvCache, S2dError
+    s = Case(torch, "f16", 8, 2, 64, [30, 40], None, 0, seed=51)
+    bad = s.ints([30, -1])
+    caches = [PagedKvCache(s.c.k, s.c.v, s.c.page_table, bad if i % 500 == 7 else s.c.lengths) for i in range(1100)]
+    for c in caches:
+        c.attention(s.q)
+    for i, c in enumerate(caches):
+        if i % 500 == 7:
+            with pytest.raises(S2dError, match="out of range"):
+                c.check()
+        c.check()
+
+
 def test_check_while_capturing_is_refused(torch):
     """The check waits, which a capture cannot: it says so and leaves the capture as it is."""
     from fish_s2pro_b200 import S2dError
