@@ -93,7 +93,7 @@ __device__ __forceinline__ void store_pack(T *to, const float (&x)[N]) {
 // with shuffles.
 //
 // HBM bound: every row is read and written once; 36,900 bf16 tokens of 32 and 8
-// heads of 128 take 168 to 175 us, 5.2 to 5.4 TB/s.  What a token needs before its rows (four
+// heads of 128 take 168 to 180 us, 5.1 to 5.4 TB/s.  What a token needs before its rows (four
 // dependent loads) is paid once for the group (8 tokens a group: 177 us, 4:
 // 196), and kAhead rows of a lane are under way at once (2, with more blocks:
 // 184; 8, with fewer: 192).

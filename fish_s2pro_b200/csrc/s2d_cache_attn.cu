@@ -519,9 +519,12 @@ size_t token_smem(const S2dCacheView &c, const AttnPlan &p, int pitch) {
            sizeof(float) * (size_t)std::min(p.rep, 8) * pitch;
 }
 // Floats between the rows of kept scores, 0 if none are kept; + 8 spreads the
-// rows over the banks.  Kept wherever they fit: 64 sequences of up to 4,096
-// slots 128 us, computed again from the keys 212; of up to 12,288, which leaves
-// one CTA an SM, 431 and 579.
+// rows over the banks.  Kept where they fit the splits that make_plan has
+// chosen: 64 sequences of up to 4,096 slots 128 us, computed again from the keys
+// 212; of up to 12,288, which leaves one CTA an SM, 431 and 579.  No splits are
+// added for longer tables (beyond 19,400 slots of 64 sequences, 9,600 of 128, at
+// 8 KV heads of 128), where the keys are read twice: 64 sequences that fill
+// tables of 32,768 take 1,932 us, 1,013 without weights.
 int score_pitch(const S2dCacheView &c, const S2dCacheAttention &a, const AttnPlan &p) {
     if (!a.weigh || p.rep > 8) return 0;
     const int chunks = c.max_pages * (kCachePage / 16), pitch = (chunks + p.own_splits - 1) / p.own_splits * 16 + 8;
@@ -558,7 +561,9 @@ void make_plan(const S2dCacheView &c, const S2dCacheAttention &a, AttnPlan &p, s
         p.parts = p.prefix_splits;
         // Kept scores: twice the CTAs where two of them then fit an SM and one
         // does not leave room (64 sequences in tables of 8,192 slots, filled to
-        // 2,048 and more 300 us and 235, to 100 and more 56 and 59).
+        // 2,048 and more 300 us and 235, to 100 and more 56 and 59).  Once only:
+        // 128 sequences in such tables, which four splits would need, stay at
+        // one CTA an SM (801 us, 527 without weights).
         auto two_fit = [&](int splits) {
             AttnPlan t = p;
             t.own_splits = splits;

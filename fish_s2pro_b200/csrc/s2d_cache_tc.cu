@@ -15,7 +15,7 @@
 // the longest first; one item's first loads run under the last one's epilogue.
 //
 // What bounds it: bf16 prompts of 500 to 2,048 tokens behind 2,000 positions (32
-// and 8 heads of 128) take 254 us, 864 TFLOP/s; the products alone take 200,
+// and 8 heads of 128) take 255 us, 860 TFLOP/s; the products alone take 200,
 // the softmax alone 219 (without its exponentials 177: TMEM reads, the
 // hand-overs, the items' starts and ends), so the two row tiles overlap most
 // of the smaller one.  S in halves of 64 positions, one under the other's
@@ -1010,8 +1010,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // Every wait is bounded, as above.
 //
 // Bound by latency: 8 sequences of 1,968 to 8,160 slots, 32 tokens each, 8 KV
-// heads of 128 take 36 us, of which reading the keys is 13.  The whole call: 106
-// us with 2 tiles a CTA, 99 to 103 with 4 to 16.
+// heads of 128 take 37 us, of which reading the keys is 13.  The whole call: 106
+// us with 2 tiles a CTA, 99 to 104 with 4 to 16.
 constexpr int kWeighTiles = 8, kWeighThreads = 320;
 
 template <typename Q, int HD>

@@ -37,14 +37,24 @@
  * word.
  *
  * Limits (S2D_EINVAL beyond): head_dim 64 or 128, heads / kv_heads <= 16,
- * kv_heads <= 1024, n_seq <= 65,535, max_pages <= 2^18, prefix_len <= 2^24,
- * tokens * heads <= 2^26.
+ * kv_heads <= 1024, n_seq <= 65,535, max_pages <= 2^18; of attention, prefix_len
+ * <= 2^24 and tokens * heads <= 2^26.
+ *
+ * Precision: norms, rotations, softmax statistics, lse and mass are f32, and
+ * results are rounded to their type once.  Attention with f32 queries takes
+ * queries and softmax weights as f16 pairs of about 22 bits: its results are
+ * within 2e-5 of the largest value.  With f16 or bf16 queries the weights of
+ * packed tokens (q_start), and those of a prefix's positions, are rounded to that
+ * type before they meet the values, by up to half a step each, which adds on
+ * average as much again as the result's own rounding; the own slots of single
+ * tokens are weighed without it.  f32 queries avoid it at twice the products.
  *
  * Pages may be shared by sequences that only read them.  Append and evict
  * write their sequence's pages, so a page that they reach belongs to one
  * sequence.  Key rows and value rows that no token may see yet enter with
  * weight 0, so an infinity or a NaN in the value row of a slot can reach the
- * sequence's earlier tokens of the same call; slots at and past the length
+ * sequence's earlier tokens of the same call (0 times it is a NaN, as in a
+ * product over all slots); slots at and past the length
  * never count, whatever they hold.
  */
 #ifndef S2D_CACHE_H
