@@ -1190,3 +1190,108 @@ def test_check_while_capturing_is_refused(torch):
     g.replay()
     s.c.check()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("ty,tokens", [("f32", None), ("bf16", [40, 3, 0, 130])])
+def test_heads_apart_in_the_pool(torch, ty, tokens):
+    """A pool laid out [page][head][K | V][64][D]: a head stride that is not the rows' size."""
+    from fish_s2pro_b200 import PagedKvCache
+    s = SharedPages(torch, ty, 8, 4, 64, [200, 3, 0, 150], 4, tokens, 100, seed=3)
+    pool = torch.stack([s.k, s.v], 2)
+    s.c = PagedKvCache(pool[:, :, 0], pool[:, :, 1], s.table, s.c.lengths, mass=s.mass)
+    s.check()
+
+
+@pytest.mark.parametrize("ty,H,G,tokens", [("f16", 1024, 1024, None), ("bf16", 600, 300, [60, 5])])
+def test_many_kv_heads(torch, ty, H, G, tokens):
+    SharedPages(torch, ty, H, G, 64, [100, 37], 3, tokens, 70, pool=8, seed=1).check()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_the_most_sequences(torch, packed):
+    """65,535 sequences of up to a page, each with one token: appended, and weighed over what they hold."""
+    from fish_s2pro_b200 import PagedKvCache
+    B, G, D = 65535, 2, 64
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(B, G, PAGE, D, generator=gen, device="cuda").half() for _ in range(2))
+    table = torch.randperm(B, generator=gen, device="cuda").to(torch.int32).view(B, 1)
+    past = torch.randint(0, PAGE, (B,), generator=gen, device="cuda", dtype=torch.int32)
+    lengths, mass = torch.zeros_like(past), torch.zeros(B, G, PAGE, device="cuda")
+    q, kn, vn = (torch.randn(B, n, D, generator=gen, device="cuda").half() for n in (4, G, G))
+    starts = torch.arange(B + 1, device="cuda", dtype=torch.int32) if packed else None
+    c = PagedKvCache(k, v, table, lengths, mass=mass)
+    qr = c.append(q, kn, vn, torch.zeros_like(past), past, q_start=starts)  # position 0: nothing turns
+    at = table[:, 0].long()
+    assert torch.equal(lengths, past + 1) and torch.equal(qr, q)
+    assert torch.equal(k[at, :, past.long()], kn) and torch.equal(v[at, :, past.long()], vn)
+    out, lse = c.attention(qr, q_start=starts, weigh=True, return_lse=True)
+    c.check()
+    for b0 in range(0, B, 8192):
+        b = slice(b0, min(B, b0 + 8192))
+        s = torch.einsum("bgrd,bgnd->bgrn", q[b].double().view(-1, G, 2, D), k[at[b]].double()) / math.sqrt(D)
+        s.masked_fill_(torch.arange(PAGE, device="cuda") >= lengths[b][:, None, None, None], -math.inf)
+        w = s.softmax(-1)
+        rows = v[at[b]].double()
+        want, spread = torch.einsum("bgrn,bgnd->bgrd", w, rows).view(-1, 4, D), torch.einsum("bgrn,bgnd->bgrd", w, rows.abs()).view(-1, 4, D)
+        bound = HALF_STEP["f16"] * (want.abs() + spread) + F32_TOL * float(v.abs().max())
+        assert torch.all((out[b].double() - want).abs() <= bound)
+        assert torch.all((lse[b].double() - torch.logsumexp(s, -1).view(-1, 4)).abs() <= 6 * F32_TOL)  # of at most 6
+        assert torch.all((mass[b].double() - w.sum(2)).abs() <= 2 * F32_TOL)
+
+
+@pytest.mark.parametrize("n", [5, 1000, 1 << 20, 1 << 24])
+@pytest.mark.parametrize("packed", [False, True])
+def test_the_longest_tables(torch, n, packed):
+    """Tables of 2^18 pages, hardly filled and full, which repeat 64 pages: the weights of a slot's copies are alike."""
+    from fish_s2pro_b200 import PagedKvCache
+    pages, D, H = 1 << 18, 64, 8
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    k, v = (torch.randn(64, 1, PAGE, D, generator=gen, device="cuda").half() for _ in range(2))
+    table = (torch.arange(pages, device="cuda") % 64).to(torch.int32).view(1, pages)
+    q = torch.randn(1, H, D, generator=gen, device="cuda").half()
+    mass = torch.zeros(1, 1, pages * PAGE, device="cuda")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    c = PagedKvCache(k, v, table, ints([n]), mass=mass)
+    out, lse = c.attention(q, q_start=ints([0, 1]) if packed else None, weigh=True, return_lse=True)
+    c.check()
+    period = min(n, 4096)
+    s = (q[0].double() @ k.reshape(-1, D)[:period].double().T) / math.sqrt(D)
+    w = s.softmax(-1)
+    want, spread = w @ v.reshape(-1, D)[:period].double(), w @ v.reshape(-1, D)[:period].double().abs()
+    bound = HALF_STEP["f16"] * (want.abs() + spread) + F32_TOL * float(v.abs().max())
+    assert torch.all((out[0].double() - want).abs() <= bound)
+    assert torch.all((lse[0].double() - torch.logsumexp(s, -1) - math.log(n / period)).abs() <= 20 * F32_TOL)  # of at most 20
+    got = mass[0, 0, :n].double().view(-1, period) if n >= period else mass[0, 0, :n].double()[None]
+    assert torch.all((got * (n // period) - w.sum(0)).abs() <= F32_TOL)
+    assert torch.all(mass[0, 0, n:] == 0)
+
+
+def test_replays_of_other_batches(torch):
+    """A captured ragged call, replayed after the starts, the lengths and the queries have changed on the device: what an eager
+    call of the same sizes gives, with fewer tokens than it was captured for."""
+    s = SharedPages(torch, "bf16", 16, 8, 64, [300, 700, 130, 64], 12, [40, 7, 60, 0], 900, seed=52)
+    first = [x.clone() for x in (s.q_start, s.c.lengths, s.q)]
+    g = torch.cuda.CUDAGraph()
+    s.check(weigh=False)  # and warm
+    with torch.cuda.graph(g):
+        out, lse = s.c.attention(s.q, q_start=s.q_start, prefix_pages=s.prefix, prefix_len=900, weigh=True, return_lse=True)
+    for starts, lengths in (([0, 1, 50, 90, 107], [1, 600, 700, 17]), ([0, 0, 0, 100, 100], [5, 0, 768, 3]), ([0, 10, 20, 30, 40], [768] * 4)):
+        s.q_start.copy_(torch.tensor(starts, dtype=torch.int32))
+        s.c.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        s.q.normal_()
+        s.mass.copy_(s.mass0)
+        out.fill_(5.0)
+        g.replay()
+        got = [out.clone(), lse.clone(), s.mass.clone()]
+        s.mass.copy_(s.mass0)
+        want = s.c.attention(s.q, q_start=s.q_start, prefix_pages=s.prefix, prefix_len=900, weigh=True, return_lse=True)
+        n = starts[-1]
+        assert torch.equal(got[0][:n], want[0][:n]) and torch.equal(got[1][:n], want[1][:n]) and torch.equal(got[2], s.mass)
+        assert torch.all(got[0][n:] == 5.0)
+        s.mass.copy_(s.mass0)
+        s.starts, s.lengths = starts, lengths
+        s.check()
+    for x, y in zip((s.q_start, s.c.lengths, s.q), first):
+        x.copy_(y)
+    g.replay()
+    s.c.check()
