@@ -43,7 +43,8 @@
  * Precision: norms, rotations, softmax statistics, lse and mass are f32, and
  * results are rounded to their type once.  Attention with f32 queries takes
  * queries and softmax weights as f16 pairs of about 22 bits: its results are
- * within 2e-5 of the largest value.  With f16 or bf16 queries the weights of
+ * within 2e-5 of the largest value over up to 2^18 positions, for scores of up
+ * to some tens (a score is right to some 2^-22 of itself).  With f16 or bf16 queries the weights of
  * packed tokens (q_start), and those of a prefix's positions, are rounded to that
  * type before they meet the values, by up to half a step each, which adds on
  * average as much again as the result's own rounding; the own slots of single
